@@ -258,8 +258,9 @@ def _run_evict(s):
         from slimkv_amd import cache_ops
         rows, counts = cache_ops.select_rows(s['weights'], case['keep'], lengths=s['lengths'], sink=case['sink'],
                                              recent=case['recent'])
-        place = {} if 'k' in s else {'pages': s['pages'], 'table': s['table'], 'status': s['status']}
-        k, v, w = cache_ops.compact_rows(rows, counts, s.get('k'), s.get('v'), weights=s['weights'], **place)
+        place = {} if 'k' in s else {'pages': s['pages'], 'table': s['table']}
+        k, v, w = cache_ops.compact_rows(rows, counts, s.get('k'), s.get('v'), weights=s['weights'], status=s['status'],
+                                          **place)
         return rows, counts, k, v, w
     B, H, N, keep = case['batch'], case['heads'], case['keys'], case['keep']
     n = s['lengths'].long()[:, None]
@@ -315,7 +316,7 @@ def exact(case, seed):
         """Rows [n, D] of one head as the cache holds them."""
         n = lengths[b]
         if 'k' in s:
-            return s['kv'[which]][b, :n, h]
+            return s['v' if which else 'k'][b, :n, h]
         i = torch.arange(n, device=DEV)
         return s['pages'][s['table'][b, i // case['block']], i % case['block'], which, h]
 
