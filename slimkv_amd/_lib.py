@@ -231,6 +231,54 @@ PagedStepRowsArgs = _struct('slimkv_paged_step_rows_args', [
     ('status', c_ptr),
 ])
 
+# include/slimkv/cache_ops.h
+CacheRows = _struct('slimkv_cache_rows', [
+    ('k', c_ptr), *_i64s('k_sb', 'k_sn', 'k_sh'),
+    ('v', c_ptr), *_i64s('v_sb', 'v_sn', 'v_sh'),
+    ('table', c_ptr), *_i64s('t_sb', 't_cols', 'num_blocks', 'block_size'),
+    ('lengths', c_ptr), ('keys', c_i64), ('status', c_ptr),
+])
+
+TreeAttentionArgs = _struct('slimkv_tree_attention_args', [
+    ('cache', CacheRows),
+    ('q', c_ptr), *_i64s('q_sb', 'q_sl', 'q_sh'),
+    ('draft_k', c_ptr), *_i64s('dk_sb', 'dk_sn', 'dk_sh'),
+    ('draft_v', c_ptr), *_i64s('dv_sb', 'dv_sn', 'dv_sh'),
+    ('mask', c_ptr), *_i64s('m_sb', 'm_sl'),
+    ('out', c_ptr), *_i64s('o_sb', 'o_sl', 'o_sh'),
+    ('lse', c_ptr),
+    *_i64s('batch', 'drafted', 'heads', 'kv_heads', 'head_dim'),
+    ('scale', c_f64), ('dtype', c_i32),
+])
+
+AttentionWeightsArgs = _struct('slimkv_attention_weights_args', [
+    ('cache', CacheRows),
+    ('q', c_ptr), *_i64s('q_sb', 'q_sl', 'q_sh'),
+    ('lse', c_ptr), *_i64s('l_sb', 'l_sh', 'l_sl'),
+    ('previous', c_ptr), *_i64s('p_sb', 'p_sh'),
+    ('out', c_ptr), *_i64s('w_sb', 'w_sh'),
+    *_i64s('batch', 'queries', 'heads', 'kv_heads', 'head_dim'),
+    ('scale', c_f64), ('causal', c_i32), ('dtype', c_i32),
+])
+
+SelectRowsArgs = _struct('slimkv_select_rows_args', [
+    ('weights', c_ptr), *_i64s('w_sb', 'w_sh'),
+    ('lengths', c_ptr), ('rows', c_ptr), ('counts', c_ptr),
+    *_i64s('batch', 'heads', 'keys', 'keep', 'sink', 'recent'),
+])
+
+CompactRowsArgs = _struct('slimkv_compact_rows_args', [
+    ('cache', CacheRows),
+    ('rows', c_ptr), *_i64s('r_sb', 'r_sh'),
+    ('counts', c_ptr),
+    ('out_k', c_ptr), *_i64s('ok_sb', 'ok_sn', 'ok_sh'),
+    ('out_v', c_ptr), *_i64s('ov_sb', 'ov_sn', 'ov_sh'),
+    ('weights', c_ptr), *_i64s('w_sb', 'w_sh'),
+    ('out_weights', c_ptr), *_i64s('ow_sb', 'ow_sh'),
+    *_i64s('weight_heads', 'weight_keys', 'batch', 'kv_heads', 'head_dim', 'keep'),
+    ('in_place', c_i32), ('dtype', c_i32),
+])
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     'slimkv_last_error': (ctypes.c_char_p, []),
@@ -279,9 +327,19 @@ SIGNATURES = {
     'slimkv_beacon_pages': (ctypes.c_int, [ctypes.POINTER(BeaconPagesArgs), c_ptr]),
     'slimkv_raw_pages': (ctypes.c_int, [ctypes.POINTER(RawPagesArgs), c_ptr]),
     'slimkv_paged_step_rows': (ctypes.c_int, [ctypes.POINTER(PagedStepRowsArgs), c_ptr]),
+    # include/slimkv/cache_ops.h
+    'slimkv_cache_abi_version': (ctypes.c_int, []),
+    'slimkv_tree_attention_workspace': (ctypes.c_size_t, [ctypes.POINTER(TreeAttentionArgs)]),
+    'slimkv_tree_attention': (ctypes.c_int, [ctypes.POINTER(TreeAttentionArgs), c_ptr, ctypes.c_size_t, c_ptr]),
+    'slimkv_attention_weights_workspace': (ctypes.c_size_t, [ctypes.POINTER(AttentionWeightsArgs)]),
+    'slimkv_attention_weights': (ctypes.c_int, [ctypes.POINTER(AttentionWeightsArgs), c_ptr, ctypes.c_size_t, c_ptr]),
+    'slimkv_select_rows_workspace': (ctypes.c_size_t, [ctypes.POINTER(SelectRowsArgs)]),
+    'slimkv_select_rows': (ctypes.c_int, [ctypes.POINTER(SelectRowsArgs), c_ptr, ctypes.c_size_t, c_ptr]),
+    'slimkv_compact_rows': (ctypes.c_int, [ctypes.POINTER(CompactRowsArgs), c_ptr]),
 }
 
 ABI_VERSION = 16
+CACHE_ABI_VERSION = 1          # include/slimkv/cache_ops.h
 
 STAGE_PROLOGUE, STAGE_ATTEND, STAGE_COMBINE, STAGE_ALL = 1, 2, 4, 7
 NOALLOC_SCRATCH_BYTES = 64 << 20
@@ -356,6 +414,9 @@ def lib():
         fn.argtypes = argtypes
     if handle.slimkv_abi_version() != ABI_VERSION:
         raise ImportError(f'{path} has ABI {handle.slimkv_abi_version()}, expected {ABI_VERSION}')
+    if handle.slimkv_cache_abi_version() != CACHE_ABI_VERSION:
+        raise ImportError(f'{path} has cache operator ABI {handle.slimkv_cache_abi_version()}, '
+                          f'expected {CACHE_ABI_VERSION}')
     return handle
 
 

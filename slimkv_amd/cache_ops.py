@@ -1,0 +1,356 @@
+"""Operators over a full-width K/V cache beside its decode: attention for a tree
+of drafted tokens, the attention weight that its rows gather, and eviction by it.
+
+    tree_attention     every drafted token over the cached rows and its ancestors
+    attention_weights  the weight each cached row gets from a step's queries
+    select_rows        the rows that a smaller cache keeps by that weight
+    compact_rows       those rows' K, V and weights moved to the front
+
+A cache is given as dense rows k, v [B, N, Hkv, D] or as raw pages
+[blocks, block, 2, Hkv, D] (RawPages' format) with a block table [B, cols] int64;
+`lengths` [B] int32 are the rows each sequence holds (default: all N).  Element
+types bf16 and fp16 (one for all tensors of a call), head_dim 64 or 128, keys
+rotated.  Cache rows start on 16-byte boundaries.
+
+A speculative step over a bounded cache: tree_attention gives the drafted
+tokens' outputs and LSEs; the accepted path's K/V rows are appended to the
+cache (RawPages.write, kernels.raw_pages); attention_weights adds that path's
+attention to the rows' weights; when a sequence passes its budget select_rows
+and compact_rows bring it back.  Rows read through a block table follow torch's
+indexing rules: an entry outside the pool raises IndexError after the call (one
+host synchronisation), or is left in the caller's device int32 `status` word
+(graph capture, serving loops; kernels.check_status).  The operators have no
+gradients and raise ValueError where one would be recorded.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .kernels import _ptr, _status_word, _workspace, check_status
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+
+
+def _common(name, *tensors):
+    """One device for every tensor, no gradient to record."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f'{name} needs device tensors (no CPU path)')
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f'{name}: tensors on {device} and {t.device}')
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f'{name} records no gradient: detach the inputs or run it under torch.no_grad()')
+    return device
+
+
+def _dtype(name, *tensors):
+    kind = tensors[0].dtype
+    if kind not in _DTYPES or any(t is not None and t.dtype is not kind for t in tensors):
+        raise ValueError(f'{name}: expected bfloat16 or float16 for every tensor, found '
+                         f'{[t.dtype for t in tensors if t is not None]}')
+    return _DTYPES[kind]
+
+
+def _rows16(t):
+    """t, or a copy where its rows do not start on 16-byte boundaries."""
+    good = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
+        all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride()))
+    return t if good else t.clone(memory_format=torch.contiguous_format)
+
+
+def _span(t):
+    """First and last byte address of t's elements."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + last * t.element_size() + t.element_size()
+
+
+def _overlap(a, b):
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _lengths(name, lengths, batch):
+    if lengths is None:
+        return None
+    if lengths.dtype is not torch.int32 or lengths.shape != (batch,):
+        raise ValueError(f'{name}: lengths must be int32 [{batch}]')
+    return lengths.contiguous()
+
+
+def _status(name, status, device, needed):
+    """(status word, owned); no word where nothing can be reported."""
+    if status is None and not needed:
+        return None, False
+    if status is None and torch.cuda.is_current_stream_capturing():
+        raise ValueError(f'{name} under graph capture needs a caller status word')
+    return _status_word(status, device)
+
+
+class _Cache:
+    """The C view of a cache and what the operators ask of it.  k alone where
+    V is not read."""
+
+    def __init__(self, name, k, v, pages, table, lengths, keys, batch, values=True):
+        self.keep = []
+        if (k is None) == (pages is None):
+            raise ValueError(f'{name}: give the cache either as dense rows or as pages with a block table')
+        if pages is None:
+            if table is not None or keys is not None:
+                raise ValueError(f'{name}: a block table and keys belong to pages')
+            if values and v is None:
+                raise ValueError(f'{name}: dense rows need both k and v')
+            if k.dim() != 4 or k.shape[0] != batch or k.stride(3) != 1 and k.shape[3] != 1:
+                raise ValueError(f'{name}: cache rows must be [{batch}, N, Hkv, D] with contiguous features')
+            if values and (v.shape != k.shape or v.stride(3) != 1):
+                raise ValueError(f'{name}: v must have the shape of k with contiguous features')
+            self.rows, self.heads, self.dim = k.shape[1:]
+            parts = (k, v) if values else (k, None)
+            self.fields = [x for t in parts for x in
+                           ((None, 0, 0, 0) if t is None else (_ptr(t), *t.stride()[:3]))]
+            self.fields += [None, 0, 0, 0, 0]
+            self.first = k
+        else:
+            if v is not None:
+                raise ValueError(f'{name}: pages hold both K and V')
+            if pages.dim() != 5 or pages.shape[2] != 2 or pages.stride(4) != 1:
+                raise ValueError(f'{name}: pages must be [blocks, block, 2, Hkv, D] with contiguous features')
+            if table is None or table.dtype is not torch.int64 or table.dim() != 2 or table.shape[0] != batch:
+                raise ValueError(f'{name}: pages need an int64 block table [{batch}, cols]')
+            table = table if table.stride(1) == 1 else table.contiguous()
+            self.keep.append(table)
+            blocks, block, _, self.heads, self.dim = pages.shape
+            cols = table.shape[1]
+            self.rows = cols * block if keys is None else int(keys)
+            if not 0 <= self.rows <= cols * block:
+                raise ValueError(f'{name}: keys must lie in [0, {cols * block}] (cols * block)')
+            sb, sn, skind, sh, _ = pages.stride()
+            base = pages.data_ptr()
+            self.fields = [base, sb, sn, sh, base + skind * pages.element_size(), sb, sn, sh]
+            self.fields += [_ptr(table), table.stride(0), cols, blocks, block] if self.rows else [None, 0, 0, 0, 0]
+            self.first = pages
+        lengths = _lengths(name, lengths, batch)
+        self.keep.append(lengths)
+        self.fields += [_ptr(lengths), self.rows]
+        self.paged = pages is not None and self.rows > 0
+
+    def struct(self, status):
+        return _lib.CacheRows(*self.fields, _ptr(status))
+
+
+def _queries(name, q, cache):
+    if q.dim() != 4 or q.shape[3] != cache.dim or q.shape[2] % cache.heads:
+        raise ValueError(f'{name}: q must be [B, rows, Hq, {cache.dim}] with Hq a multiple of {cache.heads}')
+
+
+def _launch(device, call, *args):
+    """One entry point on torch's current stream of `device`, whichever device
+    is current."""
+    if device.index == torch.cuda.current_device():
+        check(call(*args, _lib.stream_handle(device)))
+    else:
+        with torch.cuda.device(device):
+            check(call(*args, _lib.stream_handle(device)))
+
+
+def _with_workspace(device, query, call, a):
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _with_workspace(device, query, call, a)
+    nbytes = query(ctypes.byref(a))
+    if nbytes == 0:
+        check(-1)
+    ws = _workspace(nbytes, device)
+    check(call(ctypes.byref(a), _ptr(ws), nbytes, _lib.stream_handle(device)))
+
+
+def tree_attention(q, draft_k, draft_v, scale, k=None, v=None, *, pages=None, table=None, lengths=None, keys=None,
+                   mask=None, out=None, lse=None, status=None):
+    """Attention of drafted tokens over a cache and over each other.
+
+    q [B, T, Hq, D], draft_k / draft_v [B, T, Hkv, D] (rotated, not yet in the
+    cache; T up to 1024); the cache dense or paged (`keys`: the longest
+    sequence's rows, default cols * block).  mask [T, T] or [B, T, T] bool:
+    drafted token t sees drafted token j where mask[.., t, j] (itself included
+    only if so marked); None is a chain (j <= t).  Every token sees all rows of
+    its sequence's cache.  Returns (out [B, T, Hq, D], lse [B, Hq, T] fp32); a
+    row that sees nothing gives 0 and -inf, and what lies in unseen rows has no
+    influence, infinities and NaN included.  T = 1 decodes a single token."""
+    name = 'tree_attention'
+    B = q.shape[0]
+    cache = _Cache(name, k, v, pages, table, lengths, keys, B)
+    code = _dtype(name, q, draft_k, draft_v, cache.first, v, out)
+    _queries(name, q, cache)
+    T, Hq, D = q.shape[1:]
+    if draft_k.shape != (B, T, cache.heads, D) or draft_v.shape != draft_k.shape:
+        raise ValueError(f'{name}: draft_k and draft_v must be [{B}, {T}, {cache.heads}, {D}]')
+    m = (None, 0, 0)
+    if mask is not None:
+        if mask.dtype is not torch.bool or mask.shape not in ((T, T), (B, T, T)):
+            raise ValueError(f'{name}: mask must be bool [{T}, {T}] or [{B}, {T}, {T}]')
+        if mask.stride(-1) != 1:
+            mask = mask.contiguous()
+        m = (_ptr(mask), mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
+    if out is not None and (out.shape != q.shape or out.stride(3) != 1 or
+                            any(t is not None and _overlap(out, t) for t in (q, draft_k, draft_v, k, v, pages))):
+        raise ValueError(f'{name}: out must have the shape of q with contiguous features, apart from the inputs')
+    if lse is not None and (lse.shape != (B, Hq, T) or lse.dtype is not torch.float32 or not lse.is_contiguous()):
+        raise ValueError(f'{name}: lse must be a contiguous float32 [{B}, {Hq}, {T}]')
+    device = _common(name, q, draft_k, draft_v, k, v, pages, table, lengths, mask, out, lse)
+    q, draft_k, draft_v = _rows16(q), _rows16(draft_k), _rows16(draft_v)
+    if out is None:
+        out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=device)
+    if lse is None:
+        lse = torch.empty(B, Hq, T, dtype=torch.float32, device=device)
+    status, owned = _status(name, status, device, cache.paged)
+    a = _lib.TreeAttentionArgs(
+        cache.struct(status), _ptr(q), *q.stride()[:3], _ptr(draft_k), *draft_k.stride()[:3], _ptr(draft_v),
+        *draft_v.stride()[:3], *m, _ptr(out), *out.stride()[:3], _ptr(lse), B, T, Hq, cache.heads, D, float(scale), code)
+    _with_workspace(device, lib().slimkv_tree_attention_workspace, lib().slimkv_tree_attention, a)
+    if owned:
+        check_status(status)
+    return out, lse
+
+
+def attention_weights(q, lse, scale, k=None, *, pages=None, table=None, lengths=None, keys=None, causal=True,
+                      previous=None, out=None, status=None):
+    """The attention weight of every cached row, added to what it has gathered:
+
+        out[b, h, j] = previous[b, h, j] + sum over l, g of exp(scale q[b, l, hG + g] . k[b, j, h] - lse[b, hG + g, l])
+
+    q [B, L, Hq, D] rotated and lse [B, Hq, L] fp32 as the attention left it
+    (tree_attention, kernels.attention_forward, kernels.prefill_attention); the
+    cache dense (k alone) or paged.  With `causal` the last query stands at the
+    sequence's last row and query l sees rows up to length - L + l; a query row
+    whose LSE is -inf counts nothing (padding).  previous [B, Hkv, N] fp32,
+    None for zeros; N = the dense rows or `keys` (default cols * block).  Rows
+    at or past a sequence's length keep `previous`.  Returns out [B, Hkv, N]
+    fp32, which may be `previous` itself."""
+    name = 'attention_weights'
+    B = q.shape[0]
+    cache = _Cache(name, k, None, pages, table, lengths, keys, B, values=False)
+    code = _dtype(name, q, cache.first)
+    _queries(name, q, cache)
+    L, Hq, D = q.shape[1:]
+    if lse.shape != (B, Hq, L) or lse.dtype is not torch.float32:
+        raise ValueError(f'{name}: lse must be float32 [{B}, {Hq}, {L}]')
+    shape = (B, cache.heads, cache.rows)
+    for what, t in (('previous', previous), ('out', out)):
+        if t is not None and (t.shape != shape or t.dtype is not torch.float32 or t.stride(2) != 1 and shape[2] > 1):
+            raise ValueError(f'{name}: {what} must be float32 {list(shape)} with contiguous rows')
+    if out is not None and previous is not None and _overlap(out, previous) and \
+            (out.data_ptr() != previous.data_ptr() or out.stride() != previous.stride()):
+        raise ValueError(f'{name}: out must be previous itself or lie apart from it')
+    device = _common(name, q, lse, k, pages, table, lengths, previous, out)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=device)
+    q = _rows16(q)
+    status, owned = _status(name, status, device, cache.paged)
+    a = _lib.AttentionWeightsArgs(
+        cache.struct(status), _ptr(q), *q.stride()[:3], _ptr(lse), *lse.stride(),
+        _ptr(previous), *(previous.stride()[:2] if previous is not None else (0, 0)), _ptr(out), *out.stride()[:2],
+        B, L, Hq, cache.heads, D, float(scale), int(bool(causal)), code)
+    _with_workspace(device, lib().slimkv_attention_weights_workspace, lib().slimkv_attention_weights, a)
+    if owned:
+        check_status(status)
+    return out
+
+
+def select_rows(weights, keep, *, lengths=None, sink=0, recent=0):
+    """The rows a cache of `keep` rows holds on to: the first `sink`, the last
+    `recent`, and of those between the heaviest by weights [B, H, N] fp32 (H
+    the KV heads, or 1 for one choice for all heads).  Equal weights: the lower
+    index first; NaN ranks below every number.  Returns (rows [B, H, keep]
+    int32, ascending, -1 past the count; counts [B] int32 = min(length, keep))."""
+    name = 'select_rows'
+    if weights.dim() != 3 or weights.dtype is not torch.float32:
+        raise ValueError(f'{name}: weights must be float32 [B, H, N]')
+    B, H, N = weights.shape
+    keep, sink, recent = int(keep), int(sink), int(recent)
+    if keep <= 0 or sink < 0 or recent < 0 or sink + recent > keep:
+        raise ValueError(f'{name}: needs keep > 0 and 0 <= sink + recent <= keep')
+    if weights.stride(2) != 1:
+        weights = weights.contiguous()
+    lengths = _lengths(name, lengths, B)
+    device = _common(name, weights, lengths)
+    rows = torch.empty(B, H, keep, dtype=torch.int32, device=device)
+    counts = torch.empty(B, dtype=torch.int32, device=device)
+    a = _lib.SelectRowsArgs(_ptr(weights), *weights.stride()[:2], _ptr(lengths), _ptr(rows), _ptr(counts), B, H, N,
+                            keep, sink, recent)
+    _with_workspace(device, lib().slimkv_select_rows_workspace, lib().slimkv_select_rows, a)
+    return rows, counts
+
+
+def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weights=None, out_k=None, out_v=None,
+                 in_place=False, status=None):
+    """Rows rows[b, h, :counts[b]] of every sequence and KV head, moved to the
+    front of a cache; rows int32 [B, Hkv or 1, keep], counts int32 [B].
+
+    Out of place (the default): returns (k, v [B, keep, Hkv, D], weights
+    [B, Hw, keep] or None), rows from counts[b] on zero.  in_place: within the
+    given k / v or pages and within `weights`, for choices in strictly
+    ascending order (select_rows'); cache rows from counts[b] on stay as they
+    are, weights from there on become zero; returns the given tensors (None,
+    None for pages).  weights [B, rows' head count, N] fp32 move along.  A row
+    outside the cache (in place: or out of order) moves nothing and raises
+    IndexError after the call, or is left in `status`.  In place, no other
+    sequence's table may name the pages a sequence writes."""
+    name = 'compact_rows'
+    if rows.dim() != 3 or rows.dtype is not torch.int32 or counts.dtype is not torch.int32 or \
+            counts.shape != rows.shape[:1]:
+        raise ValueError(f'{name}: rows must be int32 [B, heads, keep] and counts int32 [B]')
+    B, Hw, keep = rows.shape
+    cache = _Cache(name, k, v, pages, table, None, None, B)
+    code = _dtype(name, cache.first, v, out_k, out_v)
+    H, D = cache.heads, cache.dim
+    if Hw not in (1, H):
+        raise ValueError(f'{name}: rows must have 1 or {H} heads')
+    rows = rows if rows.stride(2) == 1 else rows.contiguous()
+    counts = counts.contiguous()
+    if weights is not None and (weights.dim() != 3 or weights.shape[:2] != (B, Hw) or weights.stride(2) != 1 or
+                                weights.dtype is not torch.float32):
+        raise ValueError(f'{name}: weights must be float32 [{B}, {Hw}, N] with contiguous rows')
+    out_weights = None
+    if in_place:
+        if out_k is not None or out_v is not None:
+            raise ValueError(f'{name}: in place there are no outputs')
+        for t in (k, v, pages, weights):
+            if t is not None and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+                raise ValueError(f'{name}: in place the cache must not be an expanded view')
+        if k is not None and k.numel() and k.data_ptr() == v.data_ptr():
+            raise ValueError(f'{name}: in place k and v must be two tensors')
+    sources = [t for t in (k, v, pages) if t is not None]
+    for t in (out_k, out_v):
+        if t is not None and (t.shape != (B, keep, H, D) or t.stride(3) != 1 or any(_overlap(t, s) for s in sources)):
+            raise ValueError(f'{name}: outputs must be [{B}, {keep}, {H}, {D}] with contiguous features, apart from '
+                             'the cache')
+    if out_k is not None and out_v is not None and _overlap(out_k, out_v):
+        raise ValueError(f'{name}: out_k and out_v must lie apart')
+    device = _common(name, rows, counts, k, v, pages, table, weights, out_k, out_v)
+    outs = (None, 0, 0, 0, None, 0, 0, 0)
+    if not in_place:
+        out_k = torch.empty(B, keep, H, D, dtype=cache.first.dtype, device=device) if out_k is None else out_k
+        out_v = torch.empty(B, keep, H, D, dtype=cache.first.dtype, device=device) if out_v is None else out_v
+        if weights is not None:
+            out_weights = torch.empty(B, Hw, keep, dtype=torch.float32, device=device)
+        outs = (_ptr(out_k), *out_k.stride()[:3], _ptr(out_v), *out_v.stride()[:3])
+    status, owned = _status(name, status, device, True)
+    a = _lib.CompactRowsArgs(
+        cache.struct(status), _ptr(rows), rows.stride(0), rows.stride(1) if Hw > 1 else 0, _ptr(counts), *outs,
+        _ptr(weights), *(weights.stride()[:2] if weights is not None else (0, 0)),
+        _ptr(out_weights), *(out_weights.stride()[:2] if out_weights is not None else (0, 0)),
+        Hw, 0 if weights is None else weights.shape[2], B, H, D, keep, int(bool(in_place)), code)
+    _launch(device, lib().slimkv_compact_rows, ctypes.byref(a))
+    if owned:
+        check_status(status)
+    if in_place:
+        return k, v, weights
+    return out_k, out_v, out_weights

@@ -22,12 +22,16 @@ slimkv_amd.kernels and has no CPU implementation.
         history) -> (q_rot, k_rot)                 (decode_kernels.py:7-51)
     slimkv::merge(raw, raw_lse, latent, latent_lse) -> out
         (fa2_decode.py:57-66)
+    slimkv::tree_attention, attention_weights, select_rows, compact_rows
+        the cache operators (slimkv_amd.cache_ops), out of place; index errors
+        are left in `status`, which reads through block tables and row moves
+        need
 """
 from typing import Optional
 
 import torch
 
-from . import kernels
+from . import cache_ops, kernels
 
 Tensor = torch.Tensor
 _NS = 'slimkv'
@@ -126,3 +130,62 @@ def merge(raw: Tensor, raw_lse: Tensor, latent: Tensor, latent_lse: Tensor) -> T
 @merge.register_fake
 def _(raw, raw_lse, latent, latent_lse):
     return raw.new_empty(raw.shape)
+
+
+@torch.library.custom_op(f'{_NS}::tree_attention', mutates_args=('status',), device_types='cuda')
+def tree_attention(q: Tensor, draft_k: Tensor, draft_v: Tensor, scale: float, k: Optional[Tensor], v: Optional[Tensor],
+                   pages: Optional[Tensor], table: Optional[Tensor], lengths: Optional[Tensor], keys: Optional[int],
+                   mask: Optional[Tensor], status: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """cache_ops.tree_attention: q [B,T,Hq,D] -> (out [B,T,Hq,D], lse [B,Hq,T])."""
+    return cache_ops.tree_attention(q, draft_k, draft_v, scale, k, v, pages=pages, table=table, lengths=lengths,
+                                    keys=keys, mask=mask, status=status)
+
+
+@tree_attention.register_fake
+def _(q, draft_k, draft_v, scale, k, v, pages, table, lengths, keys, mask, status):
+    B, T, Hq, D = q.shape
+    return q.new_empty((B, T, Hq, D)), _lse_like(q, B, Hq, T)
+
+
+@torch.library.custom_op(f'{_NS}::attention_weights', mutates_args=('status',), device_types='cuda')
+def attention_weights(q: Tensor, lse: Tensor, scale: float, k: Optional[Tensor], pages: Optional[Tensor],
+                      table: Optional[Tensor], lengths: Optional[Tensor], keys: Optional[int], causal: bool,
+                      previous: Optional[Tensor], status: Optional[Tensor]) -> Tensor:
+    """cache_ops.attention_weights: -> weights [B,Hkv,N] fp32, a new tensor."""
+    return cache_ops.attention_weights(q, lse, scale, k, pages=pages, table=table, lengths=lengths, keys=keys,
+                                       causal=causal, previous=previous, status=status)
+
+
+@attention_weights.register_fake
+def _(q, lse, scale, k, pages, table, lengths, keys, causal, previous, status):
+    if k is not None:
+        heads, rows = k.shape[2], k.shape[1]
+    else:
+        heads, rows = pages.shape[3], table.shape[1] * pages.shape[1] if keys is None else keys
+    return q.new_empty((q.shape[0], heads, rows), dtype=torch.float32)
+
+
+@torch.library.custom_op(f'{_NS}::select_rows', mutates_args=(), device_types='cuda')
+def select_rows(weights: Tensor, keep: int, lengths: Optional[Tensor], sink: int, recent: int) -> tuple[Tensor, Tensor]:
+    """cache_ops.select_rows: -> (rows [B,H,keep] int32, counts [B] int32)."""
+    return cache_ops.select_rows(weights, keep, lengths=lengths, sink=sink, recent=recent)
+
+
+@select_rows.register_fake
+def _(weights, keep, lengths, sink, recent):
+    return weights.new_empty((*weights.shape[:2], keep), dtype=torch.int32), \
+        weights.new_empty((weights.shape[0],), dtype=torch.int32)
+
+
+@torch.library.custom_op(f'{_NS}::compact_rows', mutates_args=('status',), device_types='cuda')
+def compact_rows(rows: Tensor, counts: Tensor, k: Optional[Tensor], v: Optional[Tensor], pages: Optional[Tensor],
+                 table: Optional[Tensor], weights: Tensor, status: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
+    """cache_ops.compact_rows out of place: -> (k, v [B,keep,Hkv,D], weights [B,H,keep])."""
+    return cache_ops.compact_rows(rows, counts, k, v, pages=pages, table=table, weights=weights, status=status)
+
+
+@compact_rows.register_fake
+def _(rows, counts, k, v, pages, table, weights, status):
+    first = k if k is not None else pages
+    shape = (rows.shape[0], rows.shape[2], *first.shape[-2:])
+    return first.new_empty(shape), first.new_empty(shape), weights.new_empty(rows.shape)

@@ -1,0 +1,250 @@
+"""The cache operators without a GPU: the C header and its ctypes mirror, refusals before anything reaches the
+device, the torch operators' shapes, and the 64-bit plain forms on cases small enough to check by hand."""
+import ctypes
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from oracle import cache as oc
+
+ROOT = Path(__file__).resolve().parents[1]
+HEADER = ROOT / 'include' / 'slimkv' / 'cache_ops.h'
+BF16 = torch.bfloat16
+
+
+def stripped():
+    return re.sub(r'/\*.*?\*/', '', HEADER.read_text(), flags=re.S)
+
+
+def structs():
+    from slimkv_amd import _lib
+    return (_lib.CacheRows, _lib.TreeAttentionArgs, _lib.AttentionWeightsArgs, _lib.SelectRowsArgs, _lib.CompactRowsArgs)
+
+
+def test_library_exports_what_the_header_declares():
+    from slimkv_amd import _lib
+    names = sorted(set(re.findall(r'\b(slimkv_[a-z0-9_]+)\s*\(', stripped())))
+    assert len(names) == 8
+    for name in names:
+        assert hasattr(_lib.lib(), name) and name in _lib.SIGNATURES, name
+
+
+def test_struct_layouts_match_the_c_compiler(tmp_path):
+    if shutil.which('gcc') is None:
+        pytest.skip('gcc not available')
+    lines, want = [], []
+    for s in structs():
+        body = re.search(r'typedef struct %s \{(.*?)\}' % s.__name__, stripped(), re.S).group(1)
+        assert re.findall(r'\*?\s*([a-z_][a-z0-9_]*)\s*(?=[,;])', body) == [f[0] for f in s._fields_], s.__name__
+        lines.append(f'printf("%zu\\n", sizeof({s.__name__}));')
+        want.append(ctypes.sizeof(s))
+        for field, _ in s._fields_:
+            lines.append(f'printf("%zu\\n", offsetof({s.__name__}, {field}));')
+            want.append(getattr(s, field).offset)
+    src = tmp_path / 'layout.c'
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "slimkv/cache_ops.h"\nint main(void){\n' +
+                   '\n'.join(lines) + '\nreturn 0;}\n')
+    subprocess.run(['gcc', '-I', str(ROOT / 'include'), str(src), '-o', str(tmp_path / 'layout')], check=True)
+    got = subprocess.run([str(tmp_path / 'layout')], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(x) for x in got] == want
+
+
+def test_interface_number():
+    from slimkv_amd import _lib
+    assert _lib.lib().slimkv_cache_abi_version() == _lib.CACHE_ABI_VERSION
+
+
+def z(*shape, dtype=BF16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def tree(**over):
+    from slimkv_amd import cache_ops
+    a = dict(q=z(2, 3, 8, 64), draft_k=z(2, 3, 2, 64), draft_v=z(2, 3, 2, 64), scale=1.0, k=z(2, 9, 2, 64),
+             v=z(2, 9, 2, 64))
+    a.update(over)
+    return cache_ops.tree_attention(a.pop('q'), a.pop('draft_k'), a.pop('draft_v'), a.pop('scale'), **a)
+
+
+PAGED = dict(k=None, v=None, pages=z(6, 4, 2, 2, 64), table=z(2, 3, dtype=torch.int64))
+shared = z(2 * 3 * 8 * 64 + 8)
+
+
+@pytest.mark.parametrize('over,match', [
+    (dict(), 'device tensors'),
+    (PAGED, 'device tensors'),
+    (dict(q=z(2, 3, 7, 64)), 'multiple of 2'),
+    (dict(q=z(2, 3, 8, 128)), 'q must be'),
+    (dict(q=z(2, 3, 8, 64, dtype=torch.float32)), 'bfloat16 or float16'),
+    (dict(draft_k=z(2, 3, 2, 64, dtype=torch.float16)), 'bfloat16 or float16'),
+    (dict(draft_k=z(2, 4, 2, 64)), 'draft_k and draft_v'),
+    (dict(draft_v=z(2, 3, 1, 64)), 'draft_k and draft_v'),
+    (dict(v=z(2, 8, 2, 64)), 'v must have the shape'),
+    (dict(v=None), 'both k and v'),
+    (dict(k=None, v=None), 'either as dense rows or as pages'),
+    (dict(k=z(1, 9, 2, 64), v=z(1, 9, 2, 64)), 'cache rows must be'),
+    (dict(lengths=z(2, dtype=torch.int64)), 'lengths must be int32'),
+    (dict(lengths=z(3, dtype=torch.int32)), 'lengths must be int32'),
+    (dict(mask=z(3, 3, dtype=torch.uint8)), 'mask must be bool'),
+    (dict(mask=z(1, 3, 3, dtype=torch.bool)), 'mask must be bool'),
+    (dict(mask=z(2, 3, 4, dtype=torch.bool)), 'mask must be bool'),
+    (dict(out=z(2, 3, 8, 32)), 'out must have'),
+    (dict(q=shared[:-8].view(2, 3, 8, 64), out=shared[8:].view(2, 3, 8, 64)), 'apart from the inputs'),
+    (dict(lse=z(2, 8, 3)), 'lse must be'),
+    (dict(keys=9), 'belong to pages'),
+    (dict(PAGED, keys=13), 'keys must lie'),
+    (dict(PAGED, table=z(2, 3, dtype=torch.int32)), 'int64 block table'),
+    (dict(PAGED, table=z(1, 3, dtype=torch.int64)), 'int64 block table'),
+    (dict(PAGED, v=z(2, 9, 2, 64)), 'pages hold both'),
+    (dict(PAGED, pages=z(6, 4, 3, 2, 64)), 'pages must be'),
+])
+def test_tree_attention_refuses(over, match):
+    with pytest.raises(ValueError, match=match):
+        tree(**over)
+
+
+def weights(**over):
+    from slimkv_amd import cache_ops
+    a = dict(q=z(2, 3, 8, 64), lse=z(2, 8, 3, dtype=torch.float32), scale=1.0, k=z(2, 9, 2, 64))
+    a.update(over)
+    return cache_ops.attention_weights(a.pop('q'), a.pop('lse'), a.pop('scale'), **a)
+
+
+line = z(2 * 2 * 9 + 4, dtype=torch.float32)
+
+
+@pytest.mark.parametrize('over,match', [
+    (dict(), 'device tensors'),
+    (dict(lse=z(2, 3, 8, dtype=torch.float32)), 'lse must be'),
+    (dict(lse=z(2, 8, 3)), 'lse must be'),
+    (dict(previous=z(2, 2, 8, dtype=torch.float32)), 'previous must be'),
+    (dict(out=z(2, 2, 9)), 'out must be'),
+    (dict(previous=line[:36].view(2, 2, 9), out=line[4:].view(2, 2, 9)), 'previous itself'),
+    (dict(k=z(2, 9, 3, 64)), 'multiple of 3'),
+])
+def test_attention_weights_refuses(over, match):
+    with pytest.raises(ValueError, match=match):
+        weights(**over)
+
+
+@pytest.mark.parametrize('args,match', [
+    ((z(2, 3, 9, dtype=torch.float32), 4), 'device tensors'),
+    ((z(2, 3, 9), 4), 'float32'),
+    ((z(2, 9, dtype=torch.float32), 4), 'float32'),
+    ((z(2, 3, 9, dtype=torch.float32), 0), 'keep > 0'),
+    ((z(2, 3, 9, dtype=torch.float32), 4, 3, 2), 'sink'),
+    ((z(2, 3, 9, dtype=torch.float32), 4, -1, 2), 'sink'),
+])
+def test_select_rows_refuses(args, match):
+    from slimkv_amd import cache_ops
+    with pytest.raises(ValueError, match=match):
+        cache_ops.select_rows(*args[:2], **dict(zip(('sink', 'recent'), args[2:])))
+
+
+def compact(**over):
+    from slimkv_amd import cache_ops
+    a = dict(rows=z(2, 2, 4, dtype=torch.int32), counts=z(2, dtype=torch.int32), k=z(2, 9, 2, 64), v=z(2, 9, 2, 64))
+    a.update(over)
+    return cache_ops.compact_rows(a.pop('rows'), a.pop('counts'), **a)
+
+
+cache = z(2 * 9 * 2 * 64)
+
+
+@pytest.mark.parametrize('over,match', [
+    (dict(), 'device tensors'),
+    (dict(rows=z(2, 2, 4, dtype=torch.int64)), 'rows must be int32'),
+    (dict(counts=z(3, dtype=torch.int32)), 'rows must be int32'),
+    (dict(rows=z(2, 3, 4, dtype=torch.int32)), '1 or 2 heads'),
+    (dict(weights=z(2, 1, 9, dtype=torch.float32)), 'weights must be'),
+    (dict(in_place=True, out_k=z(2, 4, 2, 64)), 'no outputs'),
+    (dict(in_place=True, k=z(1, 9, 2, 64).expand(2, 9, 2, 64)), 'expanded'),
+    (dict(in_place=True, k=cache.view(2, 9, 2, 64), v=cache.view(2, 9, 2, 64)), 'two tensors'),
+    (dict(out_k=z(2, 4, 2, 32)), 'outputs must be'),
+    (dict(k=cache.view(2, 9, 2, 64), out_k=cache[:1024].view(2, 4, 2, 64)), 'apart from the cache'),
+])
+def test_compact_rows_refuses(over, match):
+    with pytest.raises(ValueError, match=match):
+        compact(**over)
+
+
+def test_the_c_entry_points_refuse_bad_sizes():
+    """Calls through the C interface that end before a launch."""
+    from slimkv_amd import _lib
+    lib, ref = _lib.lib(), ctypes.byref
+    a = _lib.TreeAttentionArgs()
+    assert lib.slimkv_tree_attention(ref(a), None, 0, None) < 0
+    a.q, a.draft_k, a.draft_v, a.out = 4096, 4096, 4096, 4096
+    a.batch, a.drafted, a.heads, a.kv_heads, a.head_dim, a.scale = 1, 1, 8, 2, 128, 1.0
+    need = lib.slimkv_tree_attention_workspace(ref(a))
+    assert need > 0
+    assert lib.slimkv_tree_attention(ref(a), 4096, need - 1, None) == -3
+    assert lib.slimkv_tree_attention(ref(a), None, need, None) == -3
+    for field, value, code in (('head_dim', 96, -2), ('dtype', 2, -2), ('drafted', 1025, -1), ('heads', 9, -1),
+                               ('scale', 0.0, -1), ('batch', -1, -1), ('q', 4098, -1), ('draft_k', 0, -1)):
+        old = getattr(a, field)
+        setattr(a, field, value)
+        assert lib.slimkv_tree_attention(ref(a), 4096, need, None) == code, field
+        setattr(a, field, old)
+    a.cache.keys = 5
+    assert lib.slimkv_tree_attention(ref(a), 4096, need, None) == -1          # null cache
+    a.cache.k, a.cache.v, a.cache.table = 4096, 4096, 4096
+    a.cache.block_size, a.cache.num_blocks, a.cache.t_cols = 2, 4, 2
+    assert lib.slimkv_tree_attention(ref(a), 4096, need, None) == -1          # rows past the table
+    assert b'block table' in lib.slimkv_last_error()
+    a.cache.table, a.cache.k_sn = None, 100
+    assert lib.slimkv_tree_attention(ref(a), 4096, need, None) == -1
+    assert b'16-byte' in lib.slimkv_last_error()
+    w = _lib.AttentionWeightsArgs()
+    assert lib.slimkv_attention_weights(ref(w), None, 0, None) < 0
+    s = _lib.SelectRowsArgs()
+    s.batch, s.heads, s.keys, s.keep, s.sink = 1, 1, 10, 4, 5
+    assert lib.slimkv_select_rows(ref(s), None, 0, None) == -1
+    c = _lib.CompactRowsArgs()
+    assert lib.slimkv_compact_rows(ref(c), None) == -2
+
+
+def test_torch_operators_shapes():
+    import slimkv_amd.torch_ops  # noqa: F401
+    with FakeTensorMode():
+        q = torch.empty(2, 3, 8, 64, dtype=BF16, device='cuda')
+        d = torch.empty(2, 3, 2, 64, dtype=BF16, device='cuda')
+        pages, table = torch.empty(6, 4, 2, 2, 64, dtype=BF16, device='cuda'), torch.empty(2, 3, dtype=torch.int64, device='cuda')
+        out, lse = torch.ops.slimkv.tree_attention(q, d, d, 1.0, None, None, pages, table, None, None, None, None)
+        assert out.shape == q.shape and out.dtype == BF16 and lse.shape == (2, 8, 3) and lse.dtype == torch.float32
+        w = torch.ops.slimkv.attention_weights(q, lse, 1.0, None, pages, table, None, None, True, None, None)
+        assert w.shape == (2, 2, 12) and w.dtype == torch.float32
+        rows, counts = torch.ops.slimkv.select_rows(w, 5, None, 1, 2)
+        assert rows.shape == (2, 2, 5) and rows.dtype == torch.int32 and counts.shape == (2,)
+        k, v, kept = torch.ops.slimkv.compact_rows(rows, counts, None, None, pages, table, w, None)
+        assert k.shape == v.shape == (2, 5, 2, 64) and k.dtype == BF16 and kept.shape == (2, 2, 5)
+
+
+def test_oracle_tree_by_hand():
+    """One head of width 1: the cache's row 0 and the tokens the mask names."""
+    q, one = np.ones((1, 2, 1, 1)), np.zeros((1, 1, 1, 1))
+    dk, dv = np.log(np.array([2.0, 5.0])).reshape(1, 2, 1, 1), np.array([4.0, 10.0]).reshape(1, 2, 1, 1)
+    mask = np.array([[False, False], [True, False]])
+    out, lse, *_ = oc.tree_attention(q, one, one + 1, [1], dk, dv, mask, 1.0)
+    assert np.allclose(out.ravel(), [1.0, (1 + 2 * 4) / 3]) and np.allclose(lse.ravel(), [0.0, np.log(3)])
+    out, lse, *_ = oc.tree_attention(q, one, one + 1, [0], dk, dv, mask, 1.0)
+    assert out[0, 0, 0, 0] == 0 and np.isneginf(lse[0, 0, 0]) and out[0, 1, 0, 0] == 4
+
+
+def test_oracle_weights_and_rows_by_hand():
+    q, k = np.ones((1, 2, 1, 1)), np.log(np.array([1.0, 3.0, 4.0])).reshape(1, 3, 1, 1)
+    lse = np.log(np.array([4.0, 8.0])).reshape(1, 1, 2)
+    w, *_ = oc.attention_weights(q, lse, k, [3], 1.0)
+    assert np.allclose(w.ravel(), [1 / 4 + 1 / 8, 3 / 4 + 3 / 8, 4 / 8])
+    rows, counts = oc.select_rows(np.array([[[5.0, 1, 9, 9, np.nan, 0, 2]]]), 4, [7], 1, 1)
+    assert rows.tolist() == [[[0, 2, 3, 6]]] and counts.tolist() == [4]
+    rows, counts = oc.select_rows(np.array([[[0.0, 1, 1, 1, 0, 0]]]), 2, [5], 0, 0)
+    assert rows.tolist() == [[[1, 2]]]
+    rows, counts = oc.select_rows(np.array([[[0.0, 1, 1]]]), 4, [2], 1, 1)
+    assert rows.tolist() == [[[0, 1, -1, -1]]] and counts.tolist() == [2]
