@@ -100,8 +100,497 @@ __device__ __forceinline__ int used_runs(const TreeParams& p, int64_t total) {
 
 __device__ __forceinline__ int64_t run_begin(int64_t total, int runs, int r) { return r * total / runs; }
 
-template <int D, int RW, int NT>
+// ---------------------------------------------------------------------------
+// what both kernels share
+// ---------------------------------------------------------------------------
+
+// The page numbers of a stretch of the cache, in LDS: a tile's loads then wait
+// for no table read.  Holds table columns [first, first + kPages).
+constexpr int kPages = 1024;
+
+struct Pages {
+    int32_t page[kPages];
+};
+
+// Tiles a stretch holds at any block size: 64 c rows span at most 64 c / block
+// + 2 columns.
+__device__ __forceinline__ int page_tiles(const CacheView& c) {
+    return (int)min<int64_t>((int64_t)(kPages - 2) * c.block.d / kKeys, 1 << 24);
+}
+
+// Columns of tiles [t, t + page_tiles) that rows below n need; every thread of
+// the workgroup, between barriers.
+__device__ __forceinline__ void load_pages(const CacheView& c, int64_t b, int t, int n, Pages& s) {
+    const int first = quotient(t * kKeys, c.block), last = quotient(n - 1, c.block);
+    const int count = min(last - first + 1, kPages);
+    for (int i = threadIdx.x; i < count; i += 256) {
+        const int64_t page = table_page(c.table[b * c.t_sb + first + i], c.num_blocks);
+        if (page < 0) report_bad_page(c.status);
+        s.page[i] = page < 0 ? 0 : (int)page;
+    }
+}
+
+// Row `row` (below the length) through the stretch that begins with tile t.
+__device__ __forceinline__ RowAt paged_row(const CacheView& c, const Pages& s, int t, int row) {
+    const int col = quotient(row, c.block);
+    const int64_t page = s.page[col - quotient(t * kKeys, c.block)];
+    const int64_t slot = row - col * (int)c.block.d;
+    return RowAt{page * c.k_sb + slot * c.k_sn, page * c.v_sb + slot * c.v_sn};
+}
+
+// Order LDS accesses of one wave: its LDS instructions execute in issue order,
+// so only the compiler's reordering has to be prevented.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Which drafted tokens first .. first + 63 the tokens of `rows` query rows from
+// row0 on see, one 64-bit word a token in the wave's own LDS: lane j reads the
+// byte of token first + j and the ballot makes the word.
+__device__ __forceinline__ void drafted_seen(const TreeParams& p, int64_t b, int row0, int rows, int first,
+                                             uint64_t* words) {
+    const int lane = threadIdx.x & 63, j = first + lane;
+    const int from = min(row0, p.M - 1) / p.G, to = min(row0 + rows - 1, p.M - 1) / p.G;
+    wave_fence();
+    for (int t0 = from; t0 <= to; t0 += 4) {               // four tokens' bytes in flight
+        bool sees[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int tq = min(t0 + i, to);
+            sees[i] = j < p.T && (p.mask ? p.mask[b * p.m_sb + tq * p.m_sl + min(j, p.T - 1)] != 0 : j <= tq);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t word = __ballot(sees[i]);
+            if (lane == 0) words[min(t0 + i, to) - from] = word;
+        }
+    }
+    wave_fence();
+}
+
+// Drafted values that are not finite stay out of the matrix product (0 there,
+// with the flag set), since a zero weight would not keep them from rows that
+// do not see them.
+template <bool F16>
+__device__ __forceinline__ u32x4 finite_only(u32x4 x, bool* wild) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t w = x[e];
+        if (Elem<F16>::unbounded(w)) {
+            *wild = true;
+            const uint32_t all = F16 ? 0x7c00u : 0x7f80u;
+            x[e] = ((w & all) == all ? 0u : w & 0xffffu) | ((w >> 16 & all) == all ? 0u : w & 0xffff0000u);
+        }
+    }
+    return x;
+}
+
+// They are then added to the rows that do see them: any positive weight makes
+// an infinity or NaN of them.  Tokens [j0, j1); lane (col, grp) holds columns
+// 16 md + 4 grp + e of row row0 + col.
+template <int MD, bool F16>
+__device__ __forceinline__ void add_unbounded(const TreeParams& p, int64_t b, int h, int j0, int j1, int row,
+                                              v4f (&o)[MD]) {
+    const int tq = min(row, p.M - 1) / p.G, grp = (threadIdx.x & 63) >> 4;
+#pragma unroll 1
+    for (int j = j0; j < j1; ++j) {
+        const bool seen = p.mask ? p.mask[b * p.m_sb + tq * p.m_sl + j] != 0 : j <= tq;
+        const uint16_t* v = p.dv + b * p.dv_sb + j * p.dv_sn + h * p.dv_sh + 4 * grp;
+#pragma unroll
+        for (int md = 0; md < MD; ++md) {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(v + 16 * md);
+            const float f[4] = {Elem<F16>::lo(x.x), Elem<F16>::hi(x.x), Elem<F16>::lo(x.y), Elem<F16>::hi(x.y)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (seen && !(__builtin_fabsf(f[e]) < __builtin_inff())) o[md][e] += f[e];
+        }
+    }
+}
+
+// Query rows row0 + 16 nt + col as MFMA operands, zero past the last one.
+template <int KS, int NT>
+__device__ __forceinline__ void load_queries(const TreeParams& p, int64_t b, int h, int row0, u32x4 (&qr)[NT][KS]) {
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = row0 + 16 * nt + col;
+        const int r = min(row, p.M - 1), t = r / p.G, g = r - t * p.G;
+        const uint16_t* src = p.q + b * p.q_sb + t * p.q_sl + (int64_t)(h * p.G + g) * p.q_sh + 8 * grp;
+        const bool ok = row < p.M;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(src + 32 * kk);
+            qr[nt][kk] = u32x4{ok ? x.x : 0u, ok ? x.y : 0u, ok ? x.z : 0u, ok ? x.w : 0u};
+        }
+    }
+}
+
+// One online-softmax step of a column's scores: the scores become weights, the
+// state moves to the new maximum.  The weights' sum is fp32 and of the
+// unrounded weights; a lane keeps the sum of its own keys.
+template <int MT, int MD>
+__device__ __forceinline__ void softmax_step(v4f (&s)[MT], float scale_log2, float& m, float& l, v4f (&o)[MD]) {
+    float mx = kNegInf;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][i]);
+    mx = rows_max(mx);
+    const float m_new = fmaxf(m, mx * scale_log2);
+    const float base = m_new == kNegInf ? 0.f : m_new;
+    const float alpha = fast_exp2(m - base);
+    m = m_new;
+    float sum = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[mt][i] = fast_exp2(__builtin_fmaf(s[mt][i], scale_log2, -base));
+            sum += s[mt][i];
+        }
+    if (__ballot(alpha != 1.f)) {
+#pragma unroll
+        for (int md = 0; md < MD; ++md) o[md] *= alpha;
+        l *= alpha;
+    }
+    l += sum;
+}
+
+// A finished row set: the output where the item lies in this run alone, else a
+// partial entry of `rows` rows.  l is summed over the lane groups.
+template <int MD, bool F16>
+__device__ __forceinline__ void finish_rows(const TreeParams& p, int64_t b, int h, int row, int in, int rows, bool whole,
+                                            float* part, float m, float l, const v4f (&o)[MD]) {
+    using E = Elem<F16>;
+    constexpr int D = 16 * MD;
+    const int grp = (threadIdx.x & 63) >> 4;
+    if (row >= p.M) return;
+    if (!whole) {
+#pragma unroll
+        for (int md = 0; md < MD; ++md) *reinterpret_cast<v4f*>(part + in * D + 16 * md + 4 * grp) = o[md];
+        if (grp == 0) {
+            part[rows * D + in] = m;
+            part[rows * D + rows + in] = l;
+        }
+        return;
+    }
+    const int tq = row / p.G, g = row - tq * p.G;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* dst = p.out + b * p.o_sb + tq * p.o_sl + (int64_t)(h * p.G + g) * p.o_sh + 4 * grp;
+#pragma unroll
+    for (int md = 0; md < MD; ++md)
+        *reinterpret_cast<u32x2*>(dst + 16 * md) =
+            u32x2{E::pack(o[md][0] * inv, o[md][1] * inv), E::pack(o[md][2] * inv, o[md][3] * inv)};
+    if (p.lse && grp == 0) p.lse[(b * p.Hq + h * p.G + g) * p.T + tq] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+}
+
+// Joins the states of KW key waves in those of wave 0: the others leave theirs
+// in LDS (entries of `rows` rows).  Every wave calls it.
+template <int MD, int NT, int KW>
+__device__ __forceinline__ void join_keys(float* lds, int rows, int row0, int kw, float (&m)[NT], float (&l)[NT],
+                                          v4f (&o)[NT][MD]) {
+    constexpr int D = 16 * MD;
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    const int size = rows * (D + 2);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) l[nt] = rows_sum(l[nt]);
+    if constexpr (KW == 1) return;
+    if (kw > 0) {
+        float* e = lds + (kw - 1) * size;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int row = row0 + 16 * nt + col;
+#pragma unroll
+            for (int md = 0; md < MD; ++md) *reinterpret_cast<v4f*>(e + row * D + 16 * md + 4 * grp) = o[nt][md];
+            if (grp == 0) {
+                e[rows * D + row] = m[nt];
+                e[rows * D + rows + row] = l[nt];
+            }
+        }
+    }
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = row0 + 16 * nt + col;
+        float top = m[nt];
+#pragma unroll
+        for (int x = 0; x < KW - 1; ++x) top = fmaxf(top, lds[x * size + rows * D + row]);
+        const float base = top == kNegInf ? 0.f : top;
+        const float own = fast_exp2(m[nt] - base);
+        l[nt] *= own;
+#pragma unroll
+        for (int md = 0; md < MD; ++md) o[nt][md] *= own;
+        m[nt] = top;
+#pragma unroll
+        for (int x = 0; x < KW - 1; ++x) {
+            const float* e = lds + x * size;
+            const float f = fast_exp2(e[rows * D + row] - base);
+            l[nt] += f * e[rows * D + rows + row];
+#pragma unroll
+            for (int md = 0; md < MD; ++md) o[nt][md] += f * *reinterpret_cast<const v4f*>(e + row * D + 16 * md + 4 * grp);
+        }
+    }
+}
+
+// The run of a workgroup, item by item.
+struct Item {
+    int64_t b;
+    int h, n, t0, t1, tiles;
+};
+
+__device__ __forceinline__ Item item_at(const TreeParams& p, int64_t pos, int64_t end) {
+    const Place at = place_of(p, pos);
+    Item it;
+    it.b = at.b;
+    it.n = at.n;
+    it.tiles = at.tiles;
+    it.h = (int)((pos - at.first) / at.tiles);
+    it.t0 = (int)(pos - at.first - (int64_t)it.h * at.tiles);
+    it.t1 = (int)min<int64_t>(at.tiles, it.t0 + end - pos);
+    return it;
+}
+
+// ---------------------------------------------------------------------------
+// up to 32 query rows a KV head: bound by the cache's bytes
+// ---------------------------------------------------------------------------
+
+// A wave owns 16 keys of each tile and works for itself: their rows go straight
+// from memory to its own LDS ring (no registers, no barrier), the next tiles'
+// while one is computed.  A row's 16-byte pieces are exchanged by an XOR with
+// its number, so that the score operand (16 rows, one piece) and the transposed
+// reads of V (16 rows, two pieces) spread over all banks.
+template <int D>
+struct Ring {
+    static constexpr int kStages = 2;
+    static constexpr int kRowBytes = 2 * D;
+    static constexpr int kTile = 16 * kRowBytes;                 // K or V of a wave's 16 keys
+    static constexpr int kWave = kStages * 2 * kTile;
+    static constexpr int P = D / 8;                              // pieces a row
+    static constexpr int kLoads = kTile / 1024;                  // 1024 bytes a wave-wide load
+    // piece c of row r lies at slot c ^ twist(r)
+    static __device__ __forceinline__ int twist(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+};
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+__device__ __forceinline__ void load_to_lds(const uint16_t* src, char* dst) {
+    __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)dst, 16, 0, 0);
+}
+
+__device__ __forceinline__ u32x2 read_transposed(const char* p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p));
+}
+
+template <int D, bool F16, int NT, bool PAGED>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) tree_few_kernel(TreeParams p) {
+    using E = Elem<F16>;
+    using R = Ring<D>;
+    constexpr int KS = D / 32, MD = D / 16, kRows = 16 * NT, kPart = kRows * (D + 2);
+    constexpr int kBytes = 4 * R::kWave > 12 * kPart ? 4 * R::kWave : 12 * kPart;      // ring, or the join of three waves
+    __shared__ __attribute__((aligned(16))) char lds[kBytes];
+    __shared__ Pages pages;
+    __shared__ uint64_t seen[4][kRows];
+    __shared__ int wild;
+
+    const int64_t slot = (int64_t)(blockIdx.x % kXcdCount) * (gridDim.x / kXcdCount) + blockIdx.x / kXcdCount;
+    if (slot >= p.slots) return;
+    const int64_t total = total_tiles(p);
+    const int runs = used_runs(p, total), run = (int)slot;
+    if (run >= runs) return;
+    int64_t pos = run_begin(total, runs, run);
+    const int64_t end = run_begin(total, runs, run + 1);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    char* ring = lds + wave * R::kWave;
+    // this lane's piece of load x: row x * 64 / P + lane / P of the wave's keys
+    const int lrow = lane / R::P, lslot = lane % R::P;
+
+    while (pos < end) {
+        const Item it = item_at(p, pos, end);
+        const int64_t b = it.b;
+        const int whole_tiles = it.n / kKeys, cached = (it.n + kKeys - 1) / kKeys;
+        const int streamed = max(it.t0, min(it.t1, whole_tiles));        // tiles [t0, streamed) by the ring
+        const uint16_t* kb = p.c.k + it.h * p.c.k_sh;
+        const uint16_t* vb = p.c.v + it.h * p.c.v_sh;
+        if constexpr (!PAGED) {
+            kb += b * p.c.k_sb;
+            vb += b * p.c.v_sb;
+        }
+        int stretch = it.t0;                                             // first tile of the pages held
+        __syncthreads();                                                 // the item before is done with LDS
+        if (threadIdx.x == 0) wild = 0;
+        if constexpr (PAGED) {
+            if (it.t0 < cached) load_pages(p.c, b, it.t0, it.n, pages);
+        }
+        __syncthreads();
+
+        auto fetch = [&](int t) {                                        // a full tile's rows of this wave
+            char* ks = ring + (t & 1) * 2 * R::kTile;
+#pragma unroll
+            for (int x = 0; x < R::kLoads; ++x) {
+                const int r = x * (64 / R::P) + lrow, row = t * kKeys + 16 * wave + r;
+                const int piece = 8 * (lslot ^ R::twist(r));
+                RowAt at;
+                if constexpr (PAGED) at = paged_row(p.c, pages, stretch, row);
+                else at = RowAt{row * p.c.k_sn, row * p.c.v_sn};
+                load_to_lds(kb + at.k + piece, ks + 1024 * x);
+                load_to_lds(vb + at.v + piece, ks + R::kTile + 1024 * x);
+            }
+        };
+        u32x4 qr[NT][KS];
+        if (it.t0 < streamed) fetch(it.t0);
+        if (it.t0 + 1 < streamed) fetch(it.t0 + 1);
+        load_queries<KS, NT>(p, b, it.h, 0, qr);
+
+        v4f o[NT][MD];
+        float m[NT], l[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt] = kNegInf;
+            l[nt] = 0.f;
+#pragma unroll
+            for (int md = 0; md < MD; ++md) o[nt][md] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
+
+        // the wave's 16 keys of a tile at ks / vs; key i of the lane visible
+        // where bit i of `bits` of its column is set
+        auto compute = [&](const char* ks, auto visible) {
+            v4f s[NT][1];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                const u32x4 a = *reinterpret_cast<const u32x4*>(ks + col * R::kRowBytes + 16 * ((4 * kk + grp) ^ R::twist(col)));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[nt][0] = E::mma32(a, qr[nt][kk], s[nt][0]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[nt][0][i] = visible(nt, i) ? s[nt][0][i] : kNegInf;
+                softmax_step<1, MD>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
+            }
+            const char* vs = ks + R::kTile;
+            const int vrow = 4 * grp + (col >> 2);                       // the row this lane names for the transpose
+#pragma unroll
+            for (int md = 0; md < MD; ++md) {
+                const u32x2 a = read_transposed(vs + vrow * R::kRowBytes +
+                                                16 * ((2 * md + ((col & 3) >> 1)) ^ R::twist(vrow)) + 8 * (col & 1));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    o[nt][md] = E::mma16(a, u32x2{E::pack(s[nt][0][0], s[nt][0][1]), E::pack(s[nt][0][2], s[nt][0][3])},
+                                         o[nt][md]);
+            }
+        };
+
+        for (int t = it.t0; t < streamed; ++t) {
+            // the loads of tile t are done once only the next tile's are open
+            if (t + 1 < streamed) {
+                if constexpr (D == 128) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+                else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            compute(ring + (t & 1) * 2 * R::kTile, [](int, int) { return true; });
+            if (t + 2 < streamed) {
+                if constexpr (PAGED) {
+                    if (t + 2 >= stretch + page_tiles(p.c)) {
+                        __syncthreads();
+                        stretch = t + 2;
+                        load_pages(p.c, b, stretch, it.n, pages);
+                        __syncthreads();
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // tile t is read
+                fetch(t + 2);
+            }
+        }
+
+        // the cache's last rows and the drafted tokens pass through registers:
+        // rows that do not exist become zeros, values that are not finite are
+        // taken out of drafted rows
+        for (int t = streamed; t < it.t1; ++t) {
+            const bool draft = t >= cached;
+            const int first = (draft ? t - cached : t) * kKeys, rows = draft ? p.T : it.n;
+            if constexpr (PAGED) {
+                if (!draft && t >= stretch + page_tiles(p.c)) {
+                    __syncthreads();
+                    stretch = t;
+                    load_pages(p.c, b, stretch, it.n, pages);
+                    __syncthreads();
+                }
+            }
+            const int key0 = first + 16 * wave;
+            if (key0 >= rows) continue;
+            u32x4 x[2 * R::kLoads];
+#pragma unroll
+            for (int y = 0; y < R::kLoads; ++y) {
+                const int row = min(key0 + y * (64 / R::P) + lrow, rows - 1);
+                const uint16_t *ks, *vs;
+                if (draft) {
+                    ks = p.dk + b * p.dk_sb + row * p.dk_sn + it.h * p.dk_sh;
+                    vs = p.dv + b * p.dv_sb + row * p.dv_sn + it.h * p.dv_sh;
+                } else {
+                    RowAt at;
+                    if constexpr (PAGED) at = paged_row(p.c, pages, stretch, row);
+                    else at = RowAt{row * p.c.k_sn, row * p.c.v_sn};
+                    ks = kb + at.k;
+                    vs = vb + at.v;
+                }
+                x[2 * y] = *reinterpret_cast<const u32x4*>(ks + 8 * lslot);
+                x[2 * y + 1] = *reinterpret_cast<const u32x4*>(vs + 8 * lslot);
+            }
+            if (draft) drafted_seen(p, b, 0, kRows, first, seen[wave]);
+            bool bad = false;
+            wave_fence();
+#pragma unroll
+            for (int y = 0; y < R::kLoads; ++y) {
+                const int r = y * (64 / R::P) + lrow;
+                const bool in = key0 + r < rows;
+                u32x4 v = x[2 * y + 1];
+                if (draft) v = finite_only<F16>(v, &bad);
+                char* dst = ring + r * R::kRowBytes + 16 * (lslot ^ R::twist(r));
+                *reinterpret_cast<u32x4*>(dst) = x[2 * y];
+                *reinterpret_cast<u32x4*>(dst + R::kTile) = u32x4{in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u};
+            }
+            if (bad) wild = 1;
+            wave_fence();
+            uint32_t bits[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                bits[nt] = draft ? (uint32_t)(seen[wave][min(16 * nt + col, p.M - 1) / p.G] >> (16 * wave + 4 * grp)) & 15u
+                                 : (1u << max(0, min(4, rows - key0 - 4 * grp))) - 1;
+            compute(ring, [&](int nt, int i) { return (bits[nt] >> i & 1u) != 0; });
+            wave_fence();
+        }
+
+        __syncthreads();
+        join_keys<MD, NT, 4>(reinterpret_cast<float*>(lds), kRows, 0, wave, m, l, o);
+        if (wave == 0) {
+            float* part = p.part + (2 * slot + (it.t0 == 0)) * kPart;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int row = 16 * nt + col;
+                if (wild) add_unbounded<MD, F16>(p, b, it.h, 0, p.T, row, o[nt]);
+                finish_rows<MD, F16>(p, b, it.h, row, row, kRows, it.t0 == 0 && it.t1 == it.tiles, part, m[nt], l[nt], o[nt]);
+            }
+        }
+        pos += it.t1 - it.t0;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// more than 32 query rows a KV head: bound by the matrix cores
+// ---------------------------------------------------------------------------
+
+template <int D, int RW>
 struct Shape {
+    static constexpr int NT = 2;
     static constexpr int KW = 4 / RW;                      // waves side by side on a tile's keys
     static constexpr int MT = 4 / KW;                      // 16-key tiles a wave takes of a tile
     static constexpr int kRows = 16 * RW * NT;             // query rows of a workgroup
@@ -111,40 +600,12 @@ struct Shape {
     static constexpr int kPart = kRows * (D + 2);          // floats of one partial
 };
 
-// Where a tile's rows lie: row `first` is the tile's first, rows from `n` on do
-// not exist.
-struct Tile {
-    int first, n;
-    bool draft;
-};
-
 template <int KR>
 struct TileRegs {
     u32x4 k[KR], v[KR];
 };
 
-// The tile's rows KR kq + r (kq = thread / pieces a row), 16 bytes each of K
-// and V.  Rows past the last one read it again; store_tile zeroes them.
-template <int D, bool PAGED>
-__device__ __forceinline__ void load_tile(TileRegs<D / 32>& t, const TreeParams& p, const Tile& w, int64_t b, int h) {
-    constexpr int KR = D / 32, P = D / 8;
-    const int kq = threadIdx.x / P, c = 8 * (threadIdx.x % P);
-#pragma unroll
-    for (int r = 0; r < KR; ++r) {
-        const int row = min(w.first + KR * kq + r, w.n - 1);
-        const uint16_t *ks, *vs;
-        if (w.draft) {
-            ks = p.dk + b * p.dk_sb + row * p.dk_sn + h * p.dk_sh;
-            vs = p.dv + b * p.dv_sb + row * p.dv_sn + h * p.dv_sh;
-        } else {
-            const RowAt at = cache_row<PAGED>(p.c, b, row);
-            ks = p.c.k + at.k + h * p.c.k_sh;
-            vs = p.c.v + at.v + h * p.c.v_sh;
-        }
-        t.k[r] = *reinterpret_cast<const u32x4*>(ks + c);
-        t.v[r] = *reinterpret_cast<const u32x4*>(vs + c);
-    }
-}
+constexpr int kBufferWord3 = 0x00020000;                   // raw buffer, 32-bit data format
 
 __device__ __forceinline__ uint32_t pair_of(uint32_t a, uint32_t b, bool high) {
     return __builtin_amdgcn_perm(b, a, high ? 0x07060302u : 0x05040100u);
@@ -157,45 +618,18 @@ __device__ __forceinline__ int vt_pos(int key) {
     return 32 * step + 8 * g + 4 * half + j;
 }
 
-// K row-major, V transposed.  A drafted row may hold infinities or NaN that
-// some query rows must not see: `wild` is then set for the tile.
-template <int D, bool F16>
-__device__ __forceinline__ void store_tile(const TileRegs<D / 32>& t, const Tile& w, uint16_t* ks, uint16_t* vts,
-                                           int* wild) {
-    constexpr int KR = D / 32, P = D / 8, kKStride = D + 16, kVStride = kKeys + 8;
-    const int kq = threadIdx.x / P, c = 8 * (threadIdx.x % P);
-    u32x4 v[KR];
-    bool bad = false;
-#pragma unroll
-    for (int r = 0; r < KR; ++r) {
-        const bool in = w.first + KR * kq + r < w.n;
-        *reinterpret_cast<u32x4*>(ks + (KR * kq + r) * kKStride + c) = t.k[r];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[r][e] = in ? t.v[r][e] : 0u;
-            if (w.draft) bad |= Elem<F16>::unbounded(v[r][e]);
-        }
-    }
-    if (w.draft && bad) wild[w.first / kKeys] = 1;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        uint16_t* dst = vts + (c + e) * kVStride + vt_pos(KR * kq);
-#pragma unroll
-        for (int r = 0; r < KR; r += 2)
-            *reinterpret_cast<uint32_t*>(dst + r) = pair_of(v[r][e >> 1], v[r + 1][e >> 1], e & 1);
-    }
-}
-
-template <int D, bool F16, int RW, int NT, bool PAGED>
-__global__ void __launch_bounds__(256) tree_kernel(TreeParams p) {
-    using S = Shape<D, RW, NT>;
+template <int D, bool F16, int RW, bool PAGED>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) tree_many_kernel(TreeParams p) {
+    using S = Shape<D, RW>;
     using E = Elem<F16>;
-    constexpr int KS = D / 32, MD = D / 16, MT = S::MT;
+    constexpr int NT = S::NT, KS = D / 32, MD = D / 16, MT = S::MT, KR = S::KR, P = D / 8;
     constexpr int kBuf = kKeys * S::kKStride + D * S::kVStride;        // 16-bit elements of one tile
     constexpr int kJoin = S::KW > 1 ? (S::KW - 1) * S::kPart : 0;      // floats of the key waves' join
     constexpr int kBytes = 4 * kBuf > 4 * kJoin ? 4 * kBuf : 4 * kJoin;
     __shared__ __attribute__((aligned(16))) char lds[kBytes];
-    __shared__ int wild[kMaxDrafted / kKeys];             // drafted tiles with values that are not finite
+    __shared__ Pages pages;
+    __shared__ uint64_t seen[4][16 * NT];
+    __shared__ int wild;
     uint16_t* bufs = reinterpret_cast<uint16_t*>(lds);
 
     const int64_t slot = (int64_t)(blockIdx.x % kXcdCount) * (gridDim.x / kXcdCount) + blockIdx.x / kXcdCount;
@@ -211,61 +645,111 @@ __global__ void __launch_bounds__(256) tree_kernel(TreeParams p) {
     const int col = lane & 15, grp = lane >> 4;
     const int rw = wave % RW, kw = wave / RW;
     const int row0 = rb * S::kRows + rw * 16 * NT;        // the wave's first query row
+    const int key0 = kw * 16 * MT;                        // the wave's first key in a tile
+    const int kq = KR * (threadIdx.x / P), piece = 8 * (threadIdx.x % P);      // this thread's rows and piece
 
     while (pos < end) {
-        const Place at = place_of(p, pos);
-        const int64_t b = at.b;
-        const int h = (int)((pos - at.first) / at.tiles);
-        const int t0 = (int)(pos - at.first - (int64_t)h * at.tiles);
-        const int t1 = (int)min<int64_t>(at.tiles, t0 + end - pos);
-        const int cached = (at.n + kKeys - 1) / kKeys;     // the first drafted tile
-        auto tile = [&](int t) {
-            return t < cached ? Tile{t * kKeys, at.n, false} : Tile{(t - cached) * kKeys, p.T, true};
-        };
-
-        TileRegs<S::KR> tr;
-        load_tile<D, PAGED>(tr, p, tile(t0), b, h);
-        u32x4 qr[NT][KS];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int row = row0 + 16 * nt + col;
-            const int r = min(row, p.M - 1), t = r / p.G, g = r - t * p.G;
-            const uint16_t* src = p.q + b * p.q_sb + t * p.q_sl + (int64_t)(h * p.G + g) * p.q_sh + 8 * grp;
-#pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                const u32x4 x = *reinterpret_cast<const u32x4*>(src + 32 * kk);
-                const bool ok = row < p.M;
-                qr[nt][kk] = u32x4{ok ? x.x : 0u, ok ? x.y : 0u, ok ? x.z : 0u, ok ? x.w : 0u};
-            }
+        const Item it = item_at(p, pos, end);
+        const int64_t b = it.b;
+        const int cached = (it.n + kKeys - 1) / kKeys;     // the first drafted tile
+        int stretch = it.t0;
+        __syncthreads();                                   // the item before is done with LDS
+        if (threadIdx.x == 0) wild = 0;
+        if constexpr (PAGED) {
+            if (it.t0 < cached) load_pages(p.c, b, it.t0, it.n, pages);
         }
-        v4f o[MD][NT];
+        __syncthreads();
+
+        // Rows kq + r of a tile.  Dense and drafted rows through a buffer
+        // resource whose range ends with the rows, so that later ones read as
+        // zero; paged rows past the last read it again and are zeroed where
+        // they are stored.
+        TileRegs<KR> tr;
+        auto load = [&](int t) {
+            const bool draft = t >= cached;
+            if (PAGED && !draft) {
+                if (t >= stretch + page_tiles(p.c)) {
+                    __syncthreads();
+                    stretch = t;
+                    load_pages(p.c, b, stretch, it.n, pages);
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int r = 0; r < KR; ++r) {
+                    const RowAt at = paged_row(p.c, pages, stretch, min(t * kKeys + kq + r, it.n - 1));
+                    tr.k[r] = *reinterpret_cast<const u32x4*>(p.c.k + it.h * p.c.k_sh + at.k + piece);
+                    tr.v[r] = *reinterpret_cast<const u32x4*>(p.c.v + it.h * p.c.v_sh + at.v + piece);
+                }
+                return;
+            }
+            const int first = (draft ? t - cached : t) * kKeys, rows = min(kKeys, (draft ? p.T : it.n) - first);
+            const int64_t ksn = draft ? p.dk_sn : p.c.k_sn, vsn = draft ? p.dv_sn : p.c.v_sn;
+            const uint16_t* kb = draft ? p.dk + b * p.dk_sb + it.h * p.dk_sh : p.c.k + b * p.c.k_sb + it.h * p.c.k_sh;
+            const uint16_t* vb = draft ? p.dv + b * p.dv_sb + it.h * p.dv_sh : p.c.v + b * p.c.v_sb + it.h * p.c.v_sh;
+            const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kb + first * ksn), 0,
+                                                              (int)((rows - 1) * 2 * ksn + 2 * D), kBufferWord3);
+            const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vb + first * vsn), 0,
+                                                              (int)((rows - 1) * 2 * vsn + 2 * D), kBufferWord3);
+#pragma unroll
+            for (int r = 0; r < KR; ++r) {
+                const uint32_t past = kq + r < rows ? 0u : 0x80000000u;
+                tr.k[r] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                    rk, past | (uint32_t)(2 * ((kq + r) * (int)ksn + piece)), 0, 0));
+                tr.v[r] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                    rv, past | (uint32_t)(2 * ((kq + r) * (int)vsn + piece)), 0, 0));
+            }
+        };
+        // K row-major, V transposed
+        auto store = [&](int t) {
+            uint16_t* ks = bufs + (t & 1) * kBuf;
+            uint16_t* vts = ks + kKeys * S::kKStride;
+            const bool draft = t >= cached;
+            bool bad = false;
+#pragma unroll
+            for (int r = 0; r < KR; ++r) {
+                *reinterpret_cast<u32x4*>(ks + (kq + r) * S::kKStride + piece) = tr.k[r];
+                if (draft) tr.v[r] = finite_only<F16>(tr.v[r], &bad);
+                if (PAGED && !draft && t * kKeys + kKeys > it.n) {
+                    const bool in = t * kKeys + kq + r < it.n;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) tr.v[r][e] = in ? tr.v[r][e] : 0u;
+                }
+            }
+            if (bad) wild = 1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                uint16_t* dst = vts + (piece + e) * S::kVStride + vt_pos(kq);
+                if constexpr (KR == 4)
+                    *reinterpret_cast<u32x2*>(dst) = u32x2{pair_of(tr.v[0][e >> 1], tr.v[1][e >> 1], e & 1),
+                                                           pair_of(tr.v[2][e >> 1], tr.v[3][e >> 1], e & 1)};
+                else
+                    *reinterpret_cast<uint32_t*>(dst) = pair_of(tr.v[0][e >> 1], tr.v[1][e >> 1], e & 1);
+            }
+        };
+        load(it.t0);
+        u32x4 qr[NT][KS];
+        load_queries<KS, NT>(p, b, it.h, row0, qr);
+        v4f o[NT][MD];
         float m[NT], l[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt] = kNegInf;
             l[nt] = 0.f;
 #pragma unroll
-            for (int md = 0; md < MD; ++md) o[md][nt] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int md = 0; md < MD; ++md) o[nt][md] = v4f{0.f, 0.f, 0.f, 0.f};
         }
-
-        __syncthreads();                                   // the item before is done with the buffers
-        if (threadIdx.x < kMaxDrafted / kKeys) wild[threadIdx.x] = 0;
-        __syncthreads();
-        store_tile<D, F16>(tr, tile(t0), bufs + (t0 & 1) * kBuf, bufs + (t0 & 1) * kBuf + kKeys * S::kKStride, wild);
-        if (t0 + 1 < t1) load_tile<D, PAGED>(tr, p, tile(t0 + 1), b, h);
+        store(it.t0);
+        if (it.t0 + 1 < it.t1) load(it.t0 + 1);
         __syncthreads();
 
-        for (int t = t0; t < t1; ++t) {
-            const Tile w = tile(t);
+        for (int t = it.t0; t < it.t1; ++t) {
             const uint16_t* ks = bufs + (t & 1) * kBuf;
             const uint16_t* vts = ks + kKeys * S::kKStride;
-            const int key0 = kw * 16 * MT;                 // the wave's first key in the tile
-
-            v4f s[MT][NT];
+            v4f s[NT][MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) s[mt][nt] = v4f{0.f, 0.f, 0.f, 0.f};
+                for (int nt = 0; nt < NT; ++nt) s[nt][mt] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
@@ -273,200 +757,66 @@ __global__ void __launch_bounds__(256) tree_kernel(TreeParams p) {
                     const u32x4 a = *reinterpret_cast<const u32x4*>(ks + (key0 + 16 * mt + col) * S::kKStride + 32 * kk +
                                                                     8 * grp);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) s[mt][nt] = E::mma32(a, qr[nt][kk], s[mt][nt]);
+                    for (int nt = 0; nt < NT; ++nt) s[nt][mt] = E::mma32(a, qr[nt][kk], s[nt][mt]);
                 }
-
-            if (w.draft) {                                 // by the mask's bytes, or j <= t without one
+            if (t >= cached) {                             // by the mask
+                const int first = (t - cached) * kKeys, from = min(row0, p.M - 1) / p.G;
+                drafted_seen(p, b, row0, 16 * NT, first, seen[wave]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const int tq = min(row0 + 16 * nt + col, p.M - 1) / p.G;
-                    const uint8_t* mrow = p.mask + b * p.m_sb + tq * p.m_sl;
+                    const uint64_t word = seen[wave][min(row0 + 16 * nt + col, p.M - 1) / p.G - from] >> (key0 + 4 * grp);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int j = w.first + key0 + 16 * mt + 4 * grp + i;
-                            const bool seen = j < p.T && (p.mask ? mrow[min(j, p.T - 1)] != 0 : j <= tq);
-                            s[mt][nt][i] = seen ? s[mt][nt][i] : kNegInf;
-                        }
+                        for (int i = 0; i < 4; ++i) s[nt][mt][i] = word >> (16 * mt + i) & 1 ? s[nt][mt][i] : kNegInf;
                 }
-            } else if (w.first + kKeys > w.n) {
+            } else if (t * kKeys + kKeys > it.n) {
+                const int left = it.n - t * kKeys - key0 - 4 * grp;
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool seen = w.first + key0 + 16 * mt + 4 * grp + i < w.n;
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) s[mt][nt][i] = seen ? s[mt][nt][i] : kNegInf;
-                    }
+                        for (int i = 0; i < 4; ++i) s[nt][mt][i] = 16 * mt + i < left ? s[nt][mt][i] : kNegInf;
             }
-
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float mx = kNegInf;
+            for (int nt = 0; nt < NT; ++nt) softmax_step<MT, MD>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+            for (int ss = 0; ss < MT / 2; ++ss) {
+                u32x4 pb[NT];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][nt][i]);
-                mx = rows_max(mx);
-                const float m_new = fmaxf(m[nt], mx * p.scale_log2);
-                const float base = m_new == kNegInf ? 0.f : m_new;
-                const float alpha = fast_exp2(m[nt] - base);
-                m[nt] = m_new;
-                float sum = 0.f;
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[mt][nt][i] = fast_exp2(__builtin_fmaf(s[mt][nt][i], p.scale_log2, -base));
-                        sum += s[mt][nt][i];
-                    }
-                if (__ballot(alpha != 1.f)) {
-#pragma unroll
-                    for (int md = 0; md < MD; ++md) o[md][nt] *= alpha;
-                    l[nt] *= alpha;
-                }
-                l[nt] += sum;                              // fp32, of the unrounded weights
-            }
-
-            if (w.draft && wild[w.first / kKeys]) {
-                // drafted values that are not finite: weight by weight, so that a
-                // row takes nothing from a token it does not see
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        for (int g = 0; g < 4; ++g) {
-                            const int j = w.first + key0 + 16 * mt + 4 * g + i;
-                            if (j >= p.T) continue;
-                            const uint16_t* vrow = p.dv + b * p.dv_sb + j * p.dv_sn + h * p.dv_sh + 4 * grp;
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const float pj = __shfl(s[mt][nt][i], col + 16 * g, 64);
-#pragma unroll
-                                for (int md = 0; md < MD; ++md) {
-                                    const u32x2 x = *reinterpret_cast<const u32x2*>(vrow + 16 * md);
-                                    const float vals[4] = {E::lo(x.x), E::hi(x.x), E::lo(x.y), E::hi(x.y)};
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) o[md][nt][e] += pj == 0.f ? 0.f : pj * vals[e];
-                                }
-                            }
-                        }
-            } else if constexpr (MT == 1) {                // 16 keys: half a step
+                for (int nt = 0; nt < NT; ++nt)
+                    pb[nt] = u32x4{E::pack(s[nt][2 * ss][0], s[nt][2 * ss][1]), E::pack(s[nt][2 * ss][2], s[nt][2 * ss][3]),
+                                   E::pack(s[nt][2 * ss + 1][0], s[nt][2 * ss + 1][1]),
+                                   E::pack(s[nt][2 * ss + 1][2], s[nt][2 * ss + 1][3])};
 #pragma unroll
                 for (int md = 0; md < MD; ++md) {
-                    const u32x2 a = *reinterpret_cast<const u32x2*>(vts + (16 * md + col) * S::kVStride +
-                                                                    32 * (kw >> 1) + 8 * grp + 4 * (kw & 1));
+                    const u32x4 a = *reinterpret_cast<const u32x4*>(vts + (16 * md + col) * S::kVStride + key0 + 32 * ss +
+                                                                    8 * grp);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        o[md][nt] = E::mma16(a, u32x2{E::pack(s[0][nt][0], s[0][nt][1]), E::pack(s[0][nt][2], s[0][nt][3])},
-                                             o[md][nt]);
-                }
-            } else {
-#pragma unroll
-                for (int ss = 0; ss < MT / 2; ++ss) {
-                    u32x4 pb[NT];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        pb[nt] = u32x4{E::pack(s[2 * ss][nt][0], s[2 * ss][nt][1]), E::pack(s[2 * ss][nt][2], s[2 * ss][nt][3]),
-                                       E::pack(s[2 * ss + 1][nt][0], s[2 * ss + 1][nt][1]),
-                                       E::pack(s[2 * ss + 1][nt][2], s[2 * ss + 1][nt][3])};
-#pragma unroll
-                    for (int md = 0; md < MD; ++md) {
-                        const u32x4 a = *reinterpret_cast<const u32x4*>(vts + (16 * md + col) * S::kVStride + key0 +
-                                                                        32 * ss + 8 * grp);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) o[md][nt] = E::mma32(a, pb[nt], o[md][nt]);
-                    }
+                    for (int nt = 0; nt < NT; ++nt) o[nt][md] = E::mma32(a, pb[nt], o[nt][md]);
                 }
             }
-
-            if (t + 1 < t1) {
-                uint16_t* next = bufs + ((t + 1) & 1) * kBuf;
-                store_tile<D, F16>(tr, tile(t + 1), next, next + kKeys * S::kKStride, wild);
-                if (t + 2 < t1) load_tile<D, PAGED>(tr, p, tile(t + 2), b, h);
+            if (t + 1 < it.t1) {
+                store(t + 1);
+                if (t + 2 < it.t1) load(t + 2);
             }
             __syncthreads();
         }
 
-        // the key waves' states joined in the first one's registers
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) l[nt] = rows_sum(l[nt]);
-        if constexpr (S::KW > 1) {
-            float* join = reinterpret_cast<float*>(lds);
-            if (kw > 0) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float* e = join + (kw - 1) * S::kPart;
-                    const int row = rw * 16 * NT + 16 * nt + col;
-#pragma unroll
-                    for (int md = 0; md < MD; ++md) *reinterpret_cast<v4f*>(e + row * D + 16 * md + 4 * grp) = o[md][nt];
-                    if (grp == 0) {
-                        e[S::kRows * D + row] = m[nt];
-                        e[S::kRows * D + S::kRows + row] = l[nt];
-                    }
-                }
-            }
-            __syncthreads();
-            if (kw == 0) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const int row = rw * 16 * NT + 16 * nt + col;
-                    float top = m[nt];
-#pragma unroll
-                    for (int x = 0; x < S::KW - 1; ++x) top = fmaxf(top, join[x * S::kPart + S::kRows * D + row]);
-                    const float base = top == kNegInf ? 0.f : top;
-                    const float own = fast_exp2(m[nt] - base);
-                    l[nt] *= own;
-#pragma unroll
-                    for (int md = 0; md < MD; ++md) o[md][nt] *= own;
-                    m[nt] = top;
-#pragma unroll
-                    for (int x = 0; x < S::KW - 1; ++x) {
-                        const float* e = join + x * S::kPart;
-                        const float f = fast_exp2(e[S::kRows * D + row] - base);
-                        l[nt] += f * e[S::kRows * D + S::kRows + row];
-#pragma unroll
-                        for (int md = 0; md < MD; ++md)
-                            o[md][nt] += f * *reinterpret_cast<const v4f*>(e + row * D + 16 * md + 4 * grp);
-                    }
-                }
-            }
-        }
-
+        join_keys<MD, NT, S::KW>(reinterpret_cast<float*>(lds), S::kRows, rw * 16 * NT, kw, m, l, o);
         if (kw == 0) {
-            if (t0 > 0 || t1 < at.tiles) {
-                float* part = p.part + (2 * slot + (t0 == 0)) * S::kPart;
+            float* part = p.part + (2 * slot + (it.t0 == 0)) * S::kPart;
+            const int j0 = max(0, it.t0 - cached) * kKeys, j1 = min(p.T, max(0, it.t1 - cached) * kKeys);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const int row = rw * 16 * NT + 16 * nt + col;
-                    if (rb * S::kRows + row >= p.M) continue;
-#pragma unroll
-                    for (int md = 0; md < MD; ++md) *reinterpret_cast<v4f*>(part + row * D + 16 * md + 4 * grp) = o[md][nt];
-                    if (grp == 0) {
-                        part[S::kRows * D + row] = m[nt];
-                        part[S::kRows * D + S::kRows + row] = l[nt];
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const int row = row0 + 16 * nt + col;
-                    if (row >= p.M) continue;
-                    const int tq = row / p.G, g = row - tq * p.G;
-                    const float inv = l[nt] == 0.f ? 0.f : 1.f / l[nt];
-                    uint16_t* dst = p.out + b * p.o_sb + tq * p.o_sl + (int64_t)(h * p.G + g) * p.o_sh + 4 * grp;
-#pragma unroll
-                    for (int md = 0; md < MD; ++md)
-                        *reinterpret_cast<u32x2*>(dst + 16 * md) = u32x2{E::pack(o[md][nt][0] * inv, o[md][nt][1] * inv),
-                                                                         E::pack(o[md][nt][2] * inv, o[md][nt][3] * inv)};
-                    if (p.lse && grp == 0)
-                        p.lse[(b * p.Hq + h * p.G + g) * p.T + tq] =
-                            l[nt] == 0.f ? kNegInf : (m[nt] + __log2f(l[nt])) * kLn2;
-                }
+            for (int nt = 0; nt < NT; ++nt) {
+                const int in = rw * 16 * NT + 16 * nt + col, row = rb * S::kRows + in;
+                if (wild) add_unbounded<MD, F16>(p, b, it.h, j0, j1, row, o[nt]);
+                finish_rows<MD, F16>(p, b, it.h, row, in, S::kRows, it.t0 == 0 && it.t1 == it.tiles, part, m[nt], l[nt],
+                                     o[nt]);
             }
         }
-        pos += t1 - t0;
+        pos += it.t1 - it.t0;
     }
 }
 
@@ -560,22 +910,19 @@ int check_tree(const slimkv_tree_attention_args* a) {
     return SLIMKV_OK;
 }
 
-template <int D, bool F16, int RW, int NT>
+template <int D, bool F16>
 void launch_tree(const TreeParams& p, const TreePlan& plan, hipStream_t st) {
     const dim3 grid((unsigned)((plan.slots + kXcdCount - 1) / kXcdCount * kXcdCount));
-    if (p.c.table) hipLaunchKernelGGL((tree_kernel<D, F16, RW, NT, true>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((tree_kernel<D, F16, RW, NT, false>), grid, dim3(256), 0, st, p);
+    const bool paged = p.c.table != nullptr;
+    void (*kernel)(TreeParams);
+    if (plan.rw == 4) kernel = paged ? tree_many_kernel<D, F16, 4, true> : tree_many_kernel<D, F16, 4, false>;
+    else if (plan.rw == 2) kernel = paged ? tree_many_kernel<D, F16, 2, true> : tree_many_kernel<D, F16, 2, false>;
+    else if (plan.nt == 2) kernel = paged ? tree_few_kernel<D, F16, 2, true> : tree_few_kernel<D, F16, 2, false>;
+    else kernel = paged ? tree_few_kernel<D, F16, 1, true> : tree_few_kernel<D, F16, 1, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p);
     const int chunks = (p.M + kMergeRows - 1) / kMergeRows;
     hipLaunchKernelGGL((tree_merge_kernel<D, F16>), dim3((unsigned)(p.B * p.Hk * chunks)), dim3(kMergeRows * D / 4), 0, st,
                        p, plan.rows(), chunks);
-}
-
-template <int D, bool F16>
-void launch_rows(const TreeParams& p, const TreePlan& plan, hipStream_t st) {
-    if (plan.rw == 4) launch_tree<D, F16, 4, 2>(p, plan, st);
-    else if (plan.rw == 2) launch_tree<D, F16, 2, 2>(p, plan, st);
-    else if (plan.nt == 2) launch_tree<D, F16, 1, 2>(p, plan, st);
-    else launch_tree<D, F16, 1, 1>(p, plan, st);
 }
 
 }  // namespace
@@ -592,7 +939,7 @@ int cache_view(const slimkv_cache_rows& r, int64_t batch, int64_t kv_heads, int6
     const std::string w(what);
     if (r.keys < 0 || r.keys > ((int64_t)1 << 30)) return fail(SLIMKV_EINVAL, w + ": invalid cache length");
     if (r.keys > 0 && (!r.k || (need_v && !r.v))) return fail(SLIMKV_EINVAL, w + ": null cache pointer");
-    if (r.table && (r.block_size <= 0 || r.num_blocks <= 0 || r.num_blocks > ((int64_t)1 << 40) || r.t_cols <= 0 ||
+    if (r.table && (r.block_size <= 0 || r.num_blocks <= 0 || r.num_blocks > 0x7fffffff || r.t_cols <= 0 ||
                     (batch > 1 && r.t_sb < r.t_cols && r.t_sb != 0) || r.block_size > ((int64_t)1 << 30) ||
                     r.t_cols > ((int64_t)1 << 30) || r.keys > r.t_cols * r.block_size))
         return fail(SLIMKV_EINVAL, w + ": invalid page layout (cache rows past the block table?)");
@@ -600,6 +947,9 @@ int cache_view(const slimkv_cache_rows& r, int64_t batch, int64_t kv_heads, int6
     if (r.keys > 0 && (!rows_aligned(r.k, {{outer, r.k_sb}, {rows, r.k_sn}, {kv_heads, r.k_sh}}) ||
                        (need_v && !rows_aligned(r.v, {{outer, r.v_sb}, {rows, r.v_sn}, {kv_heads, r.v_sh}}))))
         return fail(SLIMKV_EINVAL, w + ": cache rows must start on 16-byte boundaries (strides multiples of 8)");
+    for (int64_t s : {r.k_sn, need_v ? r.v_sn : 0})
+        if (rows > 1 && (s < 0 || s >= (1 << 23)))
+            return fail(SLIMKV_EUNSUP, w + ": cache rows must lie less than 2^23 elements apart");
     (void)head_dim;
     view->k = static_cast<const uint16_t*>(r.k); view->k_sb = r.k_sb; view->k_sn = r.k_sn; view->k_sh = r.k_sh;
     view->v = static_cast<const uint16_t*>(r.v); view->v_sb = r.v_sb; view->v_sn = r.v_sn; view->v_sh = r.v_sh;
@@ -635,6 +985,9 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
         !rows_aligned(a->draft_v, {{B, a->dv_sb}, {T, a->dv_sn}, {Hk, a->dv_sh}}) ||
         !rows_aligned(a->out, {{B, a->o_sb}, {T, a->o_sl}, {Hq, a->o_sh}}))
         return fail(SLIMKV_EINVAL, "tree attention: rows must start on 16-byte boundaries (strides multiples of 8)");
+    for (int64_t s : {a->dk_sn, a->dv_sn})
+        if (T > 1 && (s < 0 || s >= (1 << 23)))
+            return fail(SLIMKV_EUNSUP, "tree attention: drafted rows must lie less than 2^23 elements apart");
     const TreePlan plan = plan_tree(a);
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes(a->head_dim))
         return fail(SLIMKV_EWORKSPACE, "tree attention: workspace missing, misaligned or too small");
@@ -654,11 +1007,11 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
         return fail(SLIMKV_EINVAL, "tree attention: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->head_dim == 128) {
-        if (a->dtype == SLIMKV_DTYPE_F16) launch_rows<128, true>(p, plan, st);
-        else launch_rows<128, false>(p, plan, st);
+        if (a->dtype == SLIMKV_DTYPE_F16) launch_tree<128, true>(p, plan, st);
+        else launch_tree<128, false>(p, plan, st);
     } else {
-        if (a->dtype == SLIMKV_DTYPE_F16) launch_rows<64, true>(p, plan, st);
-        else launch_rows<64, false>(p, plan, st);
+        if (a->dtype == SLIMKV_DTYPE_F16) launch_tree<64, true>(p, plan, st);
+        else launch_tree<64, false>(p, plan, st);
     }
     return check_hip(hipGetLastError(), "tree attention launch");
 }
