@@ -59,9 +59,10 @@ def _dtype(name, *tensors):
 
 
 def _rows16(t):
-    """t, or a copy where its rows do not start on 16-byte boundaries."""
+    """t [B, rows, H, D], or a copy where its rows do not start on 16-byte boundaries, or overlap, or lie far apart."""
     good = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
-        all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride()))
+        all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride())) and \
+        (t.shape[1] <= 1 or t.shape[3] <= t.stride(1) < 1 << 23)
     return t if good else t.clone(memory_format=torch.contiguous_format)
 
 

@@ -39,6 +39,7 @@ struct TreeParams {
     float* lse;
     int B, T, Hq, Hk, G, M;               // M = T * G query rows of a KV head
     int row_blocks, runs, least;          // least: tiles a run takes at least
+    int together;                         // blocks of a multiple of 16 rows: the 16 rows a wave loads share one
     int64_t slots;                        // runs * row_blocks
     float scale_log2;
     float* part;
@@ -49,7 +50,15 @@ __device__ __forceinline__ int item_tiles(int n, int T) {
     return (n + kKeys - 1) / kKeys + (T + kKeys - 1) / kKeys;
 }
 
-// Tiles of all items (wave-uniform result, every lane active).
+// Values that are the same on every lane, in scalar registers: what follows
+// from them stays on the scalar unit, and buffer resources need no loop over
+// lanes.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
+}
+
+// Tiles of all items (every lane active).
 __device__ __forceinline__ int64_t total_tiles(const TreeParams& p) {
     const int lane = threadIdx.x & 63;
     int64_t sum = 0;
@@ -59,7 +68,7 @@ __device__ __forceinline__ int64_t total_tiles(const TreeParams& p) {
         for (int s = 1; s < 64; s <<= 1) x += __shfl_xor(x, s, 64);
         sum += x;
     }
-    return sum * p.Hk;
+    return uniform(sum) * p.Hk;
 }
 
 // Sequence that holds tile `pos`, the position of its first tile and its tiles
@@ -85,10 +94,11 @@ __device__ __forceinline__ Place place_of(const TreeParams& p, int64_t pos) {
         const uint64_t past = __ballot(pos < end);
         if (past) {
             const int at = __ffsll((unsigned long long)past) - 1;
-            const int tiles = __shfl(x, at, 64);
-            return Place{b0 + at, tiles, __shfl(n, at, 64), __shfl(end, at, 64) - (int64_t)tiles * p.Hk};
+            const int tiles = uniform(__shfl(x, at, 64));
+            return Place{uniform(b0 + at), tiles, uniform(__shfl(n, at, 64)),
+                         uniform(__shfl(end, at, 64)) - (int64_t)tiles * p.Hk};
         }
-        base = __shfl(end, 63, 64);
+        base = uniform(__shfl(end, 63, 64));
     }
     return Place{0, 1, 0, 0};             // not reached: pos < total_tiles
 }
@@ -98,7 +108,7 @@ __device__ __forceinline__ int used_runs(const TreeParams& p, int64_t total) {
     return (int)(most < p.runs ? most : p.runs);
 }
 
-__device__ __forceinline__ int64_t run_begin(int64_t total, int runs, int r) { return r * total / runs; }
+__device__ __forceinline__ int64_t run_begin(int64_t total, int runs, int r) { return uniform(r * total / runs); }
 
 // ---------------------------------------------------------------------------
 // what both kernels share
@@ -347,51 +357,168 @@ __device__ __forceinline__ Item item_at(const TreeParams& p, int64_t pos, int64_
     it.b = at.b;
     it.n = at.n;
     it.tiles = at.tiles;
-    it.h = (int)((pos - at.first) / at.tiles);
-    it.t0 = (int)(pos - at.first - (int64_t)it.h * at.tiles);
-    it.t1 = (int)min<int64_t>(at.tiles, it.t0 + end - pos);
+    it.h = uniform((int)((pos - at.first) / at.tiles));
+    it.t0 = uniform((int)(pos - at.first - (int64_t)it.h * at.tiles));
+    it.t1 = uniform((int)min<int64_t>(at.tiles, it.t0 + end - pos));
     return it;
 }
 
-// ---------------------------------------------------------------------------
-// up to 32 query rows a KV head: bound by the cache's bytes
-// ---------------------------------------------------------------------------
-
-// A wave owns 16 keys of each tile and works for itself: their rows go straight
-// from memory to its own LDS ring (no registers, no barrier), the next tiles'
-// while one is computed.  A row's 16-byte pieces are exchanged by an XOR with
-// its number, so that the score operand (16 rows, one piece) and the transposed
-// reads of V (16 rows, two pieces) spread over all banks.
+// The rows of 16 keys in LDS, as a wave loads them straight from memory (no
+// registers) or through registers.  A row's 16-byte pieces are exchanged by an
+// XOR with its number, so that the score operand (16 rows, one piece) and the
+// transposed reads of V (16 rows, two pieces) spread over all banks.
 template <int D>
-struct Ring {
-    static constexpr int kStages = 2;
+struct Rows16 {
     static constexpr int kRowBytes = 2 * D;
-    static constexpr int kTile = 16 * kRowBytes;                 // K or V of a wave's 16 keys
-    static constexpr int kWave = kStages * 2 * kTile;
+    static constexpr int kBytes = 16 * kRowBytes;                // K or V of 16 keys
     static constexpr int P = D / 8;                              // pieces a row
-    static constexpr int kLoads = kTile / 1024;                  // 1024 bytes a wave-wide load
+    static constexpr int kLoads = kBytes / 1024;                 // 1024 bytes a wave-wide load
     // piece c of row r lies at slot c ^ twist(r)
     static __device__ __forceinline__ int twist(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
 };
 
 typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
-__device__ __forceinline__ void load_to_lds(const uint16_t* src, char* dst) {
-    __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)dst, 16, 0, 0);
+// 16 bytes a lane from base + offset to 1024 consecutive bytes of LDS at dst
+// (wave-uniform).  Written out because the compiler, which orders LDS reads of
+// its own behind every such load it knows of, would empty the pipeline; the
+// waits are the caller's.  No register is written.
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t offset, char* dst) {
+    const uint32_t at = (uint32_t)uniform((int)(uintptr_t)(lds_void*)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base)
+                 : "memory");
+}
+__device__ __forceinline__ void load_to_lds(const char* src, char* dst) {
+    const uint32_t at = (uint32_t)uniform((int)(uintptr_t)(lds_void*)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory");
 }
 
 __device__ __forceinline__ u32x2 read_transposed(const char* p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p));
 }
 
+// Score operand: row col of 16 rows at `ks`, pieces 4 kk + grp.
+template <int D>
+__device__ __forceinline__ u32x4 key_operand(const char* ks, int kk) {
+    using R = Rows16<D>;
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    return *reinterpret_cast<const u32x4*>(ks + col * R::kRowBytes + 16 * ((4 * kk + grp) ^ R::twist(col)));
+}
+
+// Columns 16 md + col of rows 4 grp .. 4 grp + 3 of the 16 rows at `vs`.
+template <int D>
+__device__ __forceinline__ u32x2 value_operand(const char* vs, int md) {
+    using R = Rows16<D>;
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    const int row = 4 * grp + (col >> 2);                        // the row this lane names for the transpose
+    return read_transposed(vs + row * R::kRowBytes + 16 * ((2 * md + ((col & 3) >> 1)) ^ R::twist(row)) + 8 * (col & 1));
+}
+
+// A wave's view of the cache rows of one item: 16 consecutive rows into LDS.
+// Where the 16 rows lie in one tensor or in
+// one block, their first row is found on the scalar unit and a lane adds the
+// same offsets each time.
+template <int D, bool PAGED>
+struct RowLoader {
+    using R = Rows16<D>;
+    const char *kb, *vb;
+    uint32_t ko[R::kLoads], vo[R::kLoads];
+    int lrow, lslot;
+
+    __device__ __forceinline__ RowLoader(const TreeParams& p) {
+        const int lane = threadIdx.x & 63;
+        lrow = lane / R::P;
+        lslot = lane % R::P;
+#pragma unroll
+        for (int x = 0; x < R::kLoads; ++x) {
+            const int r = x * (64 / R::P) + lrow, piece = 16 * (lslot ^ R::twist(r));
+            ko[x] = 2 * r * (uint32_t)p.c.k_sn + piece;
+            vo[x] = 2 * r * (uint32_t)p.c.v_sn + piece;
+        }
+    }
+    __device__ __forceinline__ void item(const TreeParams& p, int64_t b, int h) {
+        kb = reinterpret_cast<const char*>(p.c.k + h * p.c.k_sh + (PAGED ? 0 : b * p.c.k_sb));
+        vb = reinterpret_cast<const char*>(p.c.v + h * p.c.v_sh + (PAGED ? 0 : b * p.c.v_sb));
+    }
+    // K (V false) or V of rows row .. row + 15
+    template <bool V>
+    __device__ __forceinline__ void load(const TreeParams& p, const Pages& pages, int stretch, int row, char* dst) const {
+        const char* base = V ? vb : kb;
+        if (!PAGED || p.together) {
+            int64_t at;
+            if constexpr (PAGED) {
+                const RowAt r = paged_row(p.c, pages, stretch, row);
+                at = uniform(V ? r.v : r.k);
+            } else {
+                at = row * (V ? p.c.v_sn : p.c.k_sn);
+            }
+            base += 2 * at;
+#pragma unroll
+            for (int x = 0; x < R::kLoads; ++x) load_to_lds(base, V ? vo[x] : ko[x], dst + 1024 * x);
+            return;
+        }
+#pragma unroll
+        for (int x = 0; x < R::kLoads; ++x) {
+            const int r = x * (64 / R::P) + lrow, piece = 16 * (lslot ^ R::twist(r));
+            const RowAt at = paged_row(p.c, pages, stretch, row + r);
+            load_to_lds(base + 2 * (V ? at.v : at.k) + piece, dst + 1024 * x);
+        }
+    }
+};
+
+// The 16 rows from key0 on (draft: drafted ones) through registers, for rows
+// that end before the 16th and for drafted values that are not finite: what
+// does not exist becomes zero.  Returns whether a value was taken out.
+template <int D, bool F16, bool PAGED>
+__device__ __forceinline__ bool stage_rows(const TreeParams& p, const Item& it, const Pages& pages, int stretch,
+                                           bool draft, int key0, char* dst, int apart) {
+    using R = Rows16<D>;
+    const int lane = threadIdx.x & 63, lrow = lane / R::P, lslot = lane % R::P, rows = draft ? p.T : it.n;
+    bool bad = false;
+    u32x4 x[2 * R::kLoads];
+#pragma unroll
+    for (int y = 0; y < R::kLoads; ++y) {
+        const int row = min(key0 + y * (64 / R::P) + lrow, rows - 1);
+        const uint16_t *ks, *vs;
+        if (draft) {
+            ks = p.dk + it.b * p.dk_sb + row * p.dk_sn + it.h * p.dk_sh;
+            vs = p.dv + it.b * p.dv_sb + row * p.dv_sn + it.h * p.dv_sh;
+        } else {
+            RowAt at;
+            if constexpr (PAGED) at = paged_row(p.c, pages, stretch, row);
+            else at = RowAt{it.b * p.c.k_sb + row * p.c.k_sn, it.b * p.c.v_sb + row * p.c.v_sn};
+            ks = p.c.k + at.k + it.h * p.c.k_sh;
+            vs = p.c.v + at.v + it.h * p.c.v_sh;
+        }
+        x[2 * y] = *reinterpret_cast<const u32x4*>(ks + 8 * lslot);
+        x[2 * y + 1] = *reinterpret_cast<const u32x4*>(vs + 8 * lslot);
+    }
+#pragma unroll
+    for (int y = 0; y < R::kLoads; ++y) {
+        const int r = y * (64 / R::P) + lrow;
+        const bool in = key0 + r < rows;
+        u32x4 v = x[2 * y + 1];
+        if (draft) v = finite_only<F16>(v, &bad);
+        char* at = dst + r * R::kRowBytes + 16 * (lslot ^ R::twist(r));
+        *reinterpret_cast<u32x4*>(at) = x[2 * y];
+        *reinterpret_cast<u32x4*>(at + apart) = u32x4{in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u};
+    }
+    return bad;
+}
+
+// ---------------------------------------------------------------------------
+// up to 32 query rows a KV head: bound by the cache's bytes
+// ---------------------------------------------------------------------------
+
+// A wave owns 16 keys of each tile and works for itself on its own LDS ring,
+// without a barrier: the next two tiles are on their way while one is computed.
 template <int D, bool F16, int NT, bool PAGED>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) tree_few_kernel(TreeParams p) {
     using E = Elem<F16>;
-    using R = Ring<D>;
-    constexpr int KS = D / 32, MD = D / 16, kRows = 16 * NT, kPart = kRows * (D + 2);
-    constexpr int kBytes = 4 * R::kWave > 12 * kPart ? 4 * R::kWave : 12 * kPart;      // ring, or the join of three waves
+    using R = Rows16<D>;
+    constexpr int KS = D / 32, MD = D / 16, kRows = 16 * NT, kPart = kRows * (D + 2), kWave = 4 * R::kBytes;
+    constexpr int kBytes = 4 * kWave > 12 * kPart ? 4 * kWave : 12 * kPart;      // rings, or the join of three waves
     __shared__ __attribute__((aligned(16))) char lds[kBytes];
     __shared__ Pages pages;
     __shared__ uint64_t seen[4][kRows];
@@ -404,24 +531,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     if (run >= runs) return;
     int64_t pos = run_begin(total, runs, run);
     const int64_t end = run_begin(total, runs, run + 1);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    char* ring = lds + wave * R::kWave;
-    // this lane's piece of load x: row x * 64 / P + lane / P of the wave's keys
-    const int lrow = lane / R::P, lslot = lane % R::P;
+    char* ring = lds + wave * kWave;
+    RowLoader<D, PAGED> loader(p);
 
     while (pos < end) {
         const Item it = item_at(p, pos, end);
         const int64_t b = it.b;
         const int whole_tiles = it.n / kKeys, cached = (it.n + kKeys - 1) / kKeys;
         const int streamed = max(it.t0, min(it.t1, whole_tiles));        // tiles [t0, streamed) by the ring
-        const uint16_t* kb = p.c.k + it.h * p.c.k_sh;
-        const uint16_t* vb = p.c.v + it.h * p.c.v_sh;
-        if constexpr (!PAGED) {
-            kb += b * p.c.k_sb;
-            vb += b * p.c.v_sb;
-        }
         int stretch = it.t0;                                             // first tile of the pages held
+        loader.item(p, b, it.h);
         __syncthreads();                                                 // the item before is done with LDS
         if (threadIdx.x == 0) wild = 0;
         if constexpr (PAGED) {
@@ -429,18 +550,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
         }
         __syncthreads();
 
-        auto fetch = [&](int t) {                                        // a full tile's rows of this wave
-            char* ks = ring + (t & 1) * 2 * R::kTile;
-#pragma unroll
-            for (int x = 0; x < R::kLoads; ++x) {
-                const int r = x * (64 / R::P) + lrow, row = t * kKeys + 16 * wave + r;
-                const int piece = 8 * (lslot ^ R::twist(r));
-                RowAt at;
-                if constexpr (PAGED) at = paged_row(p.c, pages, stretch, row);
-                else at = RowAt{row * p.c.k_sn, row * p.c.v_sn};
-                load_to_lds(kb + at.k + piece, ks + 1024 * x);
-                load_to_lds(vb + at.v + piece, ks + R::kTile + 1024 * x);
-            }
+        auto fetch = [&](int t) {
+            char* dst = ring + (t & 1) * 2 * R::kBytes;
+            loader.template load<false>(p, pages, stretch, t * kKeys + 16 * wave, dst);
+            loader.template load<true>(p, pages, stretch, t * kKeys + 16 * wave, dst + R::kBytes);
         };
         u32x4 qr[NT][KS];
         if (it.t0 < streamed) fetch(it.t0);
@@ -457,15 +570,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
             for (int md = 0; md < MD; ++md) o[nt][md] = v4f{0.f, 0.f, 0.f, 0.f};
         }
 
-        // the wave's 16 keys of a tile at ks / vs; key i of the lane visible
-        // where bit i of `bits` of its column is set
+        // 16 keys at ks; visible(nt, i): key 4 grp + i for column col
         auto compute = [&](const char* ks, auto visible) {
             v4f s[NT][1];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[nt][0] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
-                const u32x4 a = *reinterpret_cast<const u32x4*>(ks + col * R::kRowBytes + 16 * ((4 * kk + grp) ^ R::twist(col)));
+                const u32x4 a = key_operand<D>(ks, kk);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[nt][0] = E::mma32(a, qr[nt][kk], s[nt][0]);
             }
@@ -475,12 +587,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
                 for (int i = 0; i < 4; ++i) s[nt][0][i] = visible(nt, i) ? s[nt][0][i] : kNegInf;
                 softmax_step<1, MD>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
             }
-            const char* vs = ks + R::kTile;
-            const int vrow = 4 * grp + (col >> 2);                       // the row this lane names for the transpose
 #pragma unroll
             for (int md = 0; md < MD; ++md) {
-                const u32x2 a = read_transposed(vs + vrow * R::kRowBytes +
-                                                16 * ((2 * md + ((col & 3) >> 1)) ^ R::twist(vrow)) + 8 * (col & 1));
+                const u32x2 a = value_operand<D>(ks + R::kBytes, md);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                     o[nt][md] = E::mma16(a, u32x2{E::pack(s[nt][0][0], s[nt][0][1]), E::pack(s[nt][0][2], s[nt][0][3])},
@@ -496,7 +605,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
             } else {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             }
-            compute(ring + (t & 1) * 2 * R::kTile, [](int, int) { return true; });
+            compute(ring + (t & 1) * 2 * R::kBytes, [](int, int) { return true; });
             if (t + 2 < streamed) {
                 if constexpr (PAGED) {
                     if (t + 2 >= stretch + page_tiles(p.c)) {
@@ -511,9 +620,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
             }
         }
 
-        // the cache's last rows and the drafted tokens pass through registers:
-        // rows that do not exist become zeros, values that are not finite are
-        // taken out of drafted rows
+        // the cache's last rows and the drafted tokens
         for (int t = streamed; t < it.t1; ++t) {
             const bool draft = t >= cached;
             const int first = (draft ? t - cached : t) * kKeys, rows = draft ? p.T : it.n;
@@ -527,38 +634,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
             }
             const int key0 = first + 16 * wave;
             if (key0 >= rows) continue;
-            u32x4 x[2 * R::kLoads];
-#pragma unroll
-            for (int y = 0; y < R::kLoads; ++y) {
-                const int row = min(key0 + y * (64 / R::P) + lrow, rows - 1);
-                const uint16_t *ks, *vs;
-                if (draft) {
-                    ks = p.dk + b * p.dk_sb + row * p.dk_sn + it.h * p.dk_sh;
-                    vs = p.dv + b * p.dv_sb + row * p.dv_sn + it.h * p.dv_sh;
-                } else {
-                    RowAt at;
-                    if constexpr (PAGED) at = paged_row(p.c, pages, stretch, row);
-                    else at = RowAt{row * p.c.k_sn, row * p.c.v_sn};
-                    ks = kb + at.k;
-                    vs = vb + at.v;
-                }
-                x[2 * y] = *reinterpret_cast<const u32x4*>(ks + 8 * lslot);
-                x[2 * y + 1] = *reinterpret_cast<const u32x4*>(vs + 8 * lslot);
-            }
             if (draft) drafted_seen(p, b, 0, kRows, first, seen[wave]);
-            bool bad = false;
             wave_fence();
-#pragma unroll
-            for (int y = 0; y < R::kLoads; ++y) {
-                const int r = y * (64 / R::P) + lrow;
-                const bool in = key0 + r < rows;
-                u32x4 v = x[2 * y + 1];
-                if (draft) v = finite_only<F16>(v, &bad);
-                char* dst = ring + r * R::kRowBytes + 16 * (lslot ^ R::twist(r));
-                *reinterpret_cast<u32x4*>(dst) = x[2 * y];
-                *reinterpret_cast<u32x4*>(dst + R::kTile) = u32x4{in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u};
-            }
-            if (bad) wild = 1;
+            if (stage_rows<D, F16, PAGED>(p, it, pages, stretch, draft, key0, ring, R::kBytes)) wild = 1;
             wave_fence();
             uint32_t bits[NT];
 #pragma unroll
@@ -588,49 +666,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
 // more than 32 query rows a KV head: bound by the matrix cores
 // ---------------------------------------------------------------------------
 
-template <int D, int RW>
-struct Shape {
-    static constexpr int NT = 2;
-    static constexpr int KW = 4 / RW;                      // waves side by side on a tile's keys
-    static constexpr int MT = 4 / KW;                      // 16-key tiles a wave takes of a tile
-    static constexpr int kRows = 16 * RW * NT;             // query rows of a workgroup
-    static constexpr int KR = D / 32;                      // rows a thread loads of a tile (one 16-byte piece each)
-    static constexpr int kKStride = D + 16;                // K tile row (16-bit elements)
-    static constexpr int kVStride = kKeys + 8;             // V^T tile row
-    static constexpr int kPart = kRows * (D + 2);          // floats of one partial
-};
-
-template <int KR>
-struct TileRegs {
-    u32x4 k[KR], v[KR];
-};
-
-constexpr int kBufferWord3 = 0x00020000;                   // raw buffer, 32-bit data format
-
-__device__ __forceinline__ uint32_t pair_of(uint32_t a, uint32_t b, bool high) {
-    return __builtin_amdgcn_perm(b, a, high ? 0x07060302u : 0x05040100u);
-}
-
-// V^T keeps, per 32-key step, the keys a lane group reads together side by
-// side: key 16 half + 4 g + j of the step at 8 g + 4 half + j.
-__device__ __forceinline__ int vt_pos(int key) {
-    const int step = key >> 5, half = (key >> 4) & 1, g = (key >> 2) & 3, j = key & 3;
-    return 32 * step + 8 * g + 4 * half + j;
-}
-
+// A tile of 64 rows lies in LDS as four groups of 16 (K, then V), each loaded by
+// one wave, two tiles side by side.
 template <int D, bool F16, int RW, bool PAGED>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) tree_many_kernel(TreeParams p) {
-    using S = Shape<D, RW>;
+    using R = Rows16<D>;
     using E = Elem<F16>;
-    constexpr int NT = S::NT, KS = D / 32, MD = D / 16, MT = S::MT, KR = S::KR, P = D / 8;
-    constexpr int kBuf = kKeys * S::kKStride + D * S::kVStride;        // 16-bit elements of one tile
-    constexpr int kJoin = S::KW > 1 ? (S::KW - 1) * S::kPart : 0;      // floats of the key waves' join
-    constexpr int kBytes = 4 * kBuf > 4 * kJoin ? 4 * kBuf : 4 * kJoin;
+    constexpr int NT = 2, KS = D / 32, MD = D / 16;
+    constexpr int KW = 4 / RW, MT = 4 / KW;                // waves side by side on a tile's keys, 16-key groups of each
+    constexpr int kRows = 16 * RW * NT, kPart = kRows * (D + 2);
+    constexpr int kTile = 8 * R::kBytes, kApart = 4 * R::kBytes;
+    constexpr int kJoin = KW > 1 ? 4 * (KW - 1) * kPart : 0;
+    constexpr int kBytes = 2 * kTile > kJoin ? 2 * kTile : kJoin;
     __shared__ __attribute__((aligned(16))) char lds[kBytes];
     __shared__ Pages pages;
     __shared__ uint64_t seen[4][16 * NT];
     __shared__ int wild;
-    uint16_t* bufs = reinterpret_cast<uint16_t*>(lds);
 
     const int64_t slot = (int64_t)(blockIdx.x % kXcdCount) * (gridDim.x / kXcdCount) + blockIdx.x / kXcdCount;
     if (slot >= p.slots) return;
@@ -641,92 +692,46 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     int64_t pos = run_begin(total, runs, run);
     const int64_t end = run_begin(total, runs, run + 1);
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int rw = wave % RW, kw = wave / RW;
-    const int row0 = rb * S::kRows + rw * 16 * NT;        // the wave's first query row
+    const int row0 = rb * kRows + rw * 16 * NT;           // the wave's first query row
     const int key0 = kw * 16 * MT;                        // the wave's first key in a tile
-    const int kq = KR * (threadIdx.x / P), piece = 8 * (threadIdx.x % P);      // this thread's rows and piece
+    RowLoader<D, PAGED> loader(p);
 
     while (pos < end) {
         const Item it = item_at(p, pos, end);
         const int64_t b = it.b;
-        const int cached = (it.n + kKeys - 1) / kKeys;     // the first drafted tile
+        const int whole_tiles = it.n / kKeys, cached = (it.n + kKeys - 1) / kKeys;
+        const int streamed = max(it.t0, min(it.t1, whole_tiles));        // tiles [t0, streamed) straight to LDS
         int stretch = it.t0;
+        loader.item(p, b, it.h);
         __syncthreads();                                   // the item before is done with LDS
         if (threadIdx.x == 0) wild = 0;
         if constexpr (PAGED) {
             if (it.t0 < cached) load_pages(p.c, b, it.t0, it.n, pages);
+            __syncthreads();
         }
-        __syncthreads();
-
-        // Rows kq + r of a tile.  Dense and drafted rows through a buffer
-        // resource whose range ends with the rows, so that later ones read as
-        // zero; paged rows past the last read it again and are zeroed where
-        // they are stored.
-        TileRegs<KR> tr;
-        auto load = [&](int t) {
-            const bool draft = t >= cached;
-            if (PAGED && !draft) {
-                if (t >= stretch + page_tiles(p.c)) {
+        auto fetch_k = [&](int t) {
+            if constexpr (PAGED) {
+                if (t >= stretch + page_tiles(p.c)) {      // V of the tiles before is on its way
                     __syncthreads();
                     stretch = t;
                     load_pages(p.c, b, stretch, it.n, pages);
                     __syncthreads();
                 }
-#pragma unroll
-                for (int r = 0; r < KR; ++r) {
-                    const RowAt at = paged_row(p.c, pages, stretch, min(t * kKeys + kq + r, it.n - 1));
-                    tr.k[r] = *reinterpret_cast<const u32x4*>(p.c.k + it.h * p.c.k_sh + at.k + piece);
-                    tr.v[r] = *reinterpret_cast<const u32x4*>(p.c.v + it.h * p.c.v_sh + at.v + piece);
-                }
-                return;
             }
-            const int first = (draft ? t - cached : t) * kKeys, rows = min(kKeys, (draft ? p.T : it.n) - first);
-            const int64_t ksn = draft ? p.dk_sn : p.c.k_sn, vsn = draft ? p.dv_sn : p.c.v_sn;
-            const uint16_t* kb = draft ? p.dk + b * p.dk_sb + it.h * p.dk_sh : p.c.k + b * p.c.k_sb + it.h * p.c.k_sh;
-            const uint16_t* vb = draft ? p.dv + b * p.dv_sb + it.h * p.dv_sh : p.c.v + b * p.c.v_sb + it.h * p.c.v_sh;
-            const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kb + first * ksn), 0,
-                                                              (int)((rows - 1) * 2 * ksn + 2 * D), kBufferWord3);
-            const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vb + first * vsn), 0,
-                                                              (int)((rows - 1) * 2 * vsn + 2 * D), kBufferWord3);
-#pragma unroll
-            for (int r = 0; r < KR; ++r) {
-                const uint32_t past = kq + r < rows ? 0u : 0x80000000u;
-                tr.k[r] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                    rk, past | (uint32_t)(2 * ((kq + r) * (int)ksn + piece)), 0, 0));
-                tr.v[r] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                    rv, past | (uint32_t)(2 * ((kq + r) * (int)vsn + piece)), 0, 0));
-            }
+            loader.template load<false>(p, pages, stretch, t * kKeys + 16 * wave, lds + (t & 1) * kTile + wave * R::kBytes);
         };
-        // K row-major, V transposed
-        auto store = [&](int t) {
-            uint16_t* ks = bufs + (t & 1) * kBuf;
-            uint16_t* vts = ks + kKeys * S::kKStride;
-            const bool draft = t >= cached;
-            bool bad = false;
-#pragma unroll
-            for (int r = 0; r < KR; ++r) {
-                *reinterpret_cast<u32x4*>(ks + (kq + r) * S::kKStride + piece) = tr.k[r];
-                if (draft) tr.v[r] = finite_only<F16>(tr.v[r], &bad);
-                if (PAGED && !draft && t * kKeys + kKeys > it.n) {
-                    const bool in = t * kKeys + kq + r < it.n;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) tr.v[r][e] = in ? tr.v[r][e] : 0u;
-                }
-            }
-            if (bad) wild = 1;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                uint16_t* dst = vts + (piece + e) * S::kVStride + vt_pos(kq);
-                if constexpr (KR == 4)
-                    *reinterpret_cast<u32x2*>(dst) = u32x2{pair_of(tr.v[0][e >> 1], tr.v[1][e >> 1], e & 1),
-                                                           pair_of(tr.v[2][e >> 1], tr.v[3][e >> 1], e & 1)};
-                else
-                    *reinterpret_cast<uint32_t*>(dst) = pair_of(tr.v[0][e >> 1], tr.v[1][e >> 1], e & 1);
-            }
+        auto fetch_v = [&](int t) {
+            loader.template load<true>(p, pages, stretch, t * kKeys + 16 * wave,
+                                       lds + (t & 1) * kTile + kApart + wave * R::kBytes);
         };
-        load(it.t0);
+        if (it.t0 < streamed) {
+            fetch_k(it.t0);
+            fetch_v(it.t0);
+        }
+        if (it.t0 + 1 < streamed) fetch_k(it.t0 + 1);
         u32x4 qr[NT][KS];
         load_queries<KS, NT>(p, b, it.h, row0, qr);
         v4f o[NT][MD];
@@ -738,81 +743,134 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
 #pragma unroll
             for (int md = 0; md < MD; ++md) o[nt][md] = v4f{0.f, 0.f, 0.f, 0.f};
         }
-        store(it.t0);
-        if (it.t0 + 1 < it.t1) load(it.t0 + 1);
-        __syncthreads();
 
-        for (int t = it.t0; t < it.t1; ++t) {
-            const uint16_t* ks = bufs + (t & 1) * kBuf;
-            const uint16_t* vts = ks + kKeys * S::kKStride;
-            v4f s[NT][MT];
+        // the wave's MT groups of 16 keys of the tile at `tile`: scores, softmax, values
+        auto scores = [&](const char* tile, v4f(&s)[NT][MT]) {
+            const char* ks = tile + kw * MT * R::kBytes;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[nt][mt] = v4f{0.f, 0.f, 0.f, 0.f};
+            u32x4 a[KS][MT];                               // two k-steps' rows asked for ahead of their products
+            auto read = [&](int kk) {
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk)
+                for (int mt = 0; mt < MT; ++mt) a[kk][mt] = key_operand<D>(ks + mt * R::kBytes, kk);
+            };
+            read(0);
+            read(1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const u32x4 a = *reinterpret_cast<const u32x4*>(ks + (key0 + 16 * mt + col) * S::kKStride + 32 * kk +
-                                                                    8 * grp);
+            for (int kk = 0; kk < KS; ++kk) {
+                if (kk + 2 < KS) read(kk + 2);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) s[nt][mt] = E::mma32(a, qr[nt][kk], s[nt][mt]);
-                }
-            if (t >= cached) {                             // by the mask
-                const int first = (t - cached) * kKeys, from = min(row0, p.M - 1) / p.G;
-                drafted_seen(p, b, row0, 16 * NT, first, seen[wave]);
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const uint64_t word = seen[wave][min(row0 + 16 * nt + col, p.M - 1) / p.G - from] >> (key0 + 4 * grp);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[nt][mt][i] = word >> (16 * mt + i) & 1 ? s[nt][mt][i] : kNegInf;
-                }
-            } else if (t * kKeys + kKeys > it.n) {
-                const int left = it.n - t * kKeys - key0 - 4 * grp;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[nt][mt][i] = 16 * mt + i < left ? s[nt][mt][i] : kNegInf;
+                    for (int nt = 0; nt < NT; ++nt) s[nt][mt] = E::mma32(a[kk][mt], qr[nt][kk], s[nt][mt]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        auto softmax = [&](v4f(&s)[NT][MT], u32x4(&pb)[MT / 2][NT]) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) softmax_step<MT, MD>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
+            for (int nt = 0; nt < NT; ++nt) {
+                softmax_step<MT, MD>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
 #pragma unroll
-            for (int ss = 0; ss < MT / 2; ++ss) {
-                u32x4 pb[NT];
+                for (int ss = 0; ss < MT / 2; ++ss)
+                    pb[ss][nt] =
+                        u32x4{E::pack(s[nt][2 * ss][0], s[nt][2 * ss][1]), E::pack(s[nt][2 * ss][2], s[nt][2 * ss][3]),
+                              E::pack(s[nt][2 * ss + 1][0], s[nt][2 * ss + 1][1]),
+                              E::pack(s[nt][2 * ss + 1][2], s[nt][2 * ss + 1][3])};
+            }
+        };
+        auto values = [&](const char* tile, const u32x4(&pb)[MT / 2][NT]) {
+            const char* vs = tile + kApart + kw * MT * R::kBytes;
+            constexpr int kGroups = MT / 2 * MD / 4;       // four 16-column operands a group, one group ahead
+            u32x4 a[kGroups][4];
+            auto read = [&](int g) {
+                const int ss = g / (MD / 4), m0 = g % (MD / 4) * 4;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    pb[nt] = u32x4{E::pack(s[nt][2 * ss][0], s[nt][2 * ss][1]), E::pack(s[nt][2 * ss][2], s[nt][2 * ss][3]),
-                                   E::pack(s[nt][2 * ss + 1][0], s[nt][2 * ss + 1][1]),
-                                   E::pack(s[nt][2 * ss + 1][2], s[nt][2 * ss + 1][3])};
-#pragma unroll
-                for (int md = 0; md < MD; ++md) {
-                    const u32x4 a = *reinterpret_cast<const u32x4*>(vts + (16 * md + col) * S::kVStride + key0 + 32 * ss +
-                                                                    8 * grp);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) o[nt][md] = E::mma32(a, pb[nt], o[nt][md]);
+                for (int i = 0; i < 4; ++i) {
+                    const u32x2 lo = value_operand<D>(vs + 2 * ss * R::kBytes, m0 + i);
+                    const u32x2 hi = value_operand<D>(vs + (2 * ss + 1) * R::kBytes, m0 + i);
+                    a[g][i] = u32x4{lo.x, lo.y, hi.x, hi.y};
                 }
+            };
+            read(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const int ss = g / (MD / 4), m0 = g % (MD / 4) * 4;
+                if (g + 1 < kGroups) read(g + 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) o[nt][m0 + i] = E::mma32(a[g][i], pb[ss][nt], o[nt][m0 + i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (t + 1 < it.t1) {
-                store(t + 1);
-                if (t + 2 < it.t1) load(t + 2);
-            }
-            __syncthreads();
-        }
+        };
 
-        join_keys<MD, NT, S::KW>(reinterpret_cast<float*>(lds), S::kRows, rw * 16 * NT, kw, m, l, o);
+        // K of tile t + 2 is asked for once all waves are past the scores of
+        // tile t, V of tile t + 1 once all are past the values of tile t - 1,
+        // so every load has one and a half tiles' time.  A wave waits for its
+        // own rows, by the number of younger loads, then for the others' at
+        // the barrier (whose LDS reads are done by then).
+        for (int t = it.t0; t < streamed; ++t) {
+            const bool more = t + 1 < streamed;
+            v4f s[NT][MT];
+            u32x4 pb[MT / 2][NT];
+            if (!more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(R::kLoads) : "memory");
+            else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * R::kLoads) : "memory");
+            if (more) fetch_v(t + 1);
+            scores(lds + (t & 1) * kTile, s);
+            softmax(s, pb);
+            if (!more) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * R::kLoads) : "memory");
+            if (t + 2 < streamed) fetch_k(t + 2);
+            values(lds + (t & 1) * kTile, pb);
+        }
+        // the cache's last rows and the drafted tokens
+        for (int t = streamed; t < it.t1; ++t) {
+            const bool draft = t >= cached;
+            const int first = (draft ? t - cached : t) * kKeys;
+            __syncthreads();
+            if constexpr (PAGED) {
+                if (!draft && t >= stretch + page_tiles(p.c)) {
+                    stretch = t;
+                    load_pages(p.c, b, stretch, it.n, pages);
+                    __syncthreads();
+                }
+            }
+            if (stage_rows<D, F16, PAGED>(p, it, pages, stretch, draft, first + 16 * wave, lds + wave * R::kBytes, kApart))
+                wild = 1;
+            if (draft) drafted_seen(p, b, row0, 16 * NT, first, seen[wave]);
+            __syncthreads();
+            v4f s[NT][MT];
+            u32x4 pb[MT / 2][NT];
+            scores(lds, s);
+            const int from = min(row0, p.M - 1) / p.G, left = it.n - first - key0 - 4 * grp;
+            const uint64_t all = left <= 0 ? 0 : left >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << left) - 1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint64_t word =
+                    draft ? seen[wave][min(row0 + 16 * nt + col, p.M - 1) / p.G - from] >> (key0 + 4 * grp) : all;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nt][mt][i] = word >> (16 * mt + i) & 1 ? s[nt][mt][i] : kNegInf;
+            }
+            softmax(s, pb);
+            values(lds, pb);
+        }
+        __syncthreads();
+
+        join_keys<MD, NT, KW>(reinterpret_cast<float*>(lds), kRows, rw * 16 * NT, kw, m, l, o);
         if (kw == 0) {
-            float* part = p.part + (2 * slot + (it.t0 == 0)) * S::kPart;
+            float* part = p.part + (2 * slot + (it.t0 == 0)) * kPart;
             const int j0 = max(0, it.t0 - cached) * kKeys, j1 = min(p.T, max(0, it.t1 - cached) * kKeys);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const int in = rw * 16 * NT + 16 * nt + col, row = rb * S::kRows + in;
+                const int in = rw * 16 * NT + 16 * nt + col, row = rb * kRows + in;
                 if (wild) add_unbounded<MD, F16>(p, b, it.h, j0, j1, row, o[nt]);
-                finish_rows<MD, F16>(p, b, it.h, row, in, S::kRows, it.t0 == 0 && it.t1 == it.tiles, part, m[nt], l[nt],
+                finish_rows<MD, F16>(p, b, it.h, row, in, kRows, it.t0 == 0 && it.t1 == it.tiles, part, m[nt], l[nt],
                                      o[nt]);
             }
         }
@@ -947,10 +1005,9 @@ int cache_view(const slimkv_cache_rows& r, int64_t batch, int64_t kv_heads, int6
     if (r.keys > 0 && (!rows_aligned(r.k, {{outer, r.k_sb}, {rows, r.k_sn}, {kv_heads, r.k_sh}}) ||
                        (need_v && !rows_aligned(r.v, {{outer, r.v_sb}, {rows, r.v_sn}, {kv_heads, r.v_sh}}))))
         return fail(SLIMKV_EINVAL, w + ": cache rows must start on 16-byte boundaries (strides multiples of 8)");
-    for (int64_t s : {r.k_sn, need_v ? r.v_sn : 0})
-        if (rows > 1 && (s < 0 || s >= (1 << 23)))
-            return fail(SLIMKV_EUNSUP, w + ": cache rows must lie less than 2^23 elements apart");
-    (void)head_dim;
+    for (int64_t s : {r.k_sn, need_v ? r.v_sn : r.k_sn})
+        if (rows > 1 && (s < head_dim || s >= (1 << 23)))
+            return fail(SLIMKV_EUNSUP, w + ": cache rows must lie [head_dim, 2^23) elements apart");
     view->k = static_cast<const uint16_t*>(r.k); view->k_sb = r.k_sb; view->k_sn = r.k_sn; view->k_sh = r.k_sh;
     view->v = static_cast<const uint16_t*>(r.v); view->v_sb = r.v_sb; view->v_sn = r.v_sn; view->v_sh = r.v_sh;
     view->table = r.table; view->t_sb = r.t_sb; view->num_blocks = r.num_blocks;
@@ -986,8 +1043,8 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
         !rows_aligned(a->out, {{B, a->o_sb}, {T, a->o_sl}, {Hq, a->o_sh}}))
         return fail(SLIMKV_EINVAL, "tree attention: rows must start on 16-byte boundaries (strides multiples of 8)");
     for (int64_t s : {a->dk_sn, a->dv_sn})
-        if (T > 1 && (s < 0 || s >= (1 << 23)))
-            return fail(SLIMKV_EUNSUP, "tree attention: drafted rows must lie less than 2^23 elements apart");
+        if (T > 1 && (s < a->head_dim || s >= (1 << 23)))
+            return fail(SLIMKV_EUNSUP, "tree attention: drafted rows must lie [head_dim, 2^23) elements apart");
     const TreePlan plan = plan_tree(a);
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes(a->head_dim))
         return fail(SLIMKV_EWORKSPACE, "tree attention: workspace missing, misaligned or too small");
@@ -1001,6 +1058,7 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     p.M = p.T * p.G;
     p.row_blocks = plan.row_blocks; p.runs = plan.runs; p.slots = plan.slots;
     p.least = 2;
+    p.together = a->cache.block_size % 16 == 0;
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.part = static_cast<float*>(workspace);
     if ((int64_t)p.B * p.Hk * ((p.M + kMergeRows - 1) / kMergeRows) > 0x7fffffff)
