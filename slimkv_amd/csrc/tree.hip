@@ -26,7 +26,6 @@ namespace slimkv {
 namespace {
 
 constexpr int kKeys = 64;                 // keys per tile
-constexpr int kMergeRows = 8;             // query rows per merge workgroup
 constexpr int kMaxDrafted = 1024;
 
 struct TreeParams {
@@ -39,7 +38,6 @@ struct TreeParams {
     float* lse;
     int B, T, Hq, Hk, G, M;               // M = T * G query rows of a KV head
     int row_blocks, runs, least;          // least: tiles a run takes at least
-    int together;                         // blocks of a multiple of 16 rows: the 16 rows a wave loads share one
     int64_t slots;                        // runs * row_blocks
     float scale_log2;
     float* part;
@@ -415,11 +413,16 @@ __device__ __forceinline__ u32x2 value_operand(const char* vs, int md) {
     return read_transposed(vs + row * R::kRowBytes + 16 * ((2 * md + ((col & 3) >> 1)) ^ R::twist(row)) + 8 * (col & 1));
 }
 
+// Where the rows of a cache lie: in one tensor, in blocks of a multiple of 16
+// rows (the 16 rows that a wave loads at a time share one), in blocks of any
+// size.
+constexpr int kDense = 0, kBlocks16 = 1, kAnyBlocks = 2;
+
 // A wave's view of the cache rows of one item: 16 consecutive rows into LDS.
 // Where the 16 rows lie in one tensor or in
 // one block, their first row is found on the scalar unit and a lane adds the
 // same offsets each time.
-template <int D, bool PAGED>
+template <int D, int PAGED>
 struct RowLoader {
     using R = Rows16<D>;
     const char *kb, *vb;
@@ -445,7 +448,7 @@ struct RowLoader {
     template <bool V>
     __device__ __forceinline__ void load(const TreeParams& p, const Pages& pages, int stretch, int row, char* dst) const {
         const char* base = V ? vb : kb;
-        if (!PAGED || p.together) {
+        if constexpr (PAGED != kAnyBlocks) {
             int64_t at;
             if constexpr (PAGED) {
                 const RowAt r = paged_row(p.c, pages, stretch, row);
@@ -456,56 +459,63 @@ struct RowLoader {
             base += 2 * at;
 #pragma unroll
             for (int x = 0; x < R::kLoads; ++x) load_to_lds(base, V ? vo[x] : ko[x], dst + 1024 * x);
-            return;
-        }
+        } else {
 #pragma unroll
-        for (int x = 0; x < R::kLoads; ++x) {
-            const int r = x * (64 / R::P) + lrow, piece = 16 * (lslot ^ R::twist(r));
-            const RowAt at = paged_row(p.c, pages, stretch, row + r);
-            load_to_lds(base + 2 * (V ? at.v : at.k) + piece, dst + 1024 * x);
+            for (int x = 0; x < R::kLoads; ++x) {
+                const int r = x * (64 / R::P) + lrow, piece = 16 * (lslot ^ R::twist(r));
+                const RowAt at = paged_row(p.c, pages, stretch, row + r);
+                load_to_lds(base + 2 * (V ? at.v : at.k) + piece, dst + 1024 * x);
+            }
         }
     }
 };
 
 // The 16 rows from key0 on (draft: drafted ones) through registers, for rows
 // that end before the 16th and for drafted values that are not finite: what
-// does not exist becomes zero.  Returns whether a value was taken out.
-template <int D, bool F16, bool PAGED>
-__device__ __forceinline__ bool stage_rows(const TreeParams& p, const Item& it, const Pages& pages, int stretch,
-                                           bool draft, int key0, char* dst, int apart) {
+// does not exist becomes zero.
+template <int D, bool F16, int PAGED>
+struct StagedRows {
     using R = Rows16<D>;
-    const int lane = threadIdx.x & 63, lrow = lane / R::P, lslot = lane % R::P, rows = draft ? p.T : it.n;
-    bool bad = false;
-    u32x4 x[2 * R::kLoads];
+    u32x4 k[R::kLoads], v[R::kLoads];
+
+    __device__ __forceinline__ void load(const TreeParams& p, const Item& it, const Pages& pages, int stretch, bool draft,
+                                         int key0) {
+        const int lane = threadIdx.x & 63, lrow = lane / R::P, lslot = lane % R::P, rows = draft ? p.T : it.n;
 #pragma unroll
-    for (int y = 0; y < R::kLoads; ++y) {
-        const int row = min(key0 + y * (64 / R::P) + lrow, rows - 1);
-        const uint16_t *ks, *vs;
-        if (draft) {
-            ks = p.dk + it.b * p.dk_sb + row * p.dk_sn + it.h * p.dk_sh;
-            vs = p.dv + it.b * p.dv_sb + row * p.dv_sn + it.h * p.dv_sh;
-        } else {
-            RowAt at;
-            if constexpr (PAGED) at = paged_row(p.c, pages, stretch, row);
-            else at = RowAt{it.b * p.c.k_sb + row * p.c.k_sn, it.b * p.c.v_sb + row * p.c.v_sn};
-            ks = p.c.k + at.k + it.h * p.c.k_sh;
-            vs = p.c.v + at.v + it.h * p.c.v_sh;
+        for (int y = 0; y < R::kLoads; ++y) {
+            const int row = min(key0 + y * (64 / R::P) + lrow, rows - 1);
+            const uint16_t *ks, *vs;
+            if (draft) {
+                ks = p.dk + it.b * p.dk_sb + row * p.dk_sn + it.h * p.dk_sh;
+                vs = p.dv + it.b * p.dv_sb + row * p.dv_sn + it.h * p.dv_sh;
+            } else {
+                RowAt at;
+                if constexpr (PAGED) at = paged_row(p.c, pages, stretch, row);
+                else at = RowAt{it.b * p.c.k_sb + row * p.c.k_sn, it.b * p.c.v_sb + row * p.c.v_sn};
+                ks = p.c.k + at.k + it.h * p.c.k_sh;
+                vs = p.c.v + at.v + it.h * p.c.v_sh;
+            }
+            k[y] = *reinterpret_cast<const u32x4*>(ks + 8 * lslot);
+            v[y] = *reinterpret_cast<const u32x4*>(vs + 8 * lslot);
         }
-        x[2 * y] = *reinterpret_cast<const u32x4*>(ks + 8 * lslot);
-        x[2 * y + 1] = *reinterpret_cast<const u32x4*>(vs + 8 * lslot);
     }
+    // Returns whether a value was taken out.
+    __device__ __forceinline__ bool store(bool draft, int left, char* dst, int apart) {
+        const int lane = threadIdx.x & 63, lrow = lane / R::P, lslot = lane % R::P;
+        bool bad = false;
 #pragma unroll
-    for (int y = 0; y < R::kLoads; ++y) {
-        const int r = y * (64 / R::P) + lrow;
-        const bool in = key0 + r < rows;
-        u32x4 v = x[2 * y + 1];
-        if (draft) v = finite_only<F16>(v, &bad);
-        char* at = dst + r * R::kRowBytes + 16 * (lslot ^ R::twist(r));
-        *reinterpret_cast<u32x4*>(at) = x[2 * y];
-        *reinterpret_cast<u32x4*>(at + apart) = u32x4{in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u};
+        for (int y = 0; y < R::kLoads; ++y) {
+            const int r = y * (64 / R::P) + lrow;
+            const bool in = r < left;
+            u32x4 x = v[y];
+            if (draft) x = finite_only<F16>(x, &bad);
+            char* at = dst + r * R::kRowBytes + 16 * (lslot ^ R::twist(r));
+            *reinterpret_cast<u32x4*>(at) = k[y];
+            *reinterpret_cast<u32x4*>(at + apart) = u32x4{in ? x.x : 0u, in ? x.y : 0u, in ? x.z : 0u, in ? x.w : 0u};
+        }
+        return bad;
     }
-    return bad;
-}
+};
 
 // ---------------------------------------------------------------------------
 // up to 32 query rows a KV head: bound by the cache's bytes
@@ -513,7 +523,7 @@ __device__ __forceinline__ bool stage_rows(const TreeParams& p, const Item& it, 
 
 // A wave owns 16 keys of each tile and works for itself on its own LDS ring,
 // without a barrier: the next two tiles are on their way while one is computed.
-template <int D, bool F16, int NT, bool PAGED>
+template <int D, bool F16, int NT, int PAGED>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) tree_few_kernel(TreeParams p) {
     using E = Elem<F16>;
     using R = Rows16<D>;
@@ -556,9 +566,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
             loader.template load<true>(p, pages, stretch, t * kKeys + 16 * wave, dst + R::kBytes);
         };
         u32x4 qr[NT][KS];
+        load_queries<KS, NT>(p, b, it.h, 0, qr);
+        // the first of the tiles that pass through registers, asked for early
+        StagedRows<D, F16, PAGED> staged;
+        auto rows_of = [&](int t) { return t >= cached ? p.T : it.n; };
+        auto key_of = [&](int t) { return (t >= cached ? t - cached : t) * kKeys + 16 * wave; };
+        const bool early = streamed < it.t1 && key_of(streamed) < rows_of(streamed) &&
+                           !(PAGED && streamed < cached && streamed >= stretch + page_tiles(p.c));
+        if (early) staged.load(p, it, pages, stretch, streamed >= cached, key_of(streamed));
         if (it.t0 < streamed) fetch(it.t0);
         if (it.t0 + 1 < streamed) fetch(it.t0 + 1);
-        load_queries<KS, NT>(p, b, it.h, 0, qr);
 
         v4f o[NT][MD];
         float m[NT], l[NT];
@@ -623,7 +640,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
         // the cache's last rows and the drafted tokens
         for (int t = streamed; t < it.t1; ++t) {
             const bool draft = t >= cached;
-            const int first = (draft ? t - cached : t) * kKeys, rows = draft ? p.T : it.n;
             if constexpr (PAGED) {
                 if (!draft && t >= stretch + page_tiles(p.c)) {
                     __syncthreads();
@@ -632,17 +648,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
                     __syncthreads();
                 }
             }
-            const int key0 = first + 16 * wave;
-            if (key0 >= rows) continue;
-            if (draft) drafted_seen(p, b, 0, kRows, first, seen[wave]);
+            const int key0 = key_of(t), left = rows_of(t) - key0;
+            if (left <= 0) continue;
+            if (t > streamed || !early) staged.load(p, it, pages, stretch, draft, key0);
+            if (draft) drafted_seen(p, b, 0, kRows, key0 - 16 * wave, seen[wave]);
             wave_fence();
-            if (stage_rows<D, F16, PAGED>(p, it, pages, stretch, draft, key0, ring, R::kBytes)) wild = 1;
+            if (staged.store(draft, left, ring, R::kBytes)) wild = 1;
             wave_fence();
             uint32_t bits[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 bits[nt] = draft ? (uint32_t)(seen[wave][min(16 * nt + col, p.M - 1) / p.G] >> (16 * wave + 4 * grp)) & 15u
-                                 : (1u << max(0, min(4, rows - key0 - 4 * grp))) - 1;
+                                 : (1u << max(0, min(4, left - 4 * grp))) - 1;
             compute(ring, [&](int nt, int i) { return (bits[nt] >> i & 1u) != 0; });
             wave_fence();
         }
@@ -668,7 +685,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
 
 // A tile of 64 rows lies in LDS as four groups of 16 (K, then V), each loaded by
 // one wave, two tiles side by side.
-template <int D, bool F16, int RW, bool PAGED>
+template <int D, bool F16, int RW, int PAGED>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) tree_many_kernel(TreeParams p) {
     using R = Rows16<D>;
     using E = Elem<F16>;
@@ -839,9 +856,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
                     __syncthreads();
                 }
             }
-            if (stage_rows<D, F16, PAGED>(p, it, pages, stretch, draft, first + 16 * wave, lds + wave * R::kBytes, kApart))
-                wild = 1;
-            if (draft) drafted_seen(p, b, row0, 16 * NT, first, seen[wave]);
+            {
+                StagedRows<D, F16, PAGED> staged;
+                const int key = first + 16 * wave;
+                staged.load(p, it, pages, stretch, draft, key);
+                if (draft) drafted_seen(p, b, row0, 16 * NT, first, seen[wave]);
+                if (staged.store(draft, (draft ? p.T : it.n) - key, lds + wave * R::kBytes, kApart)) wild = 1;
+            }
             __syncthreads();
             v4f s[NT][MT];
             u32x4 pb[MT / 2][NT];
@@ -878,15 +899,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     }
 }
 
-// Merges the runs of every item that lies in more than one: D / 4 lanes a row,
-// kMergeRows rows of one (sequence, KV head) a workgroup.
-template <int D, bool F16>
-__global__ void __launch_bounds__(kMergeRows * D / 4) tree_merge_kernel(TreeParams p, int rows_wg, int chunks) {
+// Merges the runs of every item that lies in more than one.  D / 4 lanes hold a
+// row; SHARE groups of them take every SHARE-th run of it, four runs' loads
+// side by side, and meet in LDS.
+template <int D, bool F16, int SHARE>
+__global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p, int rows_wg, int chunks) {
     using E = Elem<F16>;
+    constexpr int kGroups = 256 / (D / 4), kRowsWg = kGroups / SHARE;
+    __shared__ v4f join_o[SHARE > 1 ? kGroups : 1][D / 4];
+    __shared__ float join_m[kGroups], join_l[kGroups];
     const int item = blockIdx.x / chunks;
     const int64_t b = item / p.Hk;
     const int h = item % p.Hk;
-    const int row = (blockIdx.x % chunks) * kMergeRows + threadIdx.x / (D / 4), c = 4 * (threadIdx.x % (D / 4));
+    const int group = threadIdx.x / (D / 4), part = group % SHARE, c = 4 * (threadIdx.x % (D / 4));
+    const int row = (blockIdx.x % chunks) * kRowsWg + group / SHARE;
 
     // first tile of the item: tiles of the sequences before it
     const int lane = threadIdx.x & 63;
@@ -903,7 +929,7 @@ __global__ void __launch_bounds__(kMergeRows * D / 4) tree_merge_kernel(TreePara
         all += any;
     }
     const int tiles = item_tiles(cache_length(p.c, b), p.T);
-    const int64_t total = all * p.Hk, first = before * p.Hk + (int64_t)h * tiles, last = first + tiles - 1;
+    const int64_t total = uniform(all) * p.Hk, first = uniform(before) * p.Hk + (int64_t)h * tiles, last = first + tiles - 1;
     const int runs = used_runs(p, total);
     auto run_of = [&](int64_t pos) {
         int r = (int)(pos * runs / total);
@@ -911,24 +937,64 @@ __global__ void __launch_bounds__(kMergeRows * D / 4) tree_merge_kernel(TreePara
         return r;
     };
     const int r0 = run_of(first), r1 = run_of(last);
-    if (r0 == r1 || row >= p.M) return;
-    const int rb = row / rows_wg, in = row - rb * rows_wg;
+    if (r0 == r1) return;
+    const int live = min(row, p.M - 1), rb = live / rows_wg, in = live - rb * rows_wg;
     const int64_t size = (int64_t)rows_wg * (D + 2);
-    auto entry = [&](int r) {
-        const bool starts = run_begin(total, runs, r) <= first;
-        return p.part + (2 * ((int64_t)r * p.row_blocks + rb) + starts) * size;
-    };
-    float M = kNegInf;
-    for (int r = r0; r <= r1; ++r) M = fmaxf(M, entry(r)[rows_wg * D + in]);
-    const float base = M == kNegInf ? 0.f : M;
-    float L = 0.f;
+    const bool starts = run_begin(total, runs, r0) <= first;           // only the first run can start the item
+    float M = kNegInf, L = 0.f;
     v4f acc = {0.f, 0.f, 0.f, 0.f};
-    for (int r = r0; r <= r1; ++r) {
-        const float* e = entry(r);
-        const float f = fast_exp2(e[rows_wg * D + in] - base);
-        L += f * e[rows_wg * D + rows_wg + in];
-        acc += f * *reinterpret_cast<const v4f*>(e + in * D + c);
+    for (int r = r0 + part; r <= r1; r += 4 * SHARE) {
+        float m[4], l[4];
+        v4f o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int ri = min(r + i * SHARE, r1);
+            const float* e = p.part + (2 * ((int64_t)ri * p.row_blocks + rb) + (starts && ri == r0)) * size;
+            m[i] = e[rows_wg * D + in];
+            l[i] = e[rows_wg * D + rows_wg + in];
+            o[i] = *reinterpret_cast<const v4f*>(e + in * D + c);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (r + i * SHARE > r1) m[i] = kNegInf;
+            top = fmaxf(top, m[i]);
+        }
+        const float base = top == kNegInf ? 0.f : top;
+        const float old = fast_exp2(M - base);
+        L *= old;
+        acc *= old;
+        M = top;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in_range = r + i * SHARE <= r1;
+            const float f = in_range ? fast_exp2(m[i] - base) : 0.f;
+            L += in_range ? f * l[i] : 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[x] += in_range ? f * o[i][x] : 0.f;
+        }
     }
+    if constexpr (SHARE > 1) {
+        join_o[group][c / 4] = acc;
+        join_m[group] = M;
+        join_l[group] = L;
+        __syncthreads();
+        if (part) return;
+        float top = kNegInf;
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) top = fmaxf(top, join_m[group + i]);
+        const float base = top == kNegInf ? 0.f : top;
+        L = 0.f;
+        acc = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) {
+            const float f = fast_exp2(join_m[group + i] - base);
+            L += f * join_l[group + i];
+            acc += f * join_o[group + i][c / 4];
+        }
+        M = top;
+    }
+    if (row >= p.M) return;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int tq = row / p.G, g = row - tq * p.G;
     *reinterpret_cast<u32x2*>(p.out + b * p.o_sb + tq * p.o_sl + (int64_t)(h * p.G + g) * p.o_sh + c) =
@@ -968,19 +1034,29 @@ int check_tree(const slimkv_tree_attention_args* a) {
     return SLIMKV_OK;
 }
 
+template <int D, bool F16, int PAGED>
+auto tree_kernel(const TreePlan& plan) -> void (*)(TreeParams) {
+    if (plan.rw == 4) return tree_many_kernel<D, F16, 4, PAGED>;
+    if (plan.rw == 2) return tree_many_kernel<D, F16, 2, PAGED>;
+    return plan.nt == 2 ? tree_few_kernel<D, F16, 2, PAGED> : tree_few_kernel<D, F16, 1, PAGED>;
+}
+
 template <int D, bool F16>
 void launch_tree(const TreeParams& p, const TreePlan& plan, hipStream_t st) {
     const dim3 grid((unsigned)((plan.slots + kXcdCount - 1) / kXcdCount * kXcdCount));
-    const bool paged = p.c.table != nullptr;
     void (*kernel)(TreeParams);
-    if (plan.rw == 4) kernel = paged ? tree_many_kernel<D, F16, 4, true> : tree_many_kernel<D, F16, 4, false>;
-    else if (plan.rw == 2) kernel = paged ? tree_many_kernel<D, F16, 2, true> : tree_many_kernel<D, F16, 2, false>;
-    else if (plan.nt == 2) kernel = paged ? tree_few_kernel<D, F16, 2, true> : tree_few_kernel<D, F16, 2, false>;
-    else kernel = paged ? tree_few_kernel<D, F16, 1, true> : tree_few_kernel<D, F16, 1, false>;
+    if (!p.c.table) kernel = tree_kernel<D, F16, kDense>(plan);
+    else if (p.c.block.d % 16 == 0) kernel = tree_kernel<D, F16, kBlocks16>(plan);
+    else kernel = tree_kernel<D, F16, kAnyBlocks>(plan);
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p);
-    const int chunks = (p.M + kMergeRows - 1) / kMergeRows;
-    hipLaunchKernelGGL((tree_merge_kernel<D, F16>), dim3((unsigned)(p.B * p.Hk * chunks)), dim3(kMergeRows * D / 4), 0, st,
-                       p, plan.rows(), chunks);
+    // runs an item has at most, on average: every group of lanes its own row
+    // where they are few, all groups one row where they are many
+    const int64_t share = (int64_t)plan.runs / (p.B * p.Hk);
+    constexpr int kGroups = 256 / (D / 4);
+    const int rows = share >= 8 ? 1 : kGroups, chunks = (p.M + rows - 1) / rows;
+    const dim3 merge_grid((unsigned)(p.B * p.Hk * chunks));
+    if (share >= 8) hipLaunchKernelGGL((tree_merge_kernel<D, F16, kGroups>), merge_grid, dim3(256), 0, st, p, plan.rows(), chunks);
+    else hipLaunchKernelGGL((tree_merge_kernel<D, F16, 1>), merge_grid, dim3(256), 0, st, p, plan.rows(), chunks);
 }
 
 }  // namespace
@@ -1058,10 +1134,9 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     p.M = p.T * p.G;
     p.row_blocks = plan.row_blocks; p.runs = plan.runs; p.slots = plan.slots;
     p.least = 2;
-    p.together = a->cache.block_size % 16 == 0;
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.part = static_cast<float*>(workspace);
-    if ((int64_t)p.B * p.Hk * ((p.M + kMergeRows - 1) / kMergeRows) > 0x7fffffff)
+    if ((int64_t)p.B * p.Hk * p.M > 0x7fffffff)
         return fail(SLIMKV_EINVAL, "tree attention: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->head_dim == 128) {
