@@ -38,7 +38,6 @@ struct TreeParams {
     float* lse;
     int B, T, Hq, Hk, G, M;               // M = T * G query rows of a KV head
     int row_blocks, runs, least;          // least: tiles a run takes at least
-    int64_t slots;                        // runs * row_blocks
     float scale_log2;
     float* part;
 };
@@ -56,10 +55,10 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
     return (int64_t)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
 }
 
-// Tiles of all items (every lane active).
-__device__ __forceinline__ int64_t total_tiles(const TreeParams& p) {
+// Tiles of all items; the host keeps them below 2^31 (every lane active).
+__device__ __forceinline__ int total_tiles(const TreeParams& p) {
     const int lane = threadIdx.x & 63;
-    int64_t sum = 0;
+    int sum = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         int x = b0 + lane < p.B ? item_tiles(cache_length(p.c, b0 + lane), p.T) : 0;
 #pragma unroll
@@ -72,20 +71,19 @@ __device__ __forceinline__ int64_t total_tiles(const TreeParams& p) {
 // Sequence that holds tile `pos`, the position of its first tile and its tiles
 // a head.
 struct Place {
-    int b, tiles, n;
-    int64_t first;
+    int b, tiles, n, first;
 };
 
-__device__ __forceinline__ Place place_of(const TreeParams& p, int64_t pos) {
+__device__ __forceinline__ Place place_of(const TreeParams& p, int pos) {
     const int lane = threadIdx.x & 63;
-    int64_t base = 0;
+    int base = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         const int n = b0 + lane < p.B ? cache_length(p.c, b0 + lane) : 0;
         const int x = b0 + lane < p.B ? item_tiles(n, p.T) : 0;
-        int64_t end = x;
+        int end = x;
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
-            const int64_t y = __shfl_up(end, s, 64);
+            const int y = __shfl_up(end, s, 64);
             if (lane >= s) end += y;
         }
         end = base + end * p.Hk;
@@ -93,20 +91,34 @@ __device__ __forceinline__ Place place_of(const TreeParams& p, int64_t pos) {
         if (past) {
             const int at = __ffsll((unsigned long long)past) - 1;
             const int tiles = uniform(__shfl(x, at, 64));
-            return Place{uniform(b0 + at), tiles, uniform(__shfl(n, at, 64)),
-                         uniform(__shfl(end, at, 64)) - (int64_t)tiles * p.Hk};
+            return Place{b0 + at, tiles, uniform(__shfl(n, at, 64)), uniform(__shfl(end, at, 64)) - tiles * p.Hk};
         }
         base = uniform(__shfl(end, 63, 64));
     }
     return Place{0, 1, 0, 0};             // not reached: pos < total_tiles
 }
 
-__device__ __forceinline__ int used_runs(const TreeParams& p, int64_t total) {
-    const int64_t most = (total + p.least - 1) / p.least;
-    return (int)(most < p.runs ? most : p.runs);
+// Workgroups that follow one another in the grid go to the XCDs in turn: the
+// slots of one XCD follow one another.
+__device__ __forceinline__ int slot_of_block() {
+    return (int)((blockIdx.x % kXcdCount) * (gridDim.x / kXcdCount) + blockIdx.x / kXcdCount);
 }
 
-__device__ __forceinline__ int64_t run_begin(int64_t total, int runs, int r) { return uniform(r * total / runs); }
+// The dealing of `total` tiles: the first `extra` runs take `each` + 1 of them,
+// the others `each`.
+struct Deal {
+    int runs, each, extra;
+    __device__ __forceinline__ Deal(const TreeParams& p, int total) {
+        runs = min(p.runs, (int)(((uint32_t)total + p.least - 1) / (uint32_t)p.least));
+        each = (uint32_t)total / (uint32_t)runs;
+        extra = total - each * runs;
+    }
+    __device__ __forceinline__ int begin(int r) const { return r * each + min(r, extra); }
+    __device__ __forceinline__ int run_of(int pos) const {
+        const int split = extra * (each + 1);
+        return pos < split ? (uint32_t)pos / (uint32_t)(each + 1) : extra + (uint32_t)(pos - split) / (uint32_t)each;
+    }
+};
 
 // ---------------------------------------------------------------------------
 // what both kernels share
@@ -349,15 +361,15 @@ struct Item {
     int h, n, t0, t1, tiles;
 };
 
-__device__ __forceinline__ Item item_at(const TreeParams& p, int64_t pos, int64_t end) {
+__device__ __forceinline__ Item item_at(const TreeParams& p, int pos, int end) {
     const Place at = place_of(p, pos);
     Item it;
     it.b = at.b;
     it.n = at.n;
     it.tiles = at.tiles;
-    it.h = uniform((int)((pos - at.first) / at.tiles));
-    it.t0 = uniform((int)(pos - at.first - (int64_t)it.h * at.tiles));
-    it.t1 = uniform((int)min<int64_t>(at.tiles, it.t0 + end - pos));
+    it.h = (uint32_t)(pos - at.first) / (uint32_t)at.tiles;
+    it.t0 = pos - at.first - it.h * at.tiles;
+    it.t1 = min(at.tiles, it.t0 + end - pos);
     return it;
 }
 
@@ -534,13 +546,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     __shared__ uint64_t seen[4][kRows];
     __shared__ int wild;
 
-    const int64_t slot = (int64_t)(blockIdx.x % kXcdCount) * (gridDim.x / kXcdCount) + blockIdx.x / kXcdCount;
-    if (slot >= p.slots) return;
-    const int64_t total = total_tiles(p);
-    const int runs = used_runs(p, total), run = (int)slot;
-    if (run >= runs) return;
-    int64_t pos = run_begin(total, runs, run);
-    const int64_t end = run_begin(total, runs, run + 1);
+    const int run = slot_of_block();
+    const Deal deal(p, total_tiles(p));
+    if (run >= deal.runs) return;
+    int pos = deal.begin(run);
+    const int end = deal.begin(run + 1);
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     char* ring = lds + wave * kWave;
@@ -667,7 +677,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
         __syncthreads();
         join_keys<MD, NT, 4>(reinterpret_cast<float*>(lds), kRows, 0, wave, m, l, o);
         if (wave == 0) {
-            float* part = p.part + (2 * slot + (it.t0 == 0)) * kPart;
+            float* part = p.part + (2 * (int64_t)run + (it.t0 == 0)) * kPart;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int row = 16 * nt + col;
@@ -700,14 +710,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     __shared__ uint64_t seen[4][16 * NT];
     __shared__ int wild;
 
-    const int64_t slot = (int64_t)(blockIdx.x % kXcdCount) * (gridDim.x / kXcdCount) + blockIdx.x / kXcdCount;
-    if (slot >= p.slots) return;
-    const int run = (int)(slot / p.row_blocks), rb = (int)(slot % p.row_blocks);
-    const int64_t total = total_tiles(p);
-    const int runs = used_runs(p, total);
-    if (run >= runs) return;
-    int64_t pos = run_begin(total, runs, run);
-    const int64_t end = run_begin(total, runs, run + 1);
+    const int slot = slot_of_block();
+    const int run = (uint32_t)slot / (uint32_t)p.row_blocks, rb = slot - run * p.row_blocks;
+    const Deal deal(p, total_tiles(p));
+    if (run >= deal.runs) return;
+    int pos = deal.begin(run);
+    const int end = deal.begin(run + 1);
 
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
@@ -885,7 +893,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
 
         join_keys<MD, NT, KW>(reinterpret_cast<float*>(lds), kRows, rw * 16 * NT, kw, m, l, o);
         if (kw == 0) {
-            float* part = p.part + (2 * slot + (it.t0 == 0)) * kPart;
+            float* part = p.part + (2 * (int64_t)slot + (it.t0 == 0)) * kPart;
             const int j0 = max(0, it.t0 - cached) * kKeys, j1 = min(p.T, max(0, it.t1 - cached) * kKeys);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -916,7 +924,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p, int rows_
 
     // first tile of the item: tiles of the sequences before it
     const int lane = threadIdx.x & 63;
-    int64_t before = 0, all = 0;
+    int before = 0, all = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         const int x = b0 + lane < p.B ? item_tiles(cache_length(p.c, b0 + lane), p.T) : 0;
         int lower = b0 + lane < b ? x : 0, any = x;
@@ -929,18 +937,11 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p, int rows_
         all += any;
     }
     const int tiles = item_tiles(cache_length(p.c, b), p.T);
-    const int64_t total = uniform(all) * p.Hk, first = uniform(before) * p.Hk + (int64_t)h * tiles, last = first + tiles - 1;
-    const int runs = used_runs(p, total);
-    auto run_of = [&](int64_t pos) {
-        int r = (int)(pos * runs / total);
-        while (run_begin(total, runs, r + 1) <= pos) ++r;
-        return r;
-    };
-    const int r0 = run_of(first), r1 = run_of(last);
+    const Deal deal(p, uniform(all) * p.Hk);
+    const int first = uniform(before) * p.Hk + h * tiles, r0 = deal.run_of(first), r1 = deal.run_of(first + tiles - 1);
     if (r0 == r1) return;
     const int live = min(row, p.M - 1), rb = live / rows_wg, in = live - rb * rows_wg;
     const int64_t size = (int64_t)rows_wg * (D + 2);
-    const bool starts = run_begin(total, runs, r0) <= first;           // only the first run can start the item
     float M = kNegInf, L = 0.f;
     v4f acc = {0.f, 0.f, 0.f, 0.f};
     for (int r = r0 + part; r <= r1; r += 4 * SHARE) {
@@ -949,7 +950,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p, int rows_
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int ri = min(r + i * SHARE, r1);
-            const float* e = p.part + (2 * ((int64_t)ri * p.row_blocks + rb) + (starts && ri == r0)) * size;
+            // the run that starts the item keeps it in its second entry
+            const float* e = p.part + (2 * ((int64_t)ri * p.row_blocks + rb) + (ri == r0)) * size;
             m[i] = e[rows_wg * D + in];
             l[i] = e[rows_wg * D + rows_wg + in];
             o[i] = *reinterpret_cast<const v4f*>(e + in * D + c);
@@ -1132,11 +1134,11 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     p.lse = a->lse;
     p.B = (int)B; p.T = (int)T; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk);
     p.M = p.T * p.G;
-    p.row_blocks = plan.row_blocks; p.runs = plan.runs; p.slots = plan.slots;
+    p.row_blocks = plan.row_blocks; p.runs = plan.runs;
     p.least = 2;
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.part = static_cast<float*>(workspace);
-    if ((int64_t)p.B * p.Hk * p.M > 0x7fffffff)
+    if (B * Hk * p.M > 0x7fffffff || B * Hk * ((a->cache.keys + T) / kKeys + 2) > 0x7fffffff)
         return fail(SLIMKV_EINVAL, "tree attention: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->head_dim == 128) {
