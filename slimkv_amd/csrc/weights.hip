@@ -2,14 +2,20 @@
 // of exp(scale q_p . k_j - lse_p), from the LSEs that the attention left.
 //
 // S^T = K . Q^T on the MFMA with K rows as A, held in registers for the whole
-// pass (a wave owns 32 keys), and the query rows p = l * G + g as B, 64 at a
-// time through LDS.  The weight of a score is one fma and one exp2 against the
-// row's LSE; a lane adds the weights of its column's rows in fp32, and the 16
-// columns meet once at the end, so nothing is divided, rescaled or atomic.
+// pass, and the query rows p = l * G + g as B, 16 at a time.  The weight of a
+// score is one fma and one exp2 against the row's LSE; a lane adds the weights
+// of its column's rows in fp32, and the 16 columns meet once at the end, so
+// nothing is divided, rescaled or atomic.
 //
-// A workgroup owns (sequence, KV head, 128 keys); where these do not fill the
-// CUs the query rows are split as well and the parts are added by a second
-// kernel in order.
+// Few query rows (up to 64 a KV head): bound by K's bytes.  A wave owns 32 keys
+// and reads the queries where they lie; nothing is shared and nothing waits but
+// for memory, and many short waves a CU keep it busy.
+//
+// Many: bound by the exponentials.  A wave owns 64 keys, so that a query operand
+// read from LDS feeds four products (with 32 the LDS reads alone take as long
+// as the products), and the query rows pass through LDS 64 at a time.  Where
+// the key blocks do not fill the CUs evenly the query rows are split as well and
+// the parts are added by a second kernel in order.
 
 #include "cache.hpp"
 
@@ -17,9 +23,8 @@ namespace slimkv {
 
 namespace {
 
-constexpr int kWaveKeys = 32;                     // keys a wave owns
-constexpr int kBlockKeys = 4 * kWaveKeys;
 constexpr int kRows = 64;                         // query rows per LDS tile
+constexpr int kFewGroups = 2;                     // 16-key groups of a wave, few query rows
 
 struct WeightsParams {
     CacheView c;
@@ -34,44 +39,153 @@ struct WeightsParams {
     float* part;                                  // [splits][B][Hk][keys]
 };
 
-// Query rows row0 .. row0 + 63: operand, LSE in log2 and the last key each
-// row sees (-1: none).
+// Query row `row` (clamped to the last): its address, its LSE in log2 and the
+// last key it sees (-1: none, also for a row that counts nothing).
+__device__ __forceinline__ const uint16_t* query_address(const WeightsParams& p, int64_t b, int h, int row) {
+    const int r = min(row, p.M - 1), l = quotient(r, p.G), g = r - l * (int)p.G.d;
+    return p.q + b * p.q_sb + l * p.q_sl + (int64_t)(h * (int)p.G.d + g) * p.q_sh;
+}
+
+__device__ __forceinline__ void query_stats(const WeightsParams& p, int64_t b, int h, int n, int row, float* lse, int* last) {
+    const int r = min(row, p.M - 1), l = quotient(r, p.G), g = r - l * (int)p.G.d;
+    const float x = p.lse[b * p.l_sb + (int64_t)(h * (int)p.G.d + g) * p.l_sh + l * p.l_sl];
+    *lse = x * kLog2e;
+    *last = row < p.M && x != kNegInf ? (p.causal ? n - p.L + l : n - 1) : -1;
+}
+
+// The first query row that sees key k0.
+__device__ __forceinline__ int first_row(const WeightsParams& p, int n, int k0) {
+    return p.causal ? (int)min<int64_t>((int64_t)max(0, k0 - n + p.L) * p.G.d, p.M) : 0;
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float v) {
+    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+
+// The 16 columns' sums of 16 MT keys, MT 2 or 4: lane (col, grp) comes with its
+// column's share of keys 16 mt + 4 grp + i.  Each step pairs a lane with its
+// mirror image in 16, 8, 4 and 2 lanes; a pair splits the keys it still holds,
+// each lane sending what the other keeps, so 4 MT - 1 additions do (and one
+// more for MT 2, where two lanes end with the same key).  Lane col ends with
+// key_of_column(col).
+template <int MT>
+__device__ __forceinline__ int key_of_column(int col) {
+    const int grp = (threadIdx.x & 63) >> 4, v = MT == 4 ? col : col >> 1;
+    return 16 * (v >> 2) + 4 * grp + (v & 3);
+}
+
+template <int MT>
+__device__ __forceinline__ float columns_sum(const v4f (&acc)[MT]) {
+    const int col = threadIdx.x & 15;
+    float x[4 * MT];
+#pragma unroll
+    for (int v = 0; v < 4 * MT; ++v) x[v] = acc[v >> 2][v & 3];
+    auto halve = [&](auto move, int half, bool upper) {
+#pragma unroll
+        for (int v = 0; v < 2 * MT; ++v) {
+            if (v >= half) break;
+            const float keep = upper ? x[v + half] : x[v], send = upper ? x[v] : x[v + half];
+            x[v] = keep + move(send);
+        }
+    };
+    halve([](float v) { return dpp_move<0x140>(v); }, 2 * MT, col & 8);                  // row mirror
+    halve([](float v) { return dpp_move<0x141>(v); }, MT, col & 4);                      // half-row mirror
+    halve([](float v) { return dpp_move<0x1b>(v); }, MT / 2, col & 2);                   // quad [3, 2, 1, 0]
+    if constexpr (MT == 4) halve([](float v) { return dpp_move<0xb1>(v); }, 1, col & 1); // quad [1, 0, 3, 2]
+    else x[0] += dpp_move<0xb1>(x[0]);
+    return x[0];
+}
+
+template <int D, bool F16, bool PAGED>
+__global__ void __launch_bounds__(256) weights_few_kernel(WeightsParams p) {
+    using E = Elem<F16>;
+    constexpr int KS = D / 32, MT = kFewGroups;
+    const int rest = (int)(blockIdx.x % p.blocks), h = (int)(blockIdx.x / p.blocks % p.Hk);
+    const int64_t b = blockIdx.x / p.blocks / p.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    const int k0 = rest * 4 * 16 * MT + wave * 16 * MT;
+    const int n = cache_length(p.c, b);
+    const int key = k0 + key_of_column<MT>(col);                           // the key this lane writes
+    const bool mine = (MT == 4 || !(col & 1)) && key < p.c.keys;
+    float before = 0.f;
+    if (p.previous && mine) before = p.previous[b * p.p_sb + h * p.p_sh + key];
+    v4f acc[MT] = {};
+    if (k0 < n) {
+        u32x4 kr[MT][KS];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const RowAt at = cache_row<PAGED>(p.c, b, min(k0 + 16 * mt + col, n - 1));
+            const uint16_t* src = p.c.k + at.k + h * p.c.k_sh + 8 * grp;
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) kr[mt][kk] = *reinterpret_cast<const u32x4*>(src + 32 * kk);
+        }
+        for (int row0 = first_row(p, n, k0) / 16 * 16; row0 < p.M; row0 += 16) {
+            const uint16_t* src = query_address(p, b, h, row0 + col) + 8 * grp;
+            u32x4 x[KS];
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) x[kk] = *reinterpret_cast<const u32x4*>(src + 32 * kk);
+            float lse;
+            int last;
+            query_stats(p, b, h, n, row0 + col, &lse, &last);
+            last -= k0 + 4 * grp;
+            v4f s[MT] = {};
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt] = E::mma32(kr[mt][kk], x[kk], s[mt]);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float w = fast_exp2(__builtin_fmaf(s[mt][i], p.scale_log2, -lse));
+                    acc[mt][i] += 16 * mt + i <= last ? w : 0.f;
+                }
+        }
+    }
+    const float sum = columns_sum<MT>(acc);
+    if (mine) p.out[b * p.w_sb + h * p.w_sh + key] = key < n ? before + sum : before;
+}
+
+// The slot of piece c of row r is c ^ twist(r): the operand reads (16 rows, one
+// piece) then spread over all banks.  With rows padded by 32 bytes instead, half
+// of a 2048-query chunk's time went to bank conflicts (363 us, XXX so).
 template <int D>
-struct QueryTile {
-    uint16_t q[kRows * (D + 16)];
+__device__ __forceinline__ int twist(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+
+// Query rows row0 .. row0 + 63: operand, LSE in log2, the last key each row
+// sees, and the least of these.
+template <int D>
+struct alignas(16) QueryTile {
+    uint16_t q[kRows * D];                        // a row's 16-byte pieces exchanged by an XOR with its number
     float lse[kRows];
     int last[kRows];
+    int least;
 };
 
 template <int D, bool F16, bool PAGED>
-__global__ void __launch_bounds__(256) weights_kernel(WeightsParams p) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) weights_many_kernel(WeightsParams p) {
     using E = Elem<F16>;
-    constexpr int KS = D / 32, P = D / 8, KR = D / 32, kStride = D + 16;
+    constexpr int KS = D / 32, P = D / 8, KR = D / 32, MT = 4, NT = kRows / 16;
     __shared__ __attribute__((aligned(16))) QueryTile<D> tiles[2];
-    const int64_t item = blockIdx.x / p.blocks;
-    const int64_t b = item / p.Hk;
-    const int h = (int)(item % p.Hk);
-    const int k0 = (int)(blockIdx.x % p.blocks) * kBlockKeys;
+    const int h = (int)(blockIdx.x % p.Hk), rest = (int)(blockIdx.x / p.Hk);
+    const int64_t b = rest / p.blocks;
     const int n = cache_length(p.c, b);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    const int kw = k0 + wave * kWaveKeys;
+    const int kb = (rest % p.blocks) * 4 * 16 * MT, k0 = kb + wave * 16 * MT;
 
     // query tiles of this split that see a key of the block
     const int tiles_all = (p.M + kRows - 1) / kRows;
-    int t0 = (int)((int64_t)blockIdx.y * tiles_all / p.splits);
-    const int t1 = k0 < n ? (int)((int64_t)(blockIdx.y + 1) * tiles_all / p.splits) : t0;
-    if (p.causal && k0 < n) {
-        const int64_t first = (int64_t)max(0, k0 - n + p.L) * p.G.d;      // the first row that sees key k0
-        t0 = (int)max<int64_t>(t0, min<int64_t>(first / kRows, t1));
-    }
-
-    v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+    const int from = (int)((int64_t)blockIdx.y * tiles_all / p.splits), to = (int)((int64_t)(blockIdx.y + 1) * tiles_all / p.splits);
+    const int t1 = kb < n ? to : from, t0 = min(t1, max(from, first_row(p, n, kb) / kRows));
+    v4f acc[MT] = {};
     if (t0 < t1) {
-        u32x4 kr[2][KS];
+        u32x4 kr[MT][KS];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-            const RowAt at = cache_row<PAGED>(p.c, b, min(kw + 16 * mt + col, n - 1));
+        for (int mt = 0; mt < MT; ++mt) {
+            const RowAt at = cache_row<PAGED>(p.c, b, min(k0 + 16 * mt + col, n - 1));
             const uint16_t* src = p.c.k + at.k + h * p.c.k_sh + 8 * grp;
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) kr[mt][kk] = *reinterpret_cast<const u32x4*>(src + 32 * kk);
@@ -82,25 +196,23 @@ __global__ void __launch_bounds__(256) weights_kernel(WeightsParams p) {
         const int kq = threadIdx.x / P, cp = 8 * (threadIdx.x % P);
         auto load = [&](int t) {
 #pragma unroll
-            for (int r = 0; r < KR; ++r) {
-                const int row = min(t * kRows + kq + (256 / P) * r, p.M - 1);
-                const int l = quotient(row, p.G), g = row - l * (int)p.G.d;
-                qr[r] = *reinterpret_cast<const u32x4*>(p.q + b * p.q_sb + l * p.q_sl +
-                                                        (int64_t)(h * (int)p.G.d + g) * p.q_sh + cp);
-            }
-            const int mine = t * kRows + (threadIdx.x & (kRows - 1)), row = min(mine, p.M - 1);
-            const int l = quotient(row, p.G), g = row - l * (int)p.G.d;
-            const float x = p.lse[b * p.l_sb + (int64_t)(h * (int)p.G.d + g) * p.l_sh + l * p.l_sl];
-            lse_r = x * kLog2e;
-            last_r = mine < p.M && x != kNegInf ? (p.causal ? n - p.L + l : n - 1) : -1;
+            for (int r = 0; r < KR; ++r)
+                qr[r] = *reinterpret_cast<const u32x4*>(query_address(p, b, h, t * kRows + kq + (256 / P) * r) + cp);
+            query_stats(p, b, h, n, t * kRows + lane, &lse_r, &last_r);
         };
         auto store = [&](QueryTile<D>& t) {
 #pragma unroll
-            for (int r = 0; r < KR; ++r)
-                *reinterpret_cast<u32x4*>(t.q + (kq + (256 / P) * r) * kStride + cp) = qr[r];
-            if (threadIdx.x < kRows) {
-                t.lse[threadIdx.x] = lse_r;
-                t.last[threadIdx.x] = last_r;
+            for (int r = 0; r < KR; ++r) {
+                const int row = kq + (256 / P) * r;
+                *reinterpret_cast<u32x4*>(t.q + row * D + 8 * ((int)(threadIdx.x % P) ^ twist<D>(row))) = qr[r];
+            }
+            if (wave == 0) {
+                t.lse[lane] = lse_r;
+                t.last[lane] = last_r;
+                int least = last_r;
+#pragma unroll
+                for (int s = 1; s < 64; s <<= 1) least = min(least, __shfl_xor(least, s, 64));
+                if (lane == 0) t.least = least;
             }
         };
         load(t0);
@@ -109,25 +221,39 @@ __global__ void __launch_bounds__(256) weights_kernel(WeightsParams p) {
         __syncthreads();
         for (int t = t0; t < t1; ++t) {
             const QueryTile<D>& w = tiles[t & 1];
+            const bool all = __builtin_amdgcn_readfirstlane(w.least) >= k0 + 16 * MT - 1;
+            u32x4 x[NT][KS];
+            auto read = [&](int nt) {
 #pragma unroll
-            for (int nt = 0; nt < kRows / 16; ++nt) {
-                if (t * kRows + 16 * nt >= p.M) break;
-                v4f s[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+                for (int kk = 0; kk < KS; ++kk)
+                    x[nt][kk] = *reinterpret_cast<const u32x4*>(w.q + (16 * nt + col) * D + 8 * ((4 * kk + grp) ^ twist<D>(col)));
+            };
+            read(0);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int kk = 0; kk < KS; ++kk) {
-                    const u32x4 x = *reinterpret_cast<const u32x4*>(w.q + (16 * nt + col) * kStride + 32 * kk + 8 * grp);
-#pragma unroll
-                    for (int mt = 0; mt < 2; ++mt) s[mt] = E::mma32(kr[mt][kk], x, s[mt]);
-                }
+            for (int nt = 0; nt < NT; ++nt) {
+                if (nt + 1 < NT) read(nt + 1);             // the next rows' operand beside these products
                 const float lse = w.lse[16 * nt + col];
-                const int last = w.last[16 * nt + col] - kw - 4 * grp;
+                v4f s[MT] = {};
 #pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
+                for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = fast_exp2(__builtin_fmaf(s[mt][i], p.scale_log2, -lse));
-                        acc[mt][i] += 16 * mt + i <= last ? x : 0.f;
-                    }
+                    for (int mt = 0; mt < MT; ++mt) s[mt] = E::mma32(kr[mt][kk], x[nt][kk], s[mt]);
+                if (all) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[mt][i] += fast_exp2(__builtin_fmaf(s[mt][i], p.scale_log2, -lse));
+                } else {
+                    const int last = w.last[16 * nt + col] - k0 - 4 * grp;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float e = fast_exp2(__builtin_fmaf(s[mt][i], p.scale_log2, -lse));
+                            acc[mt][i] += 16 * mt + i <= last ? e : 0.f;
+                        }
+                }
             }
             if (t + 1 < t1) {
                 store(tiles[(t + 1) & 1]);
@@ -136,23 +262,11 @@ __global__ void __launch_bounds__(256) weights_kernel(WeightsParams p) {
             __syncthreads();
         }
     }
-
-    // over the 16 columns; lane col holds keys 4 grp + i of each 16
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int s = 1; s < 16; s <<= 1) acc[mt][i] += shfl_xor_f(acc[mt][i], s);
-    if (col >= 8) return;
-    const int mt = col >> 2, i = col & 3;
-    float sum = 0.f;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) sum = col == x ? acc[x >> 2][x & 3] : sum;
-    const int key = kw + 16 * mt + 4 * grp + i;
+    const float sum = columns_sum<MT>(acc);
+    const int key = k0 + key_of_column<MT>(col);
     if (key >= p.c.keys) return;
     if (p.splits > 1) {
-        p.part[(((int64_t)blockIdx.y * p.B + b) * p.Hk + h) * p.c.keys + key] = key < n ? sum : 0.f;
+        p.part[(((int64_t)blockIdx.y * p.B + b) * p.Hk + h) * p.c.keys + key] = sum;
         return;
     }
     const float before = p.previous ? p.previous[b * p.p_sb + h * p.p_sh + key] : 0.f;
@@ -169,14 +283,22 @@ __global__ void __launch_bounds__(256) weights_sum_kernel(WeightsParams p) {
     p.out[b * p.w_sb + h * p.w_sh + key] = key < cache_length(p.c, b) ? before + sum : before;
 }
 
-// Splits of the query rows: four workgroups a CU where the key blocks alone
-// give fewer, a tile of rows at least.
-int weight_splits(const slimkv_attention_weights_args* a) {
-    const int64_t blocks = (a->cache.keys + kBlockKeys - 1) / kBlockKeys * a->batch * a->kv_heads;
-    const int64_t tiles = (a->queries * (a->heads / a->kv_heads) + kRows - 1) / kRows;
-    const int64_t want = 4 * device_cu_count();
-    if (blocks <= 0 || blocks >= want) return 1;
-    return (int)std::max<int64_t>(1, std::min(std::min<int64_t>(want / blocks, tiles), (int64_t)64));
+// Up to 64 query rows a KV head go to the kernel without LDS.
+struct WeightsPlan {
+    bool few;
+    int64_t blocks;                                // of keys, a (sequence, head)
+    int splits;
+};
+
+WeightsPlan plan_weights(const slimkv_attention_weights_args* a) {
+    WeightsPlan w{};
+    const int64_t M = a->queries * (a->heads / a->kv_heads), tiles = (M + kRows - 1) / kRows;
+    w.few = M <= 64;
+    const int64_t keys = 64 * (w.few ? kFewGroups : 4);                    // of a workgroup
+    w.blocks = (a->cache.keys + keys - 1) / keys;
+    const int64_t groups = w.blocks * a->batch * a->kv_heads, want = 8 * device_cu_count();
+    w.splits = w.few || groups <= 0 ? 1 : (int)std::max<int64_t>(1, std::min(want / groups, tiles / 4));
+    return w;
 }
 
 int check_weights(const slimkv_attention_weights_args* a) {
@@ -195,10 +317,12 @@ int check_weights(const slimkv_attention_weights_args* a) {
 }
 
 template <int D, bool F16>
-void launch_weights(const WeightsParams& p, hipStream_t st) {
+void launch_weights(const WeightsParams& p, bool few, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.blocks), (unsigned)p.splits);
-    if (p.c.table) hipLaunchKernelGGL((weights_kernel<D, F16, true>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((weights_kernel<D, F16, false>), grid, dim3(256), 0, st, p);
+    void (*kernel)(WeightsParams);
+    if (few) kernel = p.c.table ? weights_few_kernel<D, F16, true> : weights_few_kernel<D, F16, false>;
+    else kernel = p.c.table ? weights_many_kernel<D, F16, true> : weights_many_kernel<D, F16, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p);
 }
 
 }  // namespace
@@ -209,7 +333,7 @@ using namespace slimkv;
 
 extern "C" size_t slimkv_attention_weights_workspace(const slimkv_attention_weights_args* a) {
     if (check_weights(a) != SLIMKV_OK) return 0;
-    const int splits = weight_splits(a);
+    const int splits = plan_weights(a).splits;
     return splits == 1 ? 16 : (size_t)splits * a->batch * a->kv_heads * a->cache.keys * sizeof(float);
 }
 
@@ -231,8 +355,9 @@ extern "C" int slimkv_attention_weights(const slimkv_attention_weights_args* a, 
     p.B = (int)a->batch; p.L = (int)a->queries; p.Hq = (int)a->heads; p.Hk = (int)a->kv_heads; p.causal = a->causal ? 1 : 0;
     p.G = fast_div(a->heads / a->kv_heads);
     p.M = p.L * (int)p.G.d;
-    p.splits = weight_splits(a);
-    p.blocks = (p.c.keys + kBlockKeys - 1) / kBlockKeys;
+    const WeightsPlan plan = plan_weights(a);
+    p.splits = plan.splits;
+    p.blocks = (int)plan.blocks;
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.part = static_cast<float*>(workspace);
     if (p.splits > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
@@ -241,11 +366,11 @@ extern "C" int slimkv_attention_weights(const slimkv_attention_weights_args* a, 
     if ((int64_t)p.B * p.Hk * p.blocks > 0x7fffffff) return fail(SLIMKV_EINVAL, "attention weights: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->head_dim == 128) {
-        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<128, true>(p, st);
-        else launch_weights<128, false>(p, st);
+        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<128, true>(p, plan.few, st);
+        else launch_weights<128, false>(p, plan.few, st);
     } else {
-        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<64, true>(p, st);
-        else launch_weights<64, false>(p, st);
+        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<64, true>(p, plan.few, st);
+        else launch_weights<64, false>(p, plan.few, st);
     }
     if (p.splits > 1) {
         const int64_t all = (int64_t)p.B * p.Hk * p.c.keys;
