@@ -164,10 +164,10 @@ struct alignas(16) QueryTile {
     int least;
 };
 
-template <int D, bool F16, bool PAGED>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) weights_many_kernel(WeightsParams p) {
+template <int D, bool F16, int MT, bool PAGED>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MT == 4 ? 2 : 3))) weights_many_kernel(WeightsParams p) {
     using E = Elem<F16>;
-    constexpr int KS = D / 32, P = D / 8, KR = D / 32, MT = 4, NT = kRows / 16;
+    constexpr int KS = D / 32, P = D / 8, KR = D / 32, NT = kRows / 16;
     __shared__ __attribute__((aligned(16))) QueryTile<D> tiles[2];
     const int h = (int)(blockIdx.x % p.Hk), rest = (int)(blockIdx.x / p.Hk);
     const int64_t b = rest / p.blocks;
@@ -228,24 +228,53 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) w
                 for (int kk = 0; kk < KS; ++kk)
                     x[nt][kk] = *reinterpret_cast<const u32x4*>(w.q + (16 * nt + col) * D + 8 * ((4 * kk + grp) ^ twist<D>(col)));
             };
-            read(0);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                if (nt + 1 < NT) read(nt + 1);             // the next rows' operand beside these products
-                const float lse = w.lse[16 * nt + col];
-                v4f s[MT] = {};
+            auto product = [&](int nt, v4f(&s)[MT]) {
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) s[mt] = E::mma32(kr[mt][kk], x[nt][kk], s[mt]);
-                if (all) {
+                    for (int mt = 0; mt < MT; ++mt)
+                        s[mt] = E::mma32(kr[mt][kk], x[nt][kk], kk ? s[mt] : v4f{0.f, 0.f, 0.f, 0.f});
+            };
+            if (all) {
+                // the weights of 16 rows between the products of the next 16:
+                // one product, one fma, one exp2 and one addition in turn
+                v4f s[2][MT];
+                float lse[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) lse[nt] = w.lse[16 * nt + col];
+                read(0);
+                read(1);
+                __builtin_amdgcn_sched_barrier(0);
+                product(0, s[0]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (nt + 2 < NT) read(nt + 2);
+                    if (nt + 1 < NT) product(nt + 1, s[(nt + 1) & 1]);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[mt][i] += fast_exp2(__builtin_fmaf(s[mt][i], p.scale_log2, -lse));
-                } else {
+                        for (int i = 0; i < 4; ++i)
+                            acc[mt][i] += fast_exp2(__builtin_fmaf(s[nt & 1][mt][i], p.scale_log2, -lse[nt]));
+                    if (nt + 1 < NT) {
+                        __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);
+#pragma unroll
+                        for (int x = 0; x < KS * MT; ++x) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x002, 12 / KS, 0);
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                read(0);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    if (nt + 1 < NT) read(nt + 1);
+                    const float lse = w.lse[16 * nt + col];
                     const int last = w.last[16 * nt + col] - k0 - 4 * grp;
+                    v4f s[MT];
+                    product(nt, s);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -283,9 +312,10 @@ __global__ void __launch_bounds__(256) weights_sum_kernel(WeightsParams p) {
     p.out[b * p.w_sb + h * p.w_sh + key] = key < cache_length(p.c, b) ? before + sum : before;
 }
 
-// Up to 64 query rows a KV head go to the kernel without LDS.
+// Up to 64 query rows a KV head go to the kernel without LDS, up to 512 to
+// waves of 32 keys, more to waves of 64.
 struct WeightsPlan {
-    bool few;
+    int groups;                                    // 16-key groups of a wave; 0: the kernel for few rows
     int64_t blocks;                                // of keys, a (sequence, head)
     int splits;
 };
@@ -293,11 +323,11 @@ struct WeightsPlan {
 WeightsPlan plan_weights(const slimkv_attention_weights_args* a) {
     WeightsPlan w{};
     const int64_t M = a->queries * (a->heads / a->kv_heads), tiles = (M + kRows - 1) / kRows;
-    w.few = M <= 64;
-    const int64_t keys = 64 * (w.few ? kFewGroups : 4);                    // of a workgroup
+    w.groups = M <= 64 ? 0 : M <= 512 ? 2 : 4;
+    const int64_t keys = 64 * (w.groups ? w.groups : kFewGroups);          // of a workgroup
     w.blocks = (a->cache.keys + keys - 1) / keys;
-    const int64_t groups = w.blocks * a->batch * a->kv_heads, want = 8 * device_cu_count();
-    w.splits = w.few || groups <= 0 ? 1 : (int)std::max<int64_t>(1, std::min(want / groups, tiles / 4));
+    const int64_t workgroups = w.blocks * a->batch * a->kv_heads, want = 16 * device_cu_count();
+    w.splits = !w.groups || workgroups <= 0 ? 1 : (int)std::max<int64_t>(1, std::min(want / workgroups, tiles / 4));
     return w;
 }
 
@@ -316,13 +346,17 @@ int check_weights(const slimkv_attention_weights_args* a) {
     return SLIMKV_OK;
 }
 
+template <int D, bool F16, bool PAGED>
+auto weights_kernel(int groups) -> void (*)(WeightsParams) {
+    if (groups == 4) return weights_many_kernel<D, F16, 4, PAGED>;
+    return groups == 2 ? weights_many_kernel<D, F16, 2, PAGED> : weights_few_kernel<D, F16, PAGED>;
+}
+
 template <int D, bool F16>
-void launch_weights(const WeightsParams& p, bool few, hipStream_t st) {
+void launch_weights(const WeightsParams& p, int groups, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.blocks), (unsigned)p.splits);
-    void (*kernel)(WeightsParams);
-    if (few) kernel = p.c.table ? weights_few_kernel<D, F16, true> : weights_few_kernel<D, F16, false>;
-    else kernel = p.c.table ? weights_many_kernel<D, F16, true> : weights_many_kernel<D, F16, false>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((p.c.table ? weights_kernel<D, F16, true>(groups) : weights_kernel<D, F16, false>(groups)), grid,
+                       dim3(256), 0, st, p);
 }
 
 }  // namespace
@@ -366,11 +400,11 @@ extern "C" int slimkv_attention_weights(const slimkv_attention_weights_args* a, 
     if ((int64_t)p.B * p.Hk * p.blocks > 0x7fffffff) return fail(SLIMKV_EINVAL, "attention weights: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->head_dim == 128) {
-        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<128, true>(p, plan.few, st);
-        else launch_weights<128, false>(p, plan.few, st);
+        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<128, true>(p, plan.groups, st);
+        else launch_weights<128, false>(p, plan.groups, st);
     } else {
-        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<64, true>(p, plan.few, st);
-        else launch_weights<64, false>(p, plan.few, st);
+        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<64, true>(p, plan.groups, st);
+        else launch_weights<64, false>(p, plan.groups, st);
     }
     if (p.splits > 1) {
         const int64_t all = (int64_t)p.B * p.Hk * p.c.keys;
