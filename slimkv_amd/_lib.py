@@ -327,15 +327,15 @@ SIGNATURES = {
     'slimkv_beacon_pages': (ctypes.c_int, [ctypes.POINTER(BeaconPagesArgs), c_ptr]),
     'slimkv_raw_pages': (ctypes.c_int, [ctypes.POINTER(RawPagesArgs), c_ptr]),
     'slimkv_paged_step_rows': (ctypes.c_int, [ctypes.POINTER(PagedStepRowsArgs), c_ptr]),
-    # include/slimkv/cache_ops.h
+    # include/slimkv/cache_ops.h (calls take a mirror's reference or its packed bytes)
     'slimkv_cache_abi_version': (ctypes.c_int, []),
     'slimkv_tree_attention_workspace': (ctypes.c_size_t, [ctypes.POINTER(TreeAttentionArgs)]),
-    'slimkv_tree_attention': (ctypes.c_int, [ctypes.POINTER(TreeAttentionArgs), c_ptr, ctypes.c_size_t, c_ptr]),
+    'slimkv_tree_attention': (ctypes.c_int, [c_ptr, c_ptr, ctypes.c_size_t, c_ptr]),
     'slimkv_attention_weights_workspace': (ctypes.c_size_t, [ctypes.POINTER(AttentionWeightsArgs)]),
-    'slimkv_attention_weights': (ctypes.c_int, [ctypes.POINTER(AttentionWeightsArgs), c_ptr, ctypes.c_size_t, c_ptr]),
+    'slimkv_attention_weights': (ctypes.c_int, [c_ptr, c_ptr, ctypes.c_size_t, c_ptr]),
     'slimkv_select_rows_workspace': (ctypes.c_size_t, [ctypes.POINTER(SelectRowsArgs)]),
-    'slimkv_select_rows': (ctypes.c_int, [ctypes.POINTER(SelectRowsArgs), c_ptr, ctypes.c_size_t, c_ptr]),
-    'slimkv_compact_rows': (ctypes.c_int, [ctypes.POINTER(CompactRowsArgs), c_ptr]),
+    'slimkv_select_rows': (ctypes.c_int, [c_ptr, c_ptr, ctypes.c_size_t, c_ptr]),
+    'slimkv_compact_rows': (ctypes.c_int, [c_ptr, c_ptr]),
 }
 
 ABI_VERSION = 16

@@ -22,48 +22,72 @@ host synchronisation), or is left in the caller's device int32 `status` word
 (graph capture, serving loops; kernels.check_status).  The operators have no
 gradients and raise ValueError where one would be recorded.
 """
-import ctypes
+import struct
+from functools import lru_cache
 
 import torch
 
 from . import _lib
 from ._lib import check, lib
-from .kernels import _ptr, _status_word, _workspace, check_status
+from .kernels import _status_word, check_status
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_CODES = {_lib.c_ptr: 'P', _lib.c_i64: 'q', _lib.c_f64: 'd', _lib.c_i32: 'i'}
+
+
+def _packer(mirror):
+    """The bytes of an argument struct from its field values: one struct.pack, where filling the ctypes mirror field by
+    field takes longer than the rest of a call."""
+    def codes(s):
+        return ''.join(codes(kind) if hasattr(kind, '_fields_') else _CODES[kind] for _, kind in s._fields_)
+    layout = struct.Struct(codes(mirror) + '0q')          # '0q': the trailing padding of an 8-byte aligned struct
+    assert layout.size == _lib.ctypes.sizeof(mirror)
+    return layout.pack
+
+
+_pack_tree = _packer(_lib.TreeAttentionArgs)
+_pack_weights = _packer(_lib.AttentionWeightsArgs)
+_pack_select = _packer(_lib.SelectRowsArgs)
+_pack_compact = _packer(_lib.CompactRowsArgs)
 
 
 def _common(name, *tensors):
-    """One device for every tensor, no gradient to record."""
-    device = None
+    """The device that holds every tensor; no gradient to record."""
+    index = tensors[0].get_device()
+    grad = torch.is_grad_enabled()
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0:
             raise ValueError(f'{name} needs device tensors (no CPU path)')
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError(f'{name}: tensors on {device} and {t.device}')
-        if t.requires_grad and torch.is_grad_enabled():
+        if at != index:
+            raise ValueError(f'{name}: tensors on devices {index} and {at}')
+        if grad and t.requires_grad:
             raise ValueError(f'{name} records no gradient: detach the inputs or run it under torch.no_grad()')
-    return device
+    return tensors[0].device
 
 
 def _dtype(name, *tensors):
     kind = tensors[0].dtype
-    if kind not in _DTYPES or any(t is not None and t.dtype is not kind for t in tensors):
-        raise ValueError(f'{name}: expected bfloat16 or float16 for every tensor, found '
-                         f'{[t.dtype for t in tensors if t is not None]}')
-    return _DTYPES[kind]
+    code = _DTYPES.get(kind)
+    for t in tensors:
+        if code is None or t is not None and t.dtype is not kind:
+            raise ValueError(f'{name}: expected bfloat16 or float16 for every tensor, found '
+                             f'{[t.dtype for t in tensors if t is not None]}')
+    return code
 
 
 def _rows16(t):
     """t [B, rows, H, D], or a copy where its rows do not start on 16-byte boundaries, or overlap, or lie far apart."""
-    good = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
-        all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride())) and \
-        (t.shape[1] <= 1 or t.shape[3] <= t.stride(1) < 1 << 23)
-    return t if good else t.clone(memory_format=torch.contiguous_format)
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        st = t.stride()
+        if st[3] == 1 and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape, st[:3])) and \
+                (t.shape[1] <= 1 or t.shape[3] <= st[1] < 1 << 23):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _span(t):
@@ -82,95 +106,116 @@ def _overlap(a, b):
 def _lengths(name, lengths, batch):
     if lengths is None:
         return None
-    if lengths.dtype is not torch.int32 or lengths.shape != (batch,):
+    if lengths.dtype is not torch.int32 or lengths.dim() != 1 or lengths.shape[0] != batch:
         raise ValueError(f'{name}: lengths must be int32 [{batch}]')
-    return lengths.contiguous()
+    return lengths if lengths.is_contiguous() else lengths.contiguous()
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _status(name, status, device, needed):
     """(status word, owned); no word where nothing can be reported."""
-    if status is None and not needed:
-        return None, False
-    if status is None and torch.cuda.is_current_stream_capturing():
-        raise ValueError(f'{name} under graph capture needs a caller status word')
+    if status is None:
+        if not needed:
+            return None, False
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError(f'{name} under graph capture needs a caller status word')
     return _status_word(status, device)
 
 
-class _Cache:
-    """The C view of a cache and what the operators ask of it.  k alone where
-    V is not read."""
-
-    def __init__(self, name, k, v, pages, table, lengths, keys, batch, values=True):
-        self.keep = []
-        if (k is None) == (pages is None):
-            raise ValueError(f'{name}: give the cache either as dense rows or as pages with a block table')
-        if pages is None:
-            if table is not None or keys is not None:
-                raise ValueError(f'{name}: a block table and keys belong to pages')
-            if values and v is None:
-                raise ValueError(f'{name}: dense rows need both k and v')
-            if k.dim() != 4 or k.shape[0] != batch or k.stride(3) != 1 and k.shape[3] != 1:
-                raise ValueError(f'{name}: cache rows must be [{batch}, N, Hkv, D] with contiguous features')
-            if values and (v.shape != k.shape or v.stride(3) != 1):
+def _cache(name, k, v, pages, table, lengths, keys, batch, values=True):
+    """A cache as the C struct's values but for the status word: (fields, rows, heads, features, paged, the tensors
+    they point into).  k alone where V is not read."""
+    if (k is None) == (pages is None):
+        raise ValueError(f'{name}: give the cache either as dense rows or as pages with a block table')
+    lengths = _lengths(name, lengths, batch)
+    if pages is None:
+        if table is not None or keys is not None:
+            raise ValueError(f'{name}: a block table and keys belong to pages')
+        if values and v is None:
+            raise ValueError(f'{name}: dense rows need both k and v')
+        ks = k.stride()
+        if k.dim() != 4 or k.shape[0] != batch or ks[3] != 1:
+            raise ValueError(f'{name}: cache rows must be [{batch}, N, Hkv, D] with contiguous features')
+        _, rows, heads, dim = k.shape
+        vs = (0, 0, 0, 1)
+        if values:
+            vs = v.stride()
+            if v.shape != k.shape or vs[3] != 1:
                 raise ValueError(f'{name}: v must have the shape of k with contiguous features')
-            self.rows, self.heads, self.dim = k.shape[1:]
-            parts = (k, v) if values else (k, None)
-            self.fields = [x for t in parts for x in
-                           ((None, 0, 0, 0) if t is None else (_ptr(t), *t.stride()[:3]))]
-            self.fields += [None, 0, 0, 0, 0]
-            self.first = k
-        else:
-            if v is not None:
-                raise ValueError(f'{name}: pages hold both K and V')
-            if pages.dim() != 5 or pages.shape[2] != 2 or pages.stride(4) != 1:
-                raise ValueError(f'{name}: pages must be [blocks, block, 2, Hkv, D] with contiguous features')
-            if table is None or table.dtype is not torch.int64 or table.dim() != 2 or table.shape[0] != batch:
-                raise ValueError(f'{name}: pages need an int64 block table [{batch}, cols]')
-            table = table if table.stride(1) == 1 else table.contiguous()
-            self.keep.append(table)
-            blocks, block, _, self.heads, self.dim = pages.shape
-            cols = table.shape[1]
-            self.rows = cols * block if keys is None else int(keys)
-            if not 0 <= self.rows <= cols * block:
-                raise ValueError(f'{name}: keys must lie in [0, {cols * block}] (cols * block)')
-            sb, sn, skind, sh, _ = pages.stride()
-            base = pages.data_ptr()
-            self.fields = [base, sb, sn, sh, base + skind * pages.element_size(), sb, sn, sh]
-            self.fields += [_ptr(table), table.stride(0), cols, blocks, block] if self.rows else [None, 0, 0, 0, 0]
-            self.first = pages
-        lengths = _lengths(name, lengths, batch)
-        self.keep.append(lengths)
-        self.fields += [_ptr(lengths), self.rows]
-        self.paged = pages is not None and self.rows > 0
-
-    def struct(self, status):
-        return _lib.CacheRows(*self.fields, _ptr(status))
+        fields = (k.data_ptr(), *ks[:3], v.data_ptr() if values else 0, *vs[:3], 0, 0, 0, 0, 0, _ptr(lengths), rows)
+        return fields, rows, heads, dim, False, lengths
+    if v is not None:
+        raise ValueError(f'{name}: pages hold both K and V')
+    if pages.dim() != 5 or pages.shape[2] != 2 or pages.stride(4) != 1:
+        raise ValueError(f'{name}: pages must be [blocks, block, 2, Hkv, D] with contiguous features')
+    if table is None or table.dtype is not torch.int64 or table.dim() != 2 or table.shape[0] != batch:
+        raise ValueError(f'{name}: pages need an int64 block table [{batch}, cols]')
+    if table.stride(1) != 1:
+        table = table.contiguous()
+    blocks, block, _, heads, dim = pages.shape
+    cols = table.shape[1]
+    rows = cols * block if keys is None else int(keys)
+    if not 0 <= rows <= cols * block:
+        raise ValueError(f'{name}: keys must lie in [0, {cols * block}] (cols * block)')
+    sb, sn, skind, sh, _ = pages.stride()
+    base = pages.data_ptr()
+    place = (table.data_ptr(), table.stride(0), cols, blocks, block) if rows else (0, 0, 0, 0, 0)
+    fields = (base, sb, sn, sh, base + skind * pages.element_size(), sb, sn, sh, *place, _ptr(lengths), rows)
+    return fields, rows, heads, dim, rows > 0, (table, lengths)
 
 
-def _queries(name, q, cache):
-    if q.dim() != 4 or q.shape[3] != cache.dim or q.shape[2] % cache.heads:
-        raise ValueError(f'{name}: q must be [B, rows, Hq, {cache.dim}] with Hq a multiple of {cache.heads}')
+def _queries(name, q, heads, dim):
+    if q.dim() != 4 or q.shape[3] != dim or q.shape[2] % heads:
+        raise ValueError(f'{name}: q must be [B, rows, Hq, {dim}] with Hq a multiple of {heads}')
 
 
-def _launch(device, call, *args):
-    """One entry point on torch's current stream of `device`, whichever device
-    is current."""
-    if device.index == torch.cuda.current_device():
-        check(call(*args, _lib.stream_handle(device)))
+def _on(device):
+    """None where the device is current already, else a guard that makes it so."""
+    return None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _call(device, entry, args, nbytes=None):
+    """One entry point on torch's current stream of `device`, whichever device is current, with a workspace of
+    `nbytes` where it takes one."""
+    guard = _on(device)
+    if guard is not None:
+        with guard:
+            return _call(device, entry, args, nbytes)
+    if nbytes is None:
+        check(entry(args, _lib.stream_handle(device)))
     else:
-        with torch.cuda.device(device):
-            check(call(*args, _lib.stream_handle(device)))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        check(entry(args, ws.data_ptr(), nbytes, _lib.stream_handle(device)))
 
 
-def _with_workspace(device, query, call, a):
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _with_workspace(device, query, call, a)
-    nbytes = query(ctypes.byref(a))
+def _asked(entry, a, index):
+    with torch.cuda.device(index):
+        nbytes = entry(_lib.ctypes.byref(a))
     if nbytes == 0:
         check(-1)
-    ws = _workspace(nbytes, device)
-    check(call(ctypes.byref(a), _ptr(ws), nbytes, _lib.stream_handle(device)))
+    return nbytes
+
+
+# The workspace queries go by sizes (and the device) alone: asked once for each.
+@lru_cache(1024)
+def _tree_bytes(index, B, T, Hq, H, D):
+    return _asked(lib().slimkv_tree_attention_workspace, _lib.TreeAttentionArgs(
+        q=16, batch=B, drafted=T, heads=Hq, kv_heads=H, head_dim=D, scale=1.0), index)
+
+
+@lru_cache(1024)
+def _weights_bytes(index, B, L, Hq, H, D, keys):
+    return _asked(lib().slimkv_attention_weights_workspace, _lib.AttentionWeightsArgs(
+        cache=_lib.CacheRows(keys=keys), batch=B, queries=L, heads=Hq, kv_heads=H, head_dim=D, scale=1.0), index)
+
+
+@lru_cache(1024)
+def _select_bytes(index, B, H, keys, keep, sink, recent):
+    return _asked(lib().slimkv_select_rows_workspace, _lib.SelectRowsArgs(
+        batch=B, heads=H, keys=keys, keep=keep, sink=sink, recent=recent), index)
 
 
 def tree_attention(q, draft_k, draft_v, scale, k=None, v=None, *, pages=None, table=None, lengths=None, keys=None,
@@ -187,19 +232,21 @@ def tree_attention(q, draft_k, draft_v, scale, k=None, v=None, *, pages=None, ta
     influence, infinities and NaN included.  T = 1 decodes a single token."""
     name = 'tree_attention'
     B = q.shape[0]
-    cache = _Cache(name, k, v, pages, table, lengths, keys, B)
-    code = _dtype(name, q, draft_k, draft_v, cache.first, v, out)
-    _queries(name, q, cache)
-    T, Hq, D = q.shape[1:]
-    if draft_k.shape != (B, T, cache.heads, D) or draft_v.shape != draft_k.shape:
-        raise ValueError(f'{name}: draft_k and draft_v must be [{B}, {T}, {cache.heads}, {D}]')
-    m = (None, 0, 0)
+    place, rows, H, D, paged, keep = _cache(name, k, v, pages, table, lengths, keys, B)
+    first = pages if k is None else k
+    code = _dtype(name, q, draft_k, draft_v, first, v, out)
+    _queries(name, q, H, D)
+    _, T, Hq, _ = q.shape
+    draft = (B, T, H, D)
+    if draft_k.shape != draft or draft_v.shape != draft:
+        raise ValueError(f'{name}: draft_k and draft_v must be [{B}, {T}, {H}, {D}]')
+    m = (0, 0, 0)
     if mask is not None:
         if mask.dtype is not torch.bool or mask.shape not in ((T, T), (B, T, T)):
             raise ValueError(f'{name}: mask must be bool [{T}, {T}] or [{B}, {T}, {T}]')
         if mask.stride(-1) != 1:
             mask = mask.contiguous()
-        m = (_ptr(mask), mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
+        m = (mask.data_ptr(), mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
     if out is not None and (out.shape != q.shape or out.stride(3) != 1 or
                             any(t is not None and _overlap(out, t) for t in (q, draft_k, draft_v, k, v, pages))):
         raise ValueError(f'{name}: out must have the shape of q with contiguous features, apart from the inputs')
@@ -208,14 +255,15 @@ def tree_attention(q, draft_k, draft_v, scale, k=None, v=None, *, pages=None, ta
     device = _common(name, q, draft_k, draft_v, k, v, pages, table, lengths, mask, out, lse)
     q, draft_k, draft_v = _rows16(q), _rows16(draft_k), _rows16(draft_v)
     if out is None:
-        out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=device)
+        out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=device)
     if lse is None:
-        lse = torch.empty(B, Hq, T, dtype=torch.float32, device=device)
-    status, owned = _status(name, status, device, cache.paged)
-    a = _lib.TreeAttentionArgs(
-        cache.struct(status), _ptr(q), *q.stride()[:3], _ptr(draft_k), *draft_k.stride()[:3], _ptr(draft_v),
-        *draft_v.stride()[:3], *m, _ptr(out), *out.stride()[:3], _ptr(lse), B, T, Hq, cache.heads, D, float(scale), code)
-    _with_workspace(device, lib().slimkv_tree_attention_workspace, lib().slimkv_tree_attention, a)
+        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
+    status, owned = _status(name, status, device, paged)
+    nbytes = _tree_bytes(device.index, B, T, Hq, H, D)
+    a = _pack_tree(*place, _ptr(status), q.data_ptr(), *q.stride()[:3], draft_k.data_ptr(), *draft_k.stride()[:3],
+                   draft_v.data_ptr(), *draft_v.stride()[:3], *m, out.data_ptr(), *out.stride()[:3], lse.data_ptr(),
+                   B, T, Hq, H, D, scale, code)
+    _call(device, lib().slimkv_tree_attention, a, nbytes)
     if owned:
         check_status(status)
     return out, lse
@@ -237,29 +285,31 @@ def attention_weights(q, lse, scale, k=None, *, pages=None, table=None, lengths=
     fp32, which may be `previous` itself."""
     name = 'attention_weights'
     B = q.shape[0]
-    cache = _Cache(name, k, None, pages, table, lengths, keys, B, values=False)
-    code = _dtype(name, q, cache.first)
-    _queries(name, q, cache)
-    L, Hq, D = q.shape[1:]
+    place, rows, H, D, paged, keep = _cache(name, k, None, pages, table, lengths, keys, B, values=False)
+    code = _dtype(name, q, pages if k is None else k)
+    _queries(name, q, H, D)
+    _, L, Hq, _ = q.shape
     if lse.shape != (B, Hq, L) or lse.dtype is not torch.float32:
         raise ValueError(f'{name}: lse must be float32 [{B}, {Hq}, {L}]')
-    shape = (B, cache.heads, cache.rows)
+    shape = (B, H, rows)
     for what, t in (('previous', previous), ('out', out)):
-        if t is not None and (t.shape != shape or t.dtype is not torch.float32 or t.stride(2) != 1 and shape[2] > 1):
+        if t is not None and (t.shape != shape or t.dtype is not torch.float32 or t.stride(2) != 1 and rows > 1):
             raise ValueError(f'{name}: {what} must be float32 {list(shape)} with contiguous rows')
     if out is not None and previous is not None and _overlap(out, previous) and \
             (out.data_ptr() != previous.data_ptr() or out.stride() != previous.stride()):
         raise ValueError(f'{name}: out must be previous itself or lie apart from it')
+    if out is not None and any(n > 1 and s == 0 for n, s in zip(shape, out.stride())):
+        raise ValueError(f'{name}: out must not be an expanded view')
     device = _common(name, q, lse, k, pages, table, lengths, previous, out)
     if out is None:
         out = torch.empty(shape, dtype=torch.float32, device=device)
     q = _rows16(q)
-    status, owned = _status(name, status, device, cache.paged)
-    a = _lib.AttentionWeightsArgs(
-        cache.struct(status), _ptr(q), *q.stride()[:3], _ptr(lse), *lse.stride(),
-        _ptr(previous), *(previous.stride()[:2] if previous is not None else (0, 0)), _ptr(out), *out.stride()[:2],
-        B, L, Hq, cache.heads, D, float(scale), int(bool(causal)), code)
-    _with_workspace(device, lib().slimkv_attention_weights_workspace, lib().slimkv_attention_weights, a)
+    status, owned = _status(name, status, device, paged)
+    nbytes = _weights_bytes(device.index, B, L, Hq, H, D, rows)
+    a = _pack_weights(*place, _ptr(status), q.data_ptr(), *q.stride()[:3], lse.data_ptr(), *lse.stride(),
+                      *((previous.data_ptr(), *previous.stride()[:2]) if previous is not None else (0, 0, 0)),
+                      out.data_ptr(), *out.stride()[:2], B, L, Hq, H, D, scale, bool(causal), code)
+    _call(device, lib().slimkv_attention_weights, a, nbytes)
     if owned:
         check_status(status)
     return out
@@ -282,11 +332,12 @@ def select_rows(weights, keep, *, lengths=None, sink=0, recent=0):
         weights = weights.contiguous()
     lengths = _lengths(name, lengths, B)
     device = _common(name, weights, lengths)
-    rows = torch.empty(B, H, keep, dtype=torch.int32, device=device)
+    rows = torch.empty((B, H, keep), dtype=torch.int32, device=device)
     counts = torch.empty(B, dtype=torch.int32, device=device)
-    a = _lib.SelectRowsArgs(_ptr(weights), *weights.stride()[:2], _ptr(lengths), _ptr(rows), _ptr(counts), B, H, N,
-                            keep, sink, recent)
-    _with_workspace(device, lib().slimkv_select_rows_workspace, lib().slimkv_select_rows, a)
+    a = _pack_select(weights.data_ptr(), *weights.stride()[:2], _ptr(lengths), rows.data_ptr(), counts.data_ptr(), B, H, N,
+                     keep, sink, recent)
+    nbytes = _select_bytes(device.index, B, H, N, keep, sink, recent)
+    _call(device, lib().slimkv_select_rows, a, nbytes)
     return rows, counts
 
 
@@ -309,9 +360,9 @@ def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weight
             counts.shape != rows.shape[:1]:
         raise ValueError(f'{name}: rows must be int32 [B, heads, keep] and counts int32 [B]')
     B, Hw, keep = rows.shape
-    cache = _Cache(name, k, v, pages, table, None, None, B)
-    code = _dtype(name, cache.first, v, out_k, out_v)
-    H, D = cache.heads, cache.dim
+    place, _, H, D, _, held = _cache(name, k, v, pages, table, None, None, B)
+    first = pages if k is None else k
+    code = _dtype(name, first, v, out_k, out_v)
     if Hw not in (1, H):
         raise ValueError(f'{name}: rows must have 1 or {H} heads')
     rows = rows if rows.stride(2) == 1 else rows.contiguous()
@@ -336,20 +387,22 @@ def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weight
     if out_k is not None and out_v is not None and _overlap(out_k, out_v):
         raise ValueError(f'{name}: out_k and out_v must lie apart')
     device = _common(name, rows, counts, k, v, pages, table, weights, out_k, out_v)
-    outs = (None, 0, 0, 0, None, 0, 0, 0)
+    outs = (0, 0, 0, 0, 0, 0, 0, 0)
     if not in_place:
-        out_k = torch.empty(B, keep, H, D, dtype=cache.first.dtype, device=device) if out_k is None else out_k
-        out_v = torch.empty(B, keep, H, D, dtype=cache.first.dtype, device=device) if out_v is None else out_v
+        if out_k is None:
+            out_k = torch.empty((B, keep, H, D), dtype=first.dtype, device=device)
+        if out_v is None:
+            out_v = torch.empty((B, keep, H, D), dtype=first.dtype, device=device)
         if weights is not None:
-            out_weights = torch.empty(B, Hw, keep, dtype=torch.float32, device=device)
-        outs = (_ptr(out_k), *out_k.stride()[:3], _ptr(out_v), *out_v.stride()[:3])
+            out_weights = torch.empty((B, Hw, keep), dtype=torch.float32, device=device)
+        outs = (out_k.data_ptr(), *out_k.stride()[:3], out_v.data_ptr(), *out_v.stride()[:3])
     status, owned = _status(name, status, device, True)
-    a = _lib.CompactRowsArgs(
-        cache.struct(status), _ptr(rows), rows.stride(0), rows.stride(1) if Hw > 1 else 0, _ptr(counts), *outs,
-        _ptr(weights), *(weights.stride()[:2] if weights is not None else (0, 0)),
-        _ptr(out_weights), *(out_weights.stride()[:2] if out_weights is not None else (0, 0)),
-        Hw, 0 if weights is None else weights.shape[2], B, H, D, keep, int(bool(in_place)), code)
-    _launch(device, lib().slimkv_compact_rows, ctypes.byref(a))
+    a = _pack_compact(*place, status.data_ptr(), rows.data_ptr(), rows.stride(0), rows.stride(1) if Hw > 1 else 0,
+                      counts.data_ptr(), *outs,
+                      *((weights.data_ptr(), *weights.stride()[:2]) if weights is not None else (0, 0, 0)),
+                      *((out_weights.data_ptr(), *out_weights.stride()[:2]) if out_weights is not None else (0, 0, 0)),
+                      Hw, 0 if weights is None else weights.shape[2], B, H, D, keep, bool(in_place), code)
+    _call(device, lib().slimkv_compact_rows, a)
     if owned:
         check_status(status)
     if in_place:

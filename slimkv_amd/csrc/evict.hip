@@ -1,11 +1,14 @@
 // Eviction from a cache: the rows to keep by weight, and their move.
 //
-// select: a radix selection.  fp32 weights map to unsigned integers in their
-// order (NaN to 0), the rows between the first `sink` and the last `recent`
-// are ranked by them, and four passes over 8 bits each find the weight of the
-// last row kept and how many rows of exactly that weight fit.  Two more passes
-// count and write the kept rows in ascending order.  All counts are integers,
-// so the result does not depend on the order of the LDS atomics.
+// select: a radix selection over 11, 11 and 10 bits.  fp32 weights map to
+// unsigned integers in their order (NaN to 0), the rows between the first
+// `sink` and the last `recent` are ranked by them, and three histograms find
+// the weight of the last row kept and how many rows of exactly that weight fit;
+// a last pass counts and writes the kept rows in ascending order.  All counts
+// are integers, so the result does not depend on the order of the LDS atomics.
+// Rows that one workgroup would take long over are cut into chunks: a launch
+// makes each chunk's histogram, and every workgroup of the next one adds them
+// up for itself, so no launch waits for another workgroup.
 //
 // compact: bytes moved.  Out of place a lane moves 16 bytes of K and V of one
 // row; in place a workgroup takes a 64-byte column of one head's K or V and
@@ -18,7 +21,8 @@ namespace slimkv {
 
 namespace {
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 512, kSelectWaves = kSelectThreads / 64;
+constexpr int kBins = 2048, kLastBins = 1024;
 
 struct SelectParams {
     const float* weights; int64_t w_sb, w_sh;
@@ -26,6 +30,8 @@ struct SelectParams {
     int32_t* rows;
     int32_t* counts;
     int H, keys, keep, sink, recent;
+    int chunks;
+    uint32_t* ws;                 // a row's part: see SelectRow
 };
 
 // Order-preserving image of a weight: -0 as +0, NaN below everything.
@@ -39,99 +45,289 @@ __device__ __forceinline__ int lanes_below(uint64_t mask, int lane) {
     return __popcll(mask & (((uint64_t)1 << lane) - 1));
 }
 
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(SelectParams p) {
-    constexpr int kWaves = kSelectThreads / 64;
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t found[2];                        // chosen bin, rows of the bins above it
-    __shared__ int above_w[kWaves], equal_w[kWaves];
-    const int64_t b = blockIdx.x / p.H, h = blockIdx.x % p.H;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n = p.lengths ? max(0, min(p.lengths[b], p.keys)) : p.keys;
-    int32_t* rows = p.rows + (int64_t)blockIdx.x * p.keep;
-    const int count = min(n, p.keep);
-    if (h == 0 && tid == 0) p.counts[b] = count;
-    for (int i = count + tid; i < p.keep; i += kSelectThreads) rows[i] = -1;
-    if (n <= p.keep) {
-        for (int i = tid; i < n; i += kSelectThreads) rows[i] = i;
-        return;
-    }
-    for (int i = tid; i < p.sink; i += kSelectThreads) rows[i] = i;
-    for (int i = tid; i < p.recent; i += kSelectThreads) rows[p.keep - p.recent + i] = n - p.recent + i;
-    const int need = p.keep - p.sink - p.recent, first = p.sink, last = n - p.recent;
-    if (need == 0) return;
-    const float* w = p.weights + b * p.w_sb + h * p.w_sh;
+// One (sequence, head): the ranked rows [first, last), of which `need` are
+// taken, and this workgroup's chunk [from, to) of them.  Workspace of a row:
+// histograms [chunks][2048], [chunks][2048], [chunks][1024], a count a chunk of
+// the rows above the first and above the second prefix, and the state (prefix,
+// rows left) after the first and the second level.
+struct SelectRow {
+    const float* w;
+    int32_t* rows;
+    uint32_t *h1, *h2, *h3, *above1, *above2;
+    int n, first, last, need, chunk, from, to;
+    bool trivial;                 // every row is kept, or none of the ranked ones
 
-    uint32_t prefix = 0, mask = 0;
-    int left = need;                                     // rows to take among those that match the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int i = first + tid; i < last; i += kSelectThreads) {
-            const uint32_t u = rank_of(w[i]);
-            if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (wave == 0) {                                 // bins from the top, four a lane
-            uint32_t c[4], sum = 0;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) sum += c[x] = hist[255 - (4 * lane + x)];
-            uint32_t upto = sum;
-#pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                const uint32_t y = __shfl_up(upto, s, 64);
-                if (lane >= s) upto += y;
-            }
-            uint32_t before = upto - sum;
-            if (before < (uint32_t)left && upto >= (uint32_t)left) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    if (before < (uint32_t)left && before + c[x] >= (uint32_t)left) {
-                        found[0] = 255 - (4 * lane + x);
-                        found[1] = before;
-                    }
-                    before += c[x];
-                }
-            }
-        }
-        __syncthreads();
-        prefix |= found[0] << shift;
-        mask |= 255u << shift;
-        left -= (int)found[1];
-        __syncthreads();
+    __device__ __forceinline__ SelectRow(const SelectParams& p, int item, int chunk_) {
+        const int64_t b = item / p.H, h = item % p.H;
+        n = p.lengths ? max(0, min(p.lengths[b], p.keys)) : p.keys;
+        w = p.weights + b * p.w_sb + h * p.w_sh;
+        rows = p.rows + (int64_t)item * p.keep;
+        need = p.keep - p.sink - p.recent;
+        trivial = n <= p.keep || need == 0;
+        first = p.sink;
+        last = max(first, n - p.recent);
+        chunk = chunk_;
+        const int64_t span = last - first;
+        from = first + (int)(span * chunk / p.chunks);
+        to = first + (int)(span * (chunk + 1) / p.chunks);
+        h1 = p.ws + (int64_t)item * (p.chunks * (2 * kBins + kLastBins + 2) + 4);
+        h2 = h1 + p.chunks * kBins;
+        h3 = h2 + p.chunks * kBins;
+        above1 = h3 + p.chunks * kLastBins;
+        above2 = above1 + p.chunks;
     }
+    // What needs no ranking: the first and the recent rows, the padding, the count.
+    __device__ __forceinline__ void write_given(const SelectParams& p, int item) const {
+        const int count = min(n, p.keep), tid = threadIdx.x;
+        if (item % p.H == 0 && tid == 0) p.counts[item / p.H] = count;
+        for (int i = count + tid; i < p.keep; i += kSelectThreads) rows[i] = -1;
+        if (n <= p.keep) {
+            for (int i = tid; i < n; i += kSelectThreads) rows[i] = i;
+            return;
+        }
+        for (int i = tid; i < p.sink; i += kSelectThreads) rows[i] = i;
+        for (int i = tid; i < p.recent; i += kSelectThreads) rows[p.keep - p.recent + i] = n - p.recent + i;
+    }
+};
 
-    // the rows above the prefix and the first `left` equal to it; a wave owns a
-    // contiguous part
-    const int span = last - first, part = ((span + kWaves - 1) / kWaves + 63) / 64 * 64;
-    const int from = first + wave * part, to = min(last, from + part);
+// What a workgroup shares: a histogram, the bin found, sums over its waves.
+struct SelectLds {
+    uint32_t hist[kBins];
+    uint32_t bin, above;
+    uint32_t wave[2][kSelectWaves];
+};
+
+// Sum of x over the workgroup's threads below this one, and over all of them.
+__device__ __forceinline__ uint32_t block_before(uint32_t x, SelectLds& s, uint32_t* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t upto = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += y;
+    }
+    __syncthreads();
+    if (lane == 63) s.wave[0][wave] = upto;
+    __syncthreads();
+    uint32_t below = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kSelectWaves; ++i) {
+        below += i < wave ? s.wave[0][i] : 0u;
+        all += s.wave[0][i];
+    }
+    *total = all;
+    return below + upto - x;
+}
+
+// The bin, from the highest down, that holds row `left` (counted from 1):
+// s.bin, and s.above rows in the bins above it.
+template <int NB>
+__device__ __forceinline__ void find_bin(SelectLds& s, uint32_t left) {
+    constexpr int K = NB / kSelectThreads;
+    uint32_t c[K], sum = 0, all;
+#pragma unroll
+    for (int x = 0; x < K; ++x) sum += c[x] = s.hist[NB - 1 - (K * (int)threadIdx.x + x)];
+    uint32_t before = block_before(sum, s, &all);
+#pragma unroll
+    for (int x = 0; x < K; ++x) {
+        if (before < left && before + c[x] >= left) {
+            s.bin = NB - 1 - (K * threadIdx.x + x);
+            s.above = before;
+        }
+        before += c[x];
+    }
+    __syncthreads();
+}
+
+// The three levels of the ranking: bins of 11, 11 and 10 bits from the top.
+template <int LEVEL>
+struct Level {
+    static constexpr int kN = LEVEL == 3 ? kLastBins : kBins;
+    static constexpr int kShift = LEVEL == 1 ? 21 : LEVEL == 2 ? 10 : 0;
+    static __device__ __forceinline__ bool matches(uint32_t u, uint32_t prefix) {
+        return LEVEL == 1 || u >> (LEVEL == 2 ? 21 : 10) == prefix;
+    }
+};
+
+// s.hist: the ranks in [from, to) that match the prefix, by this level's bits.
+template <int LEVEL>
+__device__ __forceinline__ void histogram(SelectLds& s, const SelectRow& r, uint32_t prefix) {
+    using V = Level<LEVEL>;
+    __syncthreads();
+    for (int i = threadIdx.x; i < V::kN; i += kSelectThreads) s.hist[i] = 0;
+    __syncthreads();
+    for (int i0 = r.from; i0 < r.to; i0 += 4 * kSelectThreads) {
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = r.w[min(i0 + k * kSelectThreads + (int)threadIdx.x, r.to - 1)];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t u = rank_of(x[k]);
+            if (i0 + k * kSelectThreads + (int)threadIdx.x < r.to && V::matches(u, prefix))
+                atomicAdd(&s.hist[u >> V::kShift & (V::kN - 1)], 1u);
+        }
+    }
+    __syncthreads();
+}
+
+// s.hist: the chunks' histograms added up.
+template <int N>
+__device__ __forceinline__ void add_chunks(SelectLds& s, const uint32_t* h, int chunks) {
+    constexpr int K = N / kSelectThreads;
+    uint32_t sum[K] = {};
+    for (int c = 0; c < chunks; ++c)
+#pragma unroll
+        for (int x = 0; x < K; ++x) sum[x] += h[(int64_t)c * N + x * kSelectThreads + threadIdx.x];
+#pragma unroll
+    for (int x = 0; x < K; ++x) s.hist[x * kSelectThreads + threadIdx.x] = sum[x];
+    __syncthreads();
+}
+
+// Rows of one chunk's histogram in the bins above `bin`, on every thread.
+template <int N>
+__device__ __forceinline__ uint32_t rows_above(SelectLds& s, const uint32_t* h, uint32_t bin) {
+    uint32_t sum = 0, all;
+#pragma unroll
+    for (int x = 0; x < N / kSelectThreads; ++x) {
+        const uint32_t i = x * kSelectThreads + threadIdx.x;
+        sum += i > bin ? h[i] : 0u;
+    }
+    block_before(sum, s, &all);
+    return all;
+}
+
+// The chunk's rows above `least` and the first `left` equal to it (of the whole
+// row: `same` equal ones lie in the chunks before), in order, from the row's
+// position `at` on.  A wave owns a contiguous part.
+__device__ __forceinline__ void write_taken(const SelectRow& r, SelectLds& s, uint32_t least, int left, int at, int same) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int part = ((r.to - r.from + kSelectWaves - 1) / kSelectWaves + 63) / 64 * 64;
+    const int from = min(r.to, r.from + wave * part), to = min(r.to, from + part);
     int above = 0, equal = 0;
     for (int i0 = from; i0 < to; i0 += 64) {
         const int i = i0 + lane;
-        const uint32_t u = i < to ? rank_of(w[i]) : 0u;
-        above += __popcll(__ballot(i < to && u > prefix));
-        equal += __popcll(__ballot(i < to && u == prefix));
+        const uint32_t u = rank_of(r.w[min(i, to - 1)]);
+        above += __popcll(__ballot(i < to && u > least));
+        equal += __popcll(__ballot(i < to && u == least));
     }
     if (lane == 0) {
-        above_w[wave] = above;
-        equal_w[wave] = equal;
+        s.wave[0][wave] = above;
+        s.wave[1][wave] = equal;
     }
     __syncthreads();
-    int taken = 0, same = 0;
     for (int x = 0; x < wave; ++x) {
-        taken += above_w[x] + min(equal_w[x], max(0, left - same));
-        same += equal_w[x];
+        at += (int)s.wave[0][x] + min((int)s.wave[1][x], max(0, left - same));
+        same += (int)s.wave[1][x];
     }
-    int32_t* dst = rows + p.sink + taken;
+    int32_t* dst = r.rows + at;
     for (int i0 = from; i0 < to; i0 += 64) {
         const int i = i0 + lane;
-        const uint32_t u = i < to ? rank_of(w[i]) : 0u;
-        const uint64_t eq = __ballot(i < to && u == prefix);
-        const bool take = i < to && (u > prefix || (u == prefix && same + lanes_below(eq, lane) < left));
+        const uint32_t u = rank_of(r.w[min(i, to - 1)]);
+        const uint64_t eq = __ballot(i < to && u == least);
+        const bool take = i < to && (u > least || (u == least && same + lanes_below(eq, lane) < left));
         const uint64_t all = __ballot(take);
         if (take) dst[lanes_below(all, lane)] = i;
         dst += __popcll(all);
         same += __popcll(eq);
     }
+}
+
+// A row in one workgroup.
+__global__ void __launch_bounds__(kSelectThreads) select_kernel(SelectParams p) {
+    __shared__ SelectLds s;
+    const SelectRow r(p, blockIdx.x, 0);
+    r.write_given(p, blockIdx.x);
+    if (r.trivial) return;
+    uint32_t left = r.need, prefix;
+    histogram<1>(s, r, 0);
+    find_bin<kBins>(s, left);
+    prefix = s.bin;
+    left -= s.above;
+    histogram<2>(s, r, prefix);
+    find_bin<kBins>(s, left);
+    prefix = prefix << 11 | s.bin;
+    left -= s.above;
+    histogram<3>(s, r, prefix);
+    find_bin<kLastBins>(s, left);
+    prefix = prefix << 10 | s.bin;
+    left -= s.above;
+    __syncthreads();
+    write_taken(r, s, prefix, (int)left, p.sink, 0);
+}
+
+// A row in chunks, one launch a level and one to write (LEVEL 4).
+template <int LEVEL>
+__global__ void __launch_bounds__(kSelectThreads) select_chunk_kernel(SelectParams p) {
+    __shared__ SelectLds s;
+    const int item = blockIdx.y, chunk = blockIdx.x;
+    const SelectRow r(p, item, chunk);
+    if (LEVEL == 1 && chunk == 0) r.write_given(p, item);
+    if (r.trivial) return;
+    // prefix and rows left after the first and the second level
+    uint32_t* state = r.above2 + p.chunks;
+    uint32_t prefix = 0, left = r.need;
+    if constexpr (LEVEL >= 3) {
+        prefix = state[2 * (LEVEL - 3)];
+        left = state[2 * (LEVEL - 3) + 1];
+    }
+    if constexpr (LEVEL >= 2) {
+        constexpr int N = LEVEL == 4 ? kLastBins : kBins;
+        const uint32_t* h = LEVEL == 2 ? r.h1 : LEVEL == 3 ? r.h2 : r.h3;
+        add_chunks<N>(s, h, p.chunks);
+        find_bin<N>(s, left);
+        const uint32_t bin = s.bin;
+        left -= s.above;
+        prefix = LEVEL == 2 ? bin : prefix << (LEVEL == 3 ? 11 : 10) | bin;
+        if constexpr (LEVEL < 4) {
+            const uint32_t above = rows_above<N>(s, h + (int64_t)chunk * N, bin);
+            if (threadIdx.x == 0) {
+                (LEVEL == 2 ? r.above1 : r.above2)[chunk] = above;
+                if (chunk == 0) {
+                    state[2 * (LEVEL - 2)] = prefix;
+                    state[2 * (LEVEL - 2) + 1] = left;
+                }
+            }
+        } else {
+            // rows taken and equal ones in the chunks before
+            uint32_t taken = 0, same = 0, unused;
+            for (int c = threadIdx.x; c < chunk; c += kSelectThreads) {
+                taken += r.above1[c] + r.above2[c];
+                same += h[(int64_t)c * N + bin];
+            }
+            for (int c = 0; c < chunk; ++c)
+#pragma unroll
+                for (int x = 0; x < N / kSelectThreads; ++x) {
+                    const uint32_t i = x * kSelectThreads + threadIdx.x;
+                    taken += i > bin ? h[(int64_t)c * N + i] : 0u;
+                }
+            block_before(taken, s, &unused);
+            const int before = (int)unused;
+            block_before(same, s, &unused);
+            const int equal = (int)unused;
+            __syncthreads();
+            write_taken(r, s, prefix, (int)left, p.sink + before + min(equal, (int)left), equal);
+            return;
+        }
+    }
+    if constexpr (LEVEL < 4) {
+        histogram<LEVEL>(s, r, prefix);
+        uint32_t* out = LEVEL == 1 ? r.h1 : LEVEL == 2 ? r.h2 : r.h3;
+        constexpr int N = Level<LEVEL>::kN;
+        for (int i = threadIdx.x; i < N; i += kSelectThreads) out[(int64_t)chunk * N + i] = s.hist[i];
+    }
+}
+
+// Chunks of a row: of 8192 values, at most 32, and no more than give four
+// workgroups a CU over all rows.
+int select_chunks(const slimkv_select_rows_args* a) {
+    const int64_t rows = std::max<int64_t>(1, a->batch * a->heads), most = 4 * device_cu_count() / rows;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({(a->keys + 8191) / 8192, 32, most}));
+}
+
+size_t select_bytes(const slimkv_select_rows_args* a) {
+    const int chunks = select_chunks(a);
+    if (chunks == 1) return 16;
+    return (size_t)(a->batch * a->heads) * ((size_t)chunks * (2 * kBins + kLastBins + 2) + 4) * sizeof(uint32_t);
 }
 
 struct CompactParams {
@@ -279,23 +475,34 @@ int check_select(const slimkv_select_rows_args* a) {
 }  // namespace
 
 extern "C" size_t slimkv_select_rows_workspace(const slimkv_select_rows_args* a) {
-    return check_select(a) == SLIMKV_OK ? 16 : 0;
+    return check_select(a) == SLIMKV_OK ? select_bytes(a) : 0;
 }
 
 extern "C" int slimkv_select_rows(const slimkv_select_rows_args* a, void* workspace, size_t workspace_bytes,
                                   void* stream) {
     const int code = check_select(a);
     if (code != SLIMKV_OK) return code;
-    (void)workspace;
-    (void)workspace_bytes;
     if (a->batch == 0) return SLIMKV_OK;
     if ((!a->weights && a->keys > 0) || !a->rows || !a->counts) return fail(SLIMKV_EINVAL, "select rows: null pointer");
     SelectParams p{};
     p.weights = a->weights; p.w_sb = a->w_sb; p.w_sh = a->w_sh;
     p.lengths = a->lengths; p.rows = a->rows; p.counts = a->counts;
     p.H = (int)a->heads; p.keys = (int)a->keys; p.keep = (int)a->keep; p.sink = (int)a->sink; p.recent = (int)a->recent;
-    hipLaunchKernelGGL(select_kernel, dim3((unsigned)(a->batch * a->heads)), dim3(kSelectThreads), 0,
-                       static_cast<hipStream_t>(stream), p);
+    p.chunks = select_chunks(a);
+    p.ws = static_cast<uint32_t*>(workspace);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const unsigned rows = (unsigned)(a->batch * a->heads);
+    if (p.chunks == 1) {
+        hipLaunchKernelGGL(select_kernel, dim3(rows), dim3(kSelectThreads), 0, st, p);
+    } else {
+        if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) || workspace_bytes < select_bytes(a))
+            return fail(SLIMKV_EWORKSPACE, "select rows: workspace missing, misaligned or too small");
+        const dim3 grid((unsigned)p.chunks, rows);
+        hipLaunchKernelGGL(select_chunk_kernel<1>, grid, dim3(kSelectThreads), 0, st, p);
+        hipLaunchKernelGGL(select_chunk_kernel<2>, grid, dim3(kSelectThreads), 0, st, p);
+        hipLaunchKernelGGL(select_chunk_kernel<3>, grid, dim3(kSelectThreads), 0, st, p);
+        hipLaunchKernelGGL(select_chunk_kernel<4>, grid, dim3(kSelectThreads), 0, st, p);
+    }
     return check_hip(hipGetLastError(), "select rows launch");
 }
 

@@ -293,6 +293,9 @@ SELECT = [
     (1, 2, 5000, 4999, None, 0, 0),
     (1, 1, 70001, 513, None, 4, 32),
     (1, 1, 300, 1, None, 0, 0),
+    (2, 1, 20000, 3000, [20000, 9001], 5, 40),
+    (1, 3, 40007, 20001, [40000], 0, 0),
+    (130, 2, 9001, 100, [(97 * i) % 9002 for i in range(130)], 2, 3),
 ]
 
 
