@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kSelectThreads = 512, kSelectWaves = kSelectThreads / 64;
 constexpr int kBins = 2048, kLastBins = 1024;
+constexpr int kBatch = 8;         // loads a thread has open at once
 
 struct SelectParams {
     const float* weights; int64_t w_sb, w_sh;
@@ -156,12 +157,12 @@ __device__ __forceinline__ void histogram(SelectLds& s, const SelectRow& r, uint
     __syncthreads();
     for (int i = threadIdx.x; i < V::kN; i += kSelectThreads) s.hist[i] = 0;
     __syncthreads();
-    for (int i0 = r.from; i0 < r.to; i0 += 4 * kSelectThreads) {
-        float x[4];
+    for (int i0 = r.from; i0 < r.to; i0 += kBatch * kSelectThreads) {
+        float x[kBatch];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = r.w[min(i0 + k * kSelectThreads + (int)threadIdx.x, r.to - 1)];
+        for (int k = 0; k < kBatch; ++k) x[k] = r.w[min(i0 + k * kSelectThreads + (int)threadIdx.x, r.to - 1)];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kBatch; ++k) {
             const uint32_t u = rank_of(x[k]);
             if (i0 + k * kSelectThreads + (int)threadIdx.x < r.to && V::matches(u, prefix))
                 atomicAdd(&s.hist[u >> V::kShift & (V::kN - 1)], 1u);
@@ -175,9 +176,18 @@ template <int N>
 __device__ __forceinline__ void add_chunks(SelectLds& s, const uint32_t* h, int chunks) {
     constexpr int K = N / kSelectThreads;
     uint32_t sum[K] = {};
-    for (int c = 0; c < chunks; ++c)
+    for (int c0 = 0; c0 < chunks; c0 += kBatch) {
+        uint32_t v[kBatch][K];
 #pragma unroll
-        for (int x = 0; x < K; ++x) sum[x] += h[(int64_t)c * N + x * kSelectThreads + threadIdx.x];
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int x = 0; x < K; ++x)
+                v[k][x] = h[(int64_t)min(c0 + k, chunks - 1) * N + x * kSelectThreads + threadIdx.x];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int x = 0; x < K; ++x) sum[x] += c0 + k < chunks ? v[k][x] : 0u;
+    }
 #pragma unroll
     for (int x = 0; x < K; ++x) s.hist[x * kSelectThreads + threadIdx.x] = sum[x];
     __syncthreads();
@@ -204,11 +214,16 @@ __device__ __forceinline__ void write_taken(const SelectRow& r, SelectLds& s, ui
     const int part = ((r.to - r.from + kSelectWaves - 1) / kSelectWaves + 63) / 64 * 64;
     const int from = min(r.to, r.from + wave * part), to = min(r.to, from + part);
     int above = 0, equal = 0;
-    for (int i0 = from; i0 < to; i0 += 64) {
-        const int i = i0 + lane;
-        const uint32_t u = rank_of(r.w[min(i, to - 1)]);
-        above += __popcll(__ballot(i < to && u > least));
-        equal += __popcll(__ballot(i < to && u == least));
+    for (int i0 = from; i0 < to; i0 += 64 * kBatch) {
+        float x[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) x[k] = r.w[min(i0 + 64 * k + lane, to - 1)];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const uint32_t u = rank_of(x[k]);
+            above += __popcll(__ballot(i0 + 64 * k + lane < to && u > least));
+            equal += __popcll(__ballot(i0 + 64 * k + lane < to && u == least));
+        }
     }
     if (lane == 0) {
         s.wave[0][wave] = above;
@@ -220,15 +235,21 @@ __device__ __forceinline__ void write_taken(const SelectRow& r, SelectLds& s, ui
         same += (int)s.wave[1][x];
     }
     int32_t* dst = r.rows + at;
-    for (int i0 = from; i0 < to; i0 += 64) {
-        const int i = i0 + lane;
-        const uint32_t u = rank_of(r.w[min(i, to - 1)]);
-        const uint64_t eq = __ballot(i < to && u == least);
-        const bool take = i < to && (u > least || (u == least && same + lanes_below(eq, lane) < left));
-        const uint64_t all = __ballot(take);
-        if (take) dst[lanes_below(all, lane)] = i;
-        dst += __popcll(all);
-        same += __popcll(eq);
+    for (int i0 = from; i0 < to; i0 += 64 * kBatch) {
+        float x[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) x[k] = r.w[min(i0 + 64 * k + lane, to - 1)];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int i = i0 + 64 * k + lane;
+            const uint32_t u = rank_of(x[k]);
+            const uint64_t eq = __ballot(i < to && u == least);
+            const bool take = i < to && (u > least || (u == least && same + lanes_below(eq, lane) < left));
+            const uint64_t all = __ballot(take);
+            if (take) dst[lanes_below(all, lane)] = i;
+            dst += __popcll(all);
+            same += __popcll(eq);
+        }
     }
 }
 
@@ -294,12 +315,19 @@ __global__ void __launch_bounds__(kSelectThreads) select_chunk_kernel(SelectPara
                 taken += r.above1[c] + r.above2[c];
                 same += h[(int64_t)c * N + bin];
             }
-            for (int c = 0; c < chunk; ++c)
+            for (int c0 = 0; c0 < chunk; c0 += kBatch) {
+                uint32_t v[kBatch][N / kSelectThreads];
 #pragma unroll
-                for (int x = 0; x < N / kSelectThreads; ++x) {
-                    const uint32_t i = x * kSelectThreads + threadIdx.x;
-                    taken += i > bin ? h[(int64_t)c * N + i] : 0u;
-                }
+                for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+                    for (int x = 0; x < N / kSelectThreads; ++x)
+                        v[k][x] = h[(int64_t)min(c0 + k, chunk - 1) * N + x * kSelectThreads + threadIdx.x];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+                    for (int x = 0; x < N / kSelectThreads; ++x)
+                        taken += c0 + k < chunk && x * kSelectThreads + threadIdx.x > bin ? v[k][x] : 0u;
+            }
             block_before(taken, s, &unused);
             const int before = (int)unused;
             block_before(same, s, &unused);
