@@ -116,4 +116,91 @@ bool rows_aligned(const void* p, std::initializer_list<std::pair<int64_t, int64_
 
 constexpr int kXcdCount = 8;
 
+// Values that are the same on every lane, in scalar registers: what follows
+// from them stays on the scalar unit, and buffer resources need no loop over
+// lanes.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
+}
+
+// The dealing of a ragged batch to workgroups.  An item is one KV head of one
+// sequence: its cache rows in tiles of `rows`, and `extra` tiles after them.  The
+// tiles of all items lie in a row, sequence by sequence and head by head, and
+// are dealt to at most `runs` workgroups in equal runs, whatever the lengths
+// are.  The host keeps their number below 2^31.
+struct Dealing {
+    int B, Hk, rows, extra, runs;
+};
+
+__device__ __forceinline__ int item_tiles(const Dealing& d, int n) {
+    return (int)((uint32_t)(n + d.rows - 1) / (uint32_t)d.rows) + d.extra;
+}
+
+// Tiles of all items (every lane active).
+__device__ __forceinline__ int total_tiles(const CacheView& c, const Dealing& d) {
+    const int lane = threadIdx.x & 63;
+    int sum = 0;
+    for (int b0 = 0; b0 < d.B; b0 += 64) {
+        int x = b0 + lane < d.B ? item_tiles(d, cache_length(c, b0 + lane)) : 0;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) x += __shfl_xor(x, s, 64);
+        sum += x;
+    }
+    return uniform(sum) * d.Hk;
+}
+
+// Sequence that holds tile `pos`, the position of its first tile, its tiles a
+// head and its rows.
+struct Place {
+    int b, tiles, n, first;
+};
+
+__device__ __forceinline__ Place place_of(const CacheView& c, const Dealing& d, int pos) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int b0 = 0; b0 < d.B; b0 += 64) {
+        const int n = b0 + lane < d.B ? cache_length(c, b0 + lane) : 0;
+        const int x = b0 + lane < d.B ? item_tiles(d, n) : 0;
+        int end = x;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int y = __shfl_up(end, s, 64);
+            if (lane >= s) end += y;
+        }
+        end = base + end * d.Hk;
+        const uint64_t past = __ballot(pos < end);
+        if (past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            const int tiles = uniform(__shfl(x, at, 64));
+            return Place{b0 + at, tiles, uniform(__shfl(n, at, 64)), uniform(__shfl(end, at, 64)) - tiles * d.Hk};
+        }
+        base = uniform(__shfl(end, 63, 64));
+    }
+    return Place{0, 1, 0, 0};             // not reached: pos < total_tiles
+}
+
+// Workgroups that follow one another in the grid go to the XCDs in turn: the
+// slots of one XCD follow one another.
+__device__ __forceinline__ int slot_of_block() {
+    return (int)((blockIdx.x % kXcdCount) * (gridDim.x / kXcdCount) + blockIdx.x / kXcdCount);
+}
+
+// The runs of `total` tiles: the first `extra` runs take `each` + 1 of them,
+// the others `each`.
+struct Deal {
+    int runs, each, extra;
+    __device__ __forceinline__ Deal(const Dealing& d, int total) {
+        runs = min(d.runs, total);
+        const int r = max(runs, 1);
+        each = (uint32_t)total / (uint32_t)r;
+        extra = total - each * r;
+    }
+    __device__ __forceinline__ int begin(int r) const { return r * each + min(r, extra); }
+    __device__ __forceinline__ int run_of(int pos) const {
+        const int split = extra * (each + 1);
+        return pos < split ? (uint32_t)pos / (uint32_t)(each + 1) : extra + (uint32_t)(pos - split) / (uint32_t)each;
+    }
+};
+
 }  // namespace slimkv

@@ -37,87 +37,10 @@ struct TreeParams {
     uint16_t* out; int64_t o_sb, o_sl, o_sh;
     float* lse;
     int B, T, Hq, Hk, G, M;               // M = T * G query rows of a KV head
-    int row_blocks, runs, least;          // least: tiles a run takes at least
+    int row_blocks;
+    Dealing deal;
     float scale_log2;
     float* part;
-};
-
-// Tiles of one KV head of a sequence with n cache rows.
-__device__ __forceinline__ int item_tiles(int n, int T) {
-    return (n + kKeys - 1) / kKeys + (T + kKeys - 1) / kKeys;
-}
-
-// Values that are the same on every lane, in scalar registers: what follows
-// from them stays on the scalar unit, and buffer resources need no loop over
-// lanes.
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-    return (int64_t)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
-}
-
-// Tiles of all items; the host keeps them below 2^31 (every lane active).
-__device__ __forceinline__ int total_tiles(const TreeParams& p) {
-    const int lane = threadIdx.x & 63;
-    int sum = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        int x = b0 + lane < p.B ? item_tiles(cache_length(p.c, b0 + lane), p.T) : 0;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) x += __shfl_xor(x, s, 64);
-        sum += x;
-    }
-    return uniform(sum) * p.Hk;
-}
-
-// Sequence that holds tile `pos`, the position of its first tile and its tiles
-// a head.
-struct Place {
-    int b, tiles, n, first;
-};
-
-__device__ __forceinline__ Place place_of(const TreeParams& p, int pos) {
-    const int lane = threadIdx.x & 63;
-    int base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int n = b0 + lane < p.B ? cache_length(p.c, b0 + lane) : 0;
-        const int x = b0 + lane < p.B ? item_tiles(n, p.T) : 0;
-        int end = x;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const int y = __shfl_up(end, s, 64);
-            if (lane >= s) end += y;
-        }
-        end = base + end * p.Hk;
-        const uint64_t past = __ballot(pos < end);
-        if (past) {
-            const int at = __ffsll((unsigned long long)past) - 1;
-            const int tiles = uniform(__shfl(x, at, 64));
-            return Place{b0 + at, tiles, uniform(__shfl(n, at, 64)), uniform(__shfl(end, at, 64)) - tiles * p.Hk};
-        }
-        base = uniform(__shfl(end, 63, 64));
-    }
-    return Place{0, 1, 0, 0};             // not reached: pos < total_tiles
-}
-
-// Workgroups that follow one another in the grid go to the XCDs in turn: the
-// slots of one XCD follow one another.
-__device__ __forceinline__ int slot_of_block() {
-    return (int)((blockIdx.x % kXcdCount) * (gridDim.x / kXcdCount) + blockIdx.x / kXcdCount);
-}
-
-// The dealing of `total` tiles: the first `extra` runs take `each` + 1 of them,
-// the others `each`.
-struct Deal {
-    int runs, each, extra;
-    __device__ __forceinline__ Deal(const TreeParams& p, int total) {
-        runs = min(p.runs, (int)(((uint32_t)total + p.least - 1) / (uint32_t)p.least));
-        each = (uint32_t)total / (uint32_t)runs;
-        extra = total - each * runs;
-    }
-    __device__ __forceinline__ int begin(int r) const { return r * each + min(r, extra); }
-    __device__ __forceinline__ int run_of(int pos) const {
-        const int split = extra * (each + 1);
-        return pos < split ? (uint32_t)pos / (uint32_t)(each + 1) : extra + (uint32_t)(pos - split) / (uint32_t)each;
-    }
 };
 
 // ---------------------------------------------------------------------------
@@ -362,7 +285,7 @@ struct Item {
 };
 
 __device__ __forceinline__ Item item_at(const TreeParams& p, int pos, int end) {
-    const Place at = place_of(p, pos);
+    const Place at = place_of(p.c, p.deal, pos);
     Item it;
     it.b = at.b;
     it.n = at.n;
@@ -390,18 +313,30 @@ struct Rows16 {
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
-// 16 bytes a lane from base + offset to 1024 consecutive bytes of LDS at dst
-// (wave-uniform).  Written out because the compiler, which orders LDS reads of
-// its own behind every such load it knows of, would empty the pipeline; the
-// waits are the caller's.  No register is written.
+// 16 bytes a lane to 1024 consecutive bytes of LDS at dst (wave-uniform), from
+// base + offset or from src.  Written out because the compiler, which orders LDS
+// reads of its own behind every such load it knows of, would empty the pipeline;
+// the waits are the caller's.  No register is written.  ONCE: rows that no other
+// workgroup reads are loaded non-temporal (16 sequences of 8-32K paged rows, one
+// token 255 us without, 228 with; 26 tokens 318 / 290; 63 tokens over one cache,
+// three blocks of query rows reading each row, 276 / 297).
+template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(const char* base, uint32_t offset, char* dst) {
     const uint32_t at = (uint32_t)uniform((int)(uintptr_t)(lds_void*)dst);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base)
-                 : "memory");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(at), "v"(offset), "s"(base)
+                     : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base)
+                     : "memory");
 }
+template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(const char* src, char* dst) {
     const uint32_t at = (uint32_t)uniform((int)(uintptr_t)(lds_void*)dst);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(src) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory");
 }
 
 __device__ __forceinline__ u32x2 read_transposed(const char* p) {
@@ -459,6 +394,12 @@ struct RowLoader {
     // K (V false) or V of rows row .. row + 15
     template <bool V>
     __device__ __forceinline__ void load(const TreeParams& p, const Pages& pages, int stretch, int row, char* dst) const {
+        if (p.row_blocks == 1) load_rows<V, true>(p, pages, stretch, row, dst);
+        else load_rows<V, false>(p, pages, stretch, row, dst);
+    }
+    template <bool V, bool ONCE>
+    __device__ __forceinline__ void load_rows(const TreeParams& p, const Pages& pages, int stretch, int row,
+                                              char* dst) const {
         const char* base = V ? vb : kb;
         if constexpr (PAGED != kAnyBlocks) {
             int64_t at;
@@ -470,13 +411,13 @@ struct RowLoader {
             }
             base += 2 * at;
 #pragma unroll
-            for (int x = 0; x < R::kLoads; ++x) load_to_lds(base, V ? vo[x] : ko[x], dst + 1024 * x);
+            for (int x = 0; x < R::kLoads; ++x) load_to_lds<ONCE>(base, V ? vo[x] : ko[x], dst + 1024 * x);
         } else {
 #pragma unroll
             for (int x = 0; x < R::kLoads; ++x) {
                 const int r = x * (64 / R::P) + lrow, piece = 16 * (lslot ^ R::twist(r));
                 const RowAt at = paged_row(p.c, pages, stretch, row + r);
-                load_to_lds(base + 2 * (V ? at.v : at.k) + piece, dst + 1024 * x);
+                load_to_lds<ONCE>(base + 2 * (V ? at.v : at.k) + piece, dst + 1024 * x);
             }
         }
     }
@@ -547,7 +488,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     __shared__ int wild;
 
     const int run = slot_of_block();
-    const Deal deal(p, total_tiles(p));
+    const Deal deal(p.deal, total_tiles(p.c, p.deal));
     if (run >= deal.runs) return;
     int pos = deal.begin(run);
     const int end = deal.begin(run + 1);
@@ -572,8 +513,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
 
         auto fetch = [&](int t) {
             char* dst = ring + (t & 1) * 2 * R::kBytes;
-            loader.template load<false>(p, pages, stretch, t * kKeys + 16 * wave, dst);
-            loader.template load<true>(p, pages, stretch, t * kKeys + 16 * wave, dst + R::kBytes);
+            loader.template load_rows<false, true>(p, pages, stretch, t * kKeys + 16 * wave, dst);
+            loader.template load_rows<true, true>(p, pages, stretch, t * kKeys + 16 * wave, dst + R::kBytes);
         };
         u32x4 qr[NT][KS];
         load_queries<KS, NT>(p, b, it.h, 0, qr);
@@ -712,7 +653,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
 
     const int slot = slot_of_block();
     const int run = (uint32_t)slot / (uint32_t)p.row_blocks, rb = slot - run * p.row_blocks;
-    const Deal deal(p, total_tiles(p));
+    const Deal deal(p.deal, total_tiles(p.c, p.deal));
     if (run >= deal.runs) return;
     int pos = deal.begin(run);
     const int end = deal.begin(run + 1);
@@ -926,7 +867,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p, int rows_
     const int lane = threadIdx.x & 63;
     int before = 0, all = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int x = b0 + lane < p.B ? item_tiles(cache_length(p.c, b0 + lane), p.T) : 0;
+        const int x = b0 + lane < p.B ? item_tiles(p.deal, cache_length(p.c, b0 + lane)) : 0;
         int lower = b0 + lane < b ? x : 0, any = x;
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
@@ -936,8 +877,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p, int rows_
         before += lower;
         all += any;
     }
-    const int tiles = item_tiles(cache_length(p.c, b), p.T);
-    const Deal deal(p, uniform(all) * p.Hk);
+    const int tiles = item_tiles(p.deal, cache_length(p.c, b));
+    const Deal deal(p.deal, uniform(all) * p.Hk);
     const int first = uniform(before) * p.Hk + h * tiles, r0 = deal.run_of(first), r1 = deal.run_of(first + tiles - 1);
     if (r0 == r1) return;
     const int live = min(row, p.M - 1), rb = live / rows_wg, in = live - rb * rows_wg;
@@ -1134,8 +1075,8 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     p.lse = a->lse;
     p.B = (int)B; p.T = (int)T; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk);
     p.M = p.T * p.G;
-    p.row_blocks = plan.row_blocks; p.runs = plan.runs;
-    p.least = 2;
+    p.row_blocks = plan.row_blocks;
+    p.deal = Dealing{p.B, p.Hk, kKeys, (p.T + kKeys - 1) / kKeys, plan.runs};
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.part = static_cast<float*>(workspace);
     if (B * Hk * p.M > 0x7fffffff || B * Hk * ((a->cache.keys + T) / kKeys + 2) > 0x7fffffff)

@@ -7,7 +7,7 @@
 // of its column's rows in fp32, and the 16 columns meet once at the end, so
 // nothing is divided, rescaled or atomic.
 //
-// Few query rows (up to 64 a KV head): bound by K's bytes.  A wave owns 32 keys
+// Few query rows (up to 16 a KV head): bound by K's bytes.  A wave owns 32 keys
 // and reads the queries where they lie; nothing is shared and nothing waits but
 // for memory, and many short waves a CU keep it busy.
 //
@@ -24,7 +24,6 @@ namespace slimkv {
 namespace {
 
 constexpr int kRows = 64;                         // query rows per LDS tile
-constexpr int kFewGroups = 2;                     // 16-key groups of a wave, few query rows
 
 struct WeightsParams {
     CacheView c;
@@ -100,7 +99,7 @@ __device__ __forceinline__ float columns_sum(const v4f (&acc)[MT]) {
 template <int D, bool F16, bool PAGED>
 __global__ void __launch_bounds__(256) weights_few_kernel(WeightsParams p) {
     using E = Elem<F16>;
-    constexpr int KS = D / 32, MT = kFewGroups;
+    constexpr int KS = D / 32, MT = 2;
     const int rest = (int)(blockIdx.x % p.blocks), h = (int)(blockIdx.x / p.blocks % p.Hk);
     const int64_t b = blockIdx.x / p.blocks / p.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -121,14 +120,14 @@ __global__ void __launch_bounds__(256) weights_few_kernel(WeightsParams p) {
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) kr[mt][kk] = *reinterpret_cast<const u32x4*>(src + 32 * kk);
         }
-        for (int row0 = first_row(p, n, k0) / 16 * 16; row0 < p.M; row0 += 16) {
-            const uint16_t* src = query_address(p, b, h, row0 + col) + 8 * grp;
+        if (first_row(p, n, k0) < p.M) {
+            const uint16_t* src = query_address(p, b, h, col) + 8 * grp;
             u32x4 x[KS];
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) x[kk] = *reinterpret_cast<const u32x4*>(src + 32 * kk);
             float lse;
             int last;
-            query_stats(p, b, h, n, row0 + col, &lse, &last);
+            query_stats(p, b, h, n, col, &lse, &last);
             last -= k0 + 4 * grp;
             v4f s[MT] = {};
 #pragma unroll
@@ -150,7 +149,7 @@ __global__ void __launch_bounds__(256) weights_few_kernel(WeightsParams p) {
 
 // The slot of piece c of row r is c ^ twist(r): the operand reads (16 rows, one
 // piece) then spread over all banks.  With rows padded by 32 bytes instead, half
-// of a 2048-query chunk's time went to bank conflicts (363 us, XXX so).
+// of a 2048-query chunk's time went to bank conflicts (363 us, 294 so).
 template <int D>
 __device__ __forceinline__ int twist(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
 
@@ -164,10 +163,10 @@ struct alignas(16) QueryTile {
     int least;
 };
 
-template <int D, bool F16, int MT, bool PAGED>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MT == 4 ? 2 : 3))) weights_many_kernel(WeightsParams p) {
+template <int D, bool F16, bool PAGED>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) weights_many_kernel(WeightsParams p) {
     using E = Elem<F16>;
-    constexpr int KS = D / 32, P = D / 8, KR = D / 32, NT = kRows / 16;
+    constexpr int KS = D / 32, P = D / 8, KR = D / 32, MT = 4, NT = kRows / 16;
     __shared__ __attribute__((aligned(16))) QueryTile<D> tiles[2];
     const int h = (int)(blockIdx.x % p.Hk), rest = (int)(blockIdx.x / p.Hk);
     const int64_t b = rest / p.blocks;
@@ -270,6 +269,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MT == 
                 read(0);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
+                    if (t * kRows + 16 * nt >= p.M) break;
                     if (nt + 1 < NT) read(nt + 1);
                     const float lse = w.lse[16 * nt + col];
                     const int last = w.last[16 * nt + col] - k0 - 4 * grp;
@@ -312,10 +312,14 @@ __global__ void __launch_bounds__(256) weights_sum_kernel(WeightsParams p) {
     p.out[b * p.w_sb + h * p.w_sh + key] = key < cache_length(p.c, b) ? before + sum : before;
 }
 
-// Up to 64 query rows a KV head go to the kernel without LDS, up to 512 to
-// waves of 32 keys, more to waves of 64.
+// Up to 16 query rows a KV head go to the kernel without LDS, more to the other
+// (8 sequences of 32768 rows, 8 KV heads: 16 query rows 100 / 122 us, 32 rows 127
+// / 123, 64 rows 183 / 121; one sequence 16.2 / 17.7, 20.3 / 17.6, 28.1 / 17.1).
+// Its query rows are split until sixteen workgroups a CU are there, since ragged
+// lengths leave part of them nothing to do (a 2048-query chunk of two sequences,
+// one a quarter of the other: 286 us at eight, 264 at sixteen, 281 at thirty-two).
 struct WeightsPlan {
-    int groups;                                    // 16-key groups of a wave; 0: the kernel for few rows
+    bool few;
     int64_t blocks;                                // of keys, a (sequence, head)
     int splits;
 };
@@ -323,11 +327,11 @@ struct WeightsPlan {
 WeightsPlan plan_weights(const slimkv_attention_weights_args* a) {
     WeightsPlan w{};
     const int64_t M = a->queries * (a->heads / a->kv_heads), tiles = (M + kRows - 1) / kRows;
-    w.groups = M <= 64 ? 0 : M <= 512 ? 2 : 4;
-    const int64_t keys = 64 * (w.groups ? w.groups : kFewGroups);          // of a workgroup
+    w.few = M <= 16;
+    const int64_t keys = w.few ? 128 : 256;        // of a workgroup
     w.blocks = (a->cache.keys + keys - 1) / keys;
     const int64_t workgroups = w.blocks * a->batch * a->kv_heads, want = 16 * device_cu_count();
-    w.splits = !w.groups || workgroups <= 0 ? 1 : (int)std::max<int64_t>(1, std::min(want / workgroups, tiles / 4));
+    w.splits = w.few || workgroups <= 0 ? 1 : (int)std::max<int64_t>(1, std::min(want / workgroups, tiles / 4));
     return w;
 }
 
@@ -346,17 +350,13 @@ int check_weights(const slimkv_attention_weights_args* a) {
     return SLIMKV_OK;
 }
 
-template <int D, bool F16, bool PAGED>
-auto weights_kernel(int groups) -> void (*)(WeightsParams) {
-    if (groups == 4) return weights_many_kernel<D, F16, 4, PAGED>;
-    return groups == 2 ? weights_many_kernel<D, F16, 2, PAGED> : weights_few_kernel<D, F16, PAGED>;
-}
-
 template <int D, bool F16>
-void launch_weights(const WeightsParams& p, int groups, hipStream_t st) {
+void launch_weights(const WeightsParams& p, bool few, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.blocks), (unsigned)p.splits);
-    hipLaunchKernelGGL((p.c.table ? weights_kernel<D, F16, true>(groups) : weights_kernel<D, F16, false>(groups)), grid,
-                       dim3(256), 0, st, p);
+    void (*kernel)(WeightsParams);
+    if (few) kernel = p.c.table ? weights_few_kernel<D, F16, true> : weights_few_kernel<D, F16, false>;
+    else kernel = p.c.table ? weights_many_kernel<D, F16, true> : weights_many_kernel<D, F16, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p);
 }
 
 }  // namespace
@@ -400,11 +400,11 @@ extern "C" int slimkv_attention_weights(const slimkv_attention_weights_args* a, 
     if ((int64_t)p.B * p.Hk * p.blocks > 0x7fffffff) return fail(SLIMKV_EINVAL, "attention weights: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->head_dim == 128) {
-        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<128, true>(p, plan.groups, st);
-        else launch_weights<128, false>(p, plan.groups, st);
+        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<128, true>(p, plan.few, st);
+        else launch_weights<128, false>(p, plan.few, st);
     } else {
-        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<64, true>(p, plan.groups, st);
-        else launch_weights<64, false>(p, plan.groups, st);
+        if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<64, true>(p, plan.few, st);
+        else launch_weights<64, false>(p, plan.few, st);
     }
     if (p.splits > 1) {
         const int64_t all = (int64_t)p.B * p.Hk * p.c.keys;

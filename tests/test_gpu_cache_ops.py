@@ -218,6 +218,10 @@ WEIGHTS = [
     (2, 65, 4, 4, 64, 300, [300, 64], 1, 'bf16', False, True),
     (1, 200, 4, 1, 128, 257, [201], 3, 'bf16', True, True),
     (3, 9, 6, 2, 64, 131, [131, 7, 130], 16, 'bf16', True, True),
+    (67, 18, 8, 2, 64, 300, [(13 * i) % 301 for i in range(67)], 16, 'bf16', True, True),
+    (2, 130, 8, 2, 128, 1400, [1400, 611], 0, 'fp16', True, True),
+    (1, 40, 6, 1, 128, 3001, None, 48, 'bf16', True, False),
+    (2, 19, 7, 1, 64, 515, [515, 100], 0, 'bf16', False, True),
 ]
 
 
