@@ -32,6 +32,7 @@ from ._lib import check, lib
 from .kernels import _status_word, check_status
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_NO_WORKSPACE = 16         # what a query answers for a call that uses none
 _CODES = {_lib.c_ptr: 'P', _lib.c_i64: 'q', _lib.c_f64: 'd', _lib.c_i32: 'i'}
 
 
@@ -111,6 +112,11 @@ def _lengths(name, lengths, batch):
     return lengths if lengths.is_contiguous() else lengths.contiguous()
 
 
+def _new(dtype, device, a, b, c):
+    """An uninitialised contiguous [a, b, c] (strides given: half torch.empty's time)."""
+    return torch.empty_strided((a, b, c), (b * c, c, 1), dtype=dtype, device=device)
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
@@ -186,8 +192,10 @@ def _call(device, entry, args, nbytes=None):
             return _call(device, entry, args, nbytes)
     if nbytes is None:
         check(entry(args, _lib.stream_handle(device)))
+    elif nbytes <= _NO_WORKSPACE:
+        check(entry(args, None, 0, _lib.stream_handle(device)))
     else:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=device)
         check(entry(args, ws.data_ptr(), nbytes, _lib.stream_handle(device)))
 
 
@@ -255,14 +263,14 @@ def tree_attention(q, draft_k, draft_v, scale, k=None, v=None, *, pages=None, ta
     device = _common(name, q, draft_k, draft_v, k, v, pages, table, lengths, mask, out, lse)
     q, draft_k, draft_v = _rows16(q), _rows16(draft_k), _rows16(draft_v)
     if out is None:
-        out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if lse is None:
-        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
+        lse = _new(torch.float32, device, B, Hq, T)
     status, owned = _status(name, status, device, paged)
     nbytes = _tree_bytes(device.index, B, T, Hq, H, D)
     a = _pack_tree(*place, _ptr(status), q.data_ptr(), *q.stride()[:3], draft_k.data_ptr(), *draft_k.stride()[:3],
                    draft_v.data_ptr(), *draft_v.stride()[:3], *m, out.data_ptr(), *out.stride()[:3], lse.data_ptr(),
-                   B, T, Hq, H, D, scale, code)
+                   B, T, Hq, H, D, float(scale), code)
     _call(device, lib().slimkv_tree_attention, a, nbytes)
     if owned:
         check_status(status)
@@ -298,17 +306,17 @@ def attention_weights(q, lse, scale, k=None, *, pages=None, table=None, lengths=
     if out is not None and previous is not None and _overlap(out, previous) and \
             (out.data_ptr() != previous.data_ptr() or out.stride() != previous.stride()):
         raise ValueError(f'{name}: out must be previous itself or lie apart from it')
-    if out is not None and any(n > 1 and s == 0 for n, s in zip(shape, out.stride())):
-        raise ValueError(f'{name}: out must not be an expanded view')
+    if out is not None and (any(n > 1 and s == 0 for n, s in zip(shape, out.stride())) or _overlap(out, lse)):
+        raise ValueError(f'{name}: out must not be an expanded view and lie apart from lse')
     device = _common(name, q, lse, k, pages, table, lengths, previous, out)
     if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=device)
+        out = _new(torch.float32, device, *shape)
     q = _rows16(q)
     status, owned = _status(name, status, device, paged)
     nbytes = _weights_bytes(device.index, B, L, Hq, H, D, rows)
     a = _pack_weights(*place, _ptr(status), q.data_ptr(), *q.stride()[:3], lse.data_ptr(), *lse.stride(),
                       *((previous.data_ptr(), *previous.stride()[:2]) if previous is not None else (0, 0, 0)),
-                      out.data_ptr(), *out.stride()[:2], B, L, Hq, H, D, scale, bool(causal), code)
+                      out.data_ptr(), *out.stride()[:2], B, L, Hq, H, D, float(scale), bool(causal), code)
     _call(device, lib().slimkv_attention_weights, a, nbytes)
     if owned:
         check_status(status)
@@ -332,8 +340,8 @@ def select_rows(weights, keep, *, lengths=None, sink=0, recent=0):
         weights = weights.contiguous()
     lengths = _lengths(name, lengths, B)
     device = _common(name, weights, lengths)
-    rows = torch.empty((B, H, keep), dtype=torch.int32, device=device)
-    counts = torch.empty(B, dtype=torch.int32, device=device)
+    rows = _new(torch.int32, device, B, H, keep)
+    counts = torch.empty_strided((B,), (1,), dtype=torch.int32, device=device)
     a = _pack_select(weights.data_ptr(), *weights.stride()[:2], _ptr(lengths), rows.data_ptr(), counts.data_ptr(), B, H, N,
                      keep, sink, recent)
     nbytes = _select_bytes(device.index, B, H, N, keep, sink, recent)
@@ -390,11 +398,11 @@ def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weight
     outs = (0, 0, 0, 0, 0, 0, 0, 0)
     if not in_place:
         if out_k is None:
-            out_k = torch.empty((B, keep, H, D), dtype=first.dtype, device=device)
+            out_k = torch.empty_strided((B, keep, H, D), (keep * H * D, H * D, D, 1), dtype=first.dtype, device=device)
         if out_v is None:
-            out_v = torch.empty((B, keep, H, D), dtype=first.dtype, device=device)
+            out_v = torch.empty_like(out_k, memory_format=torch.contiguous_format)
         if weights is not None:
-            out_weights = torch.empty((B, Hw, keep), dtype=torch.float32, device=device)
+            out_weights = _new(torch.float32, device, B, Hw, keep)
         outs = (out_k.data_ptr(), *out_k.stride()[:3], out_v.data_ptr(), *out_v.stride()[:3])
     status, owned = _status(name, status, device, True)
     a = _pack_compact(*place, status.data_ptr(), rows.data_ptr(), rows.stride(0), rows.stride(1) if Hw > 1 else 0,

@@ -555,8 +555,8 @@ extern "C" int slimkv_compact_rows(const slimkv_compact_rows_args* a, void* stre
         a->keep > ((int64_t)1 << 30) || a->weight_keys < 0 || a->weight_keys > ((int64_t)1 << 30) ||
         (a->weights && a->weight_heads != a->kv_heads && a->weight_heads != 1))
         return fail(SLIMKV_EINVAL, "compact rows: invalid sizes");
-    if (a->batch == 0 || a->keep == 0) return SLIMKV_OK;
-    if (!a->rows || !a->counts || (!a->in_place && (!a->out_k || !a->out_v || (a->weights && !a->out_weights))))
+    if (a->batch == 0 || (a->keep == 0 && !a->in_place)) return SLIMKV_OK;
+    if ((!a->rows && a->keep > 0) || !a->counts || (!a->in_place && (!a->out_k || !a->out_v || (a->weights && !a->out_weights))))
         return fail(SLIMKV_EINVAL, "compact rows: null pointer");
     CompactParams p{};
     const int view = cache_view(a->cache, a->batch, a->kv_heads, a->head_dim, true, "compact rows", &p.c);

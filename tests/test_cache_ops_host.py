@@ -127,6 +127,7 @@ line = z(2 * 2 * 9 + 4, dtype=torch.float32)
     (dict(out=z(2, 2, 9)), 'out must be'),
     (dict(previous=line[:36].view(2, 2, 9), out=line[4:].view(2, 2, 9)), 'previous itself'),
     (dict(k=z(2, 9, 3, 64)), 'multiple of 3'),
+    (dict(lse=line[:36].view(2, 6, 3), q=z(2, 3, 6, 64), out=line[4:].view(2, 2, 9)), 'apart from lse'),
 ])
 def test_attention_weights_refuses(over, match):
     with pytest.raises(ValueError, match=match):

@@ -108,6 +108,9 @@ TREE = [
     (70, 2, 4, 2, 64, 150, [(7 * i) % 151 for i in range(70)], 16, 'bf16', None),
     (1, 2, 2, 1, 128, 5003, None, 0, 'bf16', None),
     (2, 3, 2, 1, 64, 4001, [4001, 17], 16, 'fp16', 'none'),
+    (1, 5, 32, 1, 128, 300, None, 0, 'bf16', 'tree'),
+    (66, 9, 8, 1, 64, 140, [(11 * i) % 141 for i in range(66)], 16, 'fp16', 'tree'),
+    (3, 33, 32, 4, 128, 200, [200, 0, 131], 7, 'bf16', 'rows'),
 ]
 TYPES = {'bf16': torch.bfloat16, 'fp16': torch.float16}
 
@@ -197,6 +200,81 @@ def test_tree_offsets_past_32_bits():
     rows, counts = cache_ops.select_rows(w, 300, sink=2, recent=20)
     a, b = cache_ops.compact_rows(rows, counts, kk, vv)[:2], cache_ops.compact_rows(rows, counts, k, v)[:2]
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize('block', [1, 5, 16])
+@pytest.mark.parametrize('T,dtype', [(1, 'bf16'), (40, 'fp16')])
+def test_long_runs_over_small_pages(T, dtype, block):
+    """Runs longer than the stretch of page numbers kept in LDS: the bits of the same rows given densely."""
+    from slimkv_amd import cache_ops
+    B, H, D, N, g, dt = 2, 4, 64, 140001, gen(8), TYPES[dtype]
+    k, v = randn(g, B, N, H, D, dtype=dt), randn(g, B, N, H, D, dtype=dt)
+    cols = -(-N // block)
+    table = torch.randperm(B * cols, generator=g, device='cuda').view(B, cols)
+    pages = torch.zeros(B * cols, block, 2, H, D, dtype=dt, device='cuda')
+    for b in range(B):
+        rows = torch.zeros(cols * block, 2, H, D, dtype=dt, device='cuda')
+        rows[:N, 0], rows[:N, 1] = k[b], v[b]
+        pages[table[b]] = rows.view(cols, block, 2, H, D)
+    lengths = lengths_of([N, 70003])
+    q = randn(g, B, T, 2 * H, D, dtype=dt)
+    dk, dv = randn(g, B, T, H, D, dtype=dt), randn(g, B, T, H, D, dtype=dt)
+    want = cache_ops.tree_attention(q, dk, dv, 0.125, k, v, lengths=lengths)
+    got = cache_ops.tree_attention(q, dk, dv, 0.125, pages=pages, table=table, keys=N, lengths=lengths)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    w = cache_ops.attention_weights(q, want[1], 0.125, k, lengths=lengths)
+    assert torch.equal(cache_ops.attention_weights(q, want[1], 0.125, pages=pages, table=table, keys=N, lengths=lengths), w)
+
+
+def test_the_widest_tree_and_no_wider():
+    from slimkv_amd import cache_ops
+    g, D, T = gen(9), 64, 1024
+    q, dk, dv, k = (randn(g, 1, n, 1, D) for n in (T, T, T, 70))
+    out, lse = cache_ops.tree_attention(q, dk, dv, 0.125, k, k)
+    rows = torch.tensor([0, 1, 500, 1023], device='cuda')
+    keys = torch.cat([k, dk], 1)[0, :, 0].double().cpu()
+    values = torch.cat([k, dv], 1)[0, :, 0].double().cpu()
+    for t in rows.tolist():
+        s = (keys[:70 + t + 1] @ q[0, t, 0].double().cpu()) * 0.125
+        e = torch.softmax(s, 0) @ values[:70 + t + 1]
+        assert (out[0, t, 0].double().cpu() - e).abs().max() <= 2.0 ** -7 * values.abs().max()
+        assert abs(lse[0, 0, t].item() - torch.logsumexp(s, 0).item()) <= 1e-4
+    wide = randn(g, 1, T + 1, 1, D)
+    with pytest.raises(ValueError):
+        cache_ops.tree_attention(wide, wide, wide, 0.125, k, k)
+
+
+def test_pages_without_rows():
+    from slimkv_amd import cache_ops
+    g, D = gen(10), 128
+    pages = torch.full((4, 16, 2, 2, D), float('nan'), dtype=torch.bfloat16, device='cuda')
+    table = torch.full((1, 2), 99, dtype=torch.int64, device='cuda')        # no entry is read
+    q, dk, dv = randn(g, 1, 3, 4, D), randn(g, 1, 3, 2, D), randn(g, 1, 3, 2, D)
+    out, lse = cache_ops.tree_attention(q, dk, dv, D ** -0.5, pages=pages, table=table, keys=0)
+    none = torch.zeros(1, 0, 2, D, dtype=torch.bfloat16, device='cuda')
+    check_tree(out, lse, q, none, none, None, dk, dv, None, D ** -0.5)
+    again, _ = cache_ops.tree_attention(q, dk, dv, D ** -0.5, pages=pages, table=table, lengths=lengths_of([0]))
+    assert torch.equal(again, out)
+    assert not cache_ops.attention_weights(q, lse, 1.0, pages=pages, table=table, lengths=lengths_of([0])).any()
+
+
+def test_two_streams_at_once():
+    """The same calls on two streams side by side, each with its own workspace."""
+    from slimkv_amd import cache_ops
+    a, b = step_inputs(71)[0], step_inputs(72)[0]
+    want = [run_step(cache_ops, a), run_step(cache_ops, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    words = [torch.zeros(1, dtype=torch.int32, device='cuda') for _ in streams]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (s, st) in enumerate(zip((a, b), streams)):
+            with torch.cuda.stream(st):
+                got[i].append(run_step(cache_ops, s, words[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for out in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(out, want[i]))
 
 
 def test_tree_empty_calls():
@@ -372,6 +450,18 @@ def test_compact_rows(case, in_place):
             old = oc.dense_rows(bits(before), table, N)
             assert (kk[b, c[b]:] == old[0][b, c[b]:]).all() and (vv[b, c[b]:] == old[1][b, c[b]:]).all()
     assert (w.cpu().numpy()[:, :, :keep] == ew).all() and not w[:, :, keep:].any()
+
+
+def test_nothing_kept_in_place():
+    from slimkv_amd import cache_ops
+    g = gen(34)
+    k, v, _ = make_cache(g, 2, 9, 2, 64, 0, torch.bfloat16)
+    before, w = k.clone(), torch.rand(2, 2, 9, generator=g, device='cuda')
+    for keep in (0, 3):
+        rows = torch.zeros(2, 2, keep, dtype=torch.int32, device='cuda')
+        cache_ops.compact_rows(rows, torch.zeros(2, dtype=torch.int32, device='cuda'), k, v, weights=w, in_place=True)
+        assert torch.equal(k, before) and not w.any()
+        w.fill_(1.0)
 
 
 def test_compact_reports_bad_rows():
