@@ -2,22 +2,27 @@
 // rows of its sequence's cache and the drafted tokens its mask names.
 //
 // The T * G query rows of one KV head (row p = t * G + g) are the columns of
-// the score MFMA, as in the prefill kernel: S^T = K . Q^T with K rows as A and
-// the query rows held in registers as B, softmax statistics per lane column,
-// O^T = V^T . P^T with P^T straight from the score registers.  A workgroup of
-// four waves holds 16 RW NT rows: RW waves side by side on rows, 4 / RW waves
-// on the keys of a tile, joined at the end of an item.
+// the score MFMA: S^T = K . Q^T with K rows as A and the query rows held in
+// registers as B, so the softmax statistics stay in a lane's column, and O^T =
+// V^T . P^T with P^T straight from the score registers (weights rounded once to
+// the element type, their sum fp32 and unrounded).  K and V rows go from memory
+// straight to LDS, row by row; V is transposed by the LDS read.
 //
-// Key tiles of 64 rows -- the cache's, then the drafted tokens' -- pass through
-// LDS, the next one in registers.  The drafted tokens of a tile are masked by
-// their bytes; cache rows past the length read as zero and are masked.
+// Up to 32 query rows a KV head the cache's bytes are the bound: tree_few_kernel,
+// whose waves share nothing but the end (16 sequences of 8-32K paged rows, a
+// token each: 222 us for 1.34 GB, 6.0 TB/s; a copy moves 4.9-5.3).  More rows
+// are bound by the matrix cores and by how well loads hide behind them:
+// tree_many_kernel, 64 or 128 rows a workgroup (26 tokens on the same cache 283
+// us, 4.8 TB/s; 63 tokens of 40 heads over 131071 rows 262 us, 640 TFLOP/s of
+// needed work, 785 with the rows that fill up the last block of 128).
 //
-// Schedule.  The tiles of all (sequence, KV head) items lie in a row and are
-// dealt to `runs` workgroups in equal runs, whatever the lengths are; a run
-// that holds part of an item leaves its unnormalised output, maxima and sums
-// in the workspace for the merge kernel.  Each run exists once per block of
-// query rows, side by side on one XCD, so that the blocks share the tiles in
-// its L2.
+// Schedule.  The tiles of 64 rows of all (sequence, KV head) items -- the cache's
+// rows, then the drafted tokens' -- lie in a row and are dealt to two workgroups a
+// CU in equal runs, whatever the lengths are (four a CU: 26 tokens 358 us instead
+// of 318, six short chains 29 instead of 23); a run that holds part of an item
+// leaves its unnormalised output, maxima and sums in the workspace for the merge
+// kernel.  Each run exists once per block of query rows, side by side on one XCD,
+// so that the blocks share the tiles in its L2.
 
 #include "cache.hpp"
 
@@ -366,9 +371,8 @@ __device__ __forceinline__ u32x2 value_operand(const char* vs, int md) {
 constexpr int kDense = 0, kBlocks16 = 1, kAnyBlocks = 2;
 
 // A wave's view of the cache rows of one item: 16 consecutive rows into LDS.
-// Where the 16 rows lie in one tensor or in
-// one block, their first row is found on the scalar unit and a lane adds the
-// same offsets each time.
+// Where the 16 rows lie in one tensor or in one block, their first row is found
+// on the scalar unit and a lane adds the same offsets each time.
 template <int D, int PAGED>
 struct RowLoader {
     using R = Rows16<D>;
@@ -421,6 +425,17 @@ struct RowLoader {
             }
         }
     }
+};
+
+// A workgroup's LDS.  The rows come first, so that every address a load to LDS
+// names fits the 16 bits its base register holds for certain.
+template <int BYTES, int ROWS>
+struct alignas(1024) TreeLds {
+    char rows[BYTES];
+    Pages pages;
+    uint64_t seen[4][ROWS];       // drafted_seen's words, by wave
+    int wild;                     // drafted values that are not finite
+    static_assert(BYTES <= 65536, "addresses past 16 bits");
 };
 
 // The 16 rows from key0 on (draft: drafted ones) through registers, for rows
@@ -482,10 +497,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     using R = Rows16<D>;
     constexpr int KS = D / 32, MD = D / 16, kRows = 16 * NT, kPart = kRows * (D + 2), kWave = 4 * R::kBytes;
     constexpr int kBytes = 4 * kWave > 12 * kPart ? 4 * kWave : 12 * kPart;      // rings, or the join of three waves
-    __shared__ __attribute__((aligned(16))) char lds[kBytes];
-    __shared__ Pages pages;
-    __shared__ uint64_t seen[4][kRows];
-    __shared__ int wild;
+    __shared__ TreeLds<kBytes, kRows> sh;
+    char* lds = sh.rows;
+    Pages& pages = sh.pages;
+    auto& seen = sh.seen;
+    int& wild = sh.wild;
 
     const int run = slot_of_block();
     const Deal deal(p.deal, total_tiles(p.c, p.deal));
@@ -646,10 +662,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     constexpr int kTile = 8 * R::kBytes, kApart = 4 * R::kBytes;
     constexpr int kJoin = KW > 1 ? 4 * (KW - 1) * kPart : 0;
     constexpr int kBytes = 2 * kTile > kJoin ? 2 * kTile : kJoin;
-    __shared__ __attribute__((aligned(16))) char lds[kBytes];
-    __shared__ Pages pages;
-    __shared__ uint64_t seen[4][16 * NT];
-    __shared__ int wild;
+    __shared__ TreeLds<kBytes, 16 * NT> sh;
+    char* lds = sh.rows;
+    Pages& pages = sh.pages;
+    auto& seen = sh.seen;
+    int& wild = sh.wild;
 
     const int slot = slot_of_block();
     const int run = (uint32_t)slot / (uint32_t)p.row_blocks, rb = slot - run * p.row_blocks;
