@@ -129,7 +129,7 @@ int slimkv_select_rows(const slimkv_select_rows_args* a, void* workspace, size_t
  * weights (optional) [B, weight_heads, weight_keys] fp32 move along into
  * out_weights [B, weight_heads, keep], zero from counts[b] on; in place within
  * weights, whose entries from counts[b] on become zero.  weight_heads is the
- * head count of `rows` (1 or kv_heads).
+ * head count of `rows` (1 or kv_heads), or 0 without weights.
  * A row outside [0, keys) (in place: or not above the one before) moves
  * nothing, gives a zero row out of place, and stores SLIMKV_STATUS_BAD_SLOT;
  * a bad page entry likewise with SLIMKV_STATUS_BAD_PAGE.

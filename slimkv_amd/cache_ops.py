@@ -409,7 +409,7 @@ def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weight
                       counts.data_ptr(), *outs,
                       *((weights.data_ptr(), *weights.stride()[:2]) if weights is not None else (0, 0, 0)),
                       *((out_weights.data_ptr(), *out_weights.stride()[:2]) if out_weights is not None else (0, 0, 0)),
-                      Hw, 0 if weights is None else weights.shape[2], B, H, D, keep, bool(in_place), code)
+                      *((0, 0) if weights is None else (Hw, weights.shape[2])), B, H, D, keep, bool(in_place), code)
     _call(device, lib().slimkv_compact_rows, a)
     if owned:
         check_status(status)

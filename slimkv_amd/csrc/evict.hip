@@ -11,9 +11,8 @@
 // up for itself, so no launch waits for another workgroup.
 //
 // compact: bytes moved.  Out of place a lane moves 16 bytes of K and V of one
-// row; in place a workgroup takes a 64-byte column of one head's K or V and
-// walks the kept rows in order, reading a run of them before it writes them:
-// row i comes from a row not below i, and later rows come from above.
+// row; in place a workgroup takes some columns of one head's K or V and
+// walks the kept rows in order.
 
 #include "cache.hpp"
 
@@ -368,6 +367,7 @@ struct CompactParams {
     float* ow; int64_t ow_sb, ow_sh;
     int Hw, wkeys, B, Hk, D, keep;
     int move_blocks, weight_blocks;               // workgroups a sequence: K/V rows, weights
+    int lanes_log;                                // in place: log2 of the 16-byte lanes of a part
 };
 
 __device__ __forceinline__ int kept_count(const CompactParams& p, int64_t b) {
@@ -434,62 +434,120 @@ __global__ void __launch_bounds__(256) compact_kernel(CompactParams p) {
     *reinterpret_cast<u32x4*>(p.ov + b * p.ov_sb + i * p.ov_sn + h * p.ov_sh + d) = v;
 }
 
-// In place: blockIdx = ((sequence, KV head), K or V, 32-column part), then the
-// weights' workgroups.  256 threads move 64 rows of 64 bytes a step.
+// In place: blockIdx = ((sequence, KV head), K or V, part of the columns), then the
+// weights' workgroups.  A step reads the rows of kMoves places a thread, waits for
+// all of them, and writes.  Row i comes from a row not below i and the choice
+// ascends, so what a step reads lies past all that the steps before have written,
+// and one barrier a step (reads done, then writes) is enough.  Bound by the chain
+// of a step's dependent loads (row, block, data) where workgroups are few and by
+// HBM where they are many.  A part is 64 columns, whole lines, if that gives every
+// CU a workgroup, else 32: 16 sequences of 8 heads, 4096 rows kept of 32768, 136 us
+// against 178; one sequence, 34 us against 23.  Parts of 16: 294 and 25.  Steps of
+// 512 threads: 144 and 28.
+constexpr int kMoveThreads = 1024, kMoves = 8;
+
+// Whether place i of a choice may take row `row`, `prior` being the row before.
+__device__ __forceinline__ bool may_move(int row, int prior, int i, int keys) {
+    return row > prior && row >= i && row < keys;
+}
+
+// Every load above has reached its register, on all waves of the workgroup.
+__device__ __forceinline__ void reads_done() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 template <bool PAGED>
-__global__ void __launch_bounds__(256) compact_in_place_kernel(CompactParams p) {
-    const int cols = p.D / 32, per_head = 2 * cols;
+__global__ void __launch_bounds__(kMoveThreads) compact_in_place_kernel(CompactParams p) {
+    const int cols = p.D >> (p.lanes_log + 3), per_head = 2 * cols, tid = threadIdx.x;
     const int64_t b = blockIdx.y;
     const int count = kept_count(p, b);
     if ((int)blockIdx.x >= p.move_blocks) {
         const int h = (int)blockIdx.x - p.move_blocks;
         float* w = p.weights + b * p.w_sb + h * p.w_sh;
         const int32_t* rows = p.rows + b * p.r_sb + h * p.r_sh;
-        for (int i0 = 0; i0 < count; i0 += 256) {
-            const int i = i0 + threadIdx.x;
-            const int row = i < count ? rows[i] : -1;
-            const int prior = i > 0 && i < count ? rows[i - 1] : -1;
-            const bool good = i < count && row > prior && row >= i && row < p.wkeys;
-            if (i < count && !good) report_bad_row(p.c.status);
-            const float x = good ? w[row] : 0.f;
-            __syncthreads();
-            if (good) w[i] = x;
-            __syncthreads();
+        for (int i0 = 0; i0 < count; i0 += kMoves * kMoveThreads) {
+            int row[kMoves], prior[kMoves];
+            float x[kMoves];
+            bool good[kMoves];
+#pragma unroll
+            for (int y = 0; y < kMoves; ++y) {
+                const int i = min(i0 + y * kMoveThreads + tid, count - 1);
+                row[y] = rows[i];
+                prior[y] = rows[max(i - 1, 0)];
+            }
+#pragma unroll
+            for (int y = 0; y < kMoves; ++y) {
+                const int i = i0 + y * kMoveThreads + tid;
+                good[y] = i < count && may_move(row[y], i ? prior[y] : -1, i, p.wkeys);
+                if (i < count && !good[y]) report_bad_row(p.c.status);
+                if (good[y]) x[y] = w[row[y]];
+            }
+            reads_done();
+#pragma unroll
+            for (int y = 0; y < kMoves; ++y)
+                if (good[y]) w[i0 + y * kMoveThreads + tid] = x[y];
         }
-        for (int i = count + threadIdx.x; i < p.wkeys; i += 256) w[i] = 0.f;
+        __syncthreads();
+        for (int i = count + tid; i < p.wkeys; i += kMoveThreads) w[i] = 0.f;
         return;
     }
     const int h = (int)blockIdx.x / per_head, rest = (int)blockIdx.x % per_head;
-    const int kind = rest / cols, d = 32 * (rest % cols) + 8 * (threadIdx.x & 3);
+    const int lane = tid & ((1 << p.lanes_log) - 1), at = tid >> p.lanes_log;
+    const int kind = rest / cols, d = ((rest % cols) << (p.lanes_log + 3)) + 8 * lane;
     const int32_t* rows = p.rows + b * p.r_sb + h * p.r_sh;
     uint16_t* base = const_cast<uint16_t*>(kind ? p.c.v + h * p.c.v_sh : p.c.k + h * p.c.k_sh) + d;
-    for (int i0 = 0; i0 < count; i0 += 64) {
-        const int i = i0 + (threadIdx.x >> 2);
-        const int row = i < count ? rows[i] : -1;
-        const int prior = i > 0 && i < count ? rows[i - 1] : -1;
-        bool good = i < count && row > prior && row >= i && row < p.c.keys;
-        if (i < count && !good) report_bad_row(p.c.status);
-        uint16_t *src = base, *dst = base;
-        if (good) {
+    const int64_t sb = kind ? p.c.v_sb : p.c.k_sb, sn = kind ? p.c.v_sn : p.c.k_sn;
+    const int64_t* table = p.c.table + b * p.c.t_sb;
+    const int step = kMoveThreads >> p.lanes_log;          // rows a thread's moves lie apart
+    for (int i0 = 0; i0 < count; i0 += kMoves * step) {
+        int row[kMoves], prior[kMoves];
+        u32x4 x[kMoves];
+        uint16_t* dst[kMoves];                             // null: nothing moves
+#pragma unroll
+        for (int y = 0; y < kMoves; ++y) {
+            const int i = min(i0 + y * step + at, count - 1);
+            row[y] = rows[i];
+            prior[y] = rows[max(i - 1, 0)];
+        }
+        int64_t from[kMoves], to[kMoves];                  // blocks
+#pragma unroll
+        for (int y = 0; y < kMoves; ++y) {
+            const int i = i0 + y * step + at;
+            bool good = i < count && may_move(row[y], i ? prior[y] : -1, i, p.c.keys);
+            if (i < count && !good) report_bad_row(p.c.status);
             if constexpr (PAGED) {
-                const int64_t* table = p.c.table + b * p.c.t_sb;
-                if (table_page(table[quotient(row, p.c.block)], p.c.num_blocks) < 0 ||
-                    table_page(table[quotient(i, p.c.block)], p.c.num_blocks) < 0) {
-                    report_bad_page(p.c.status);
-                    good = false;
+                from[y] = good ? table_page(table[quotient(row[y], p.c.block)], p.c.num_blocks) : 0;
+                to[y] = good ? table_page(table[quotient(i, p.c.block)], p.c.num_blocks) : 0;
+            }
+            if (!good) row[y] = -1;
+        }
+#pragma unroll
+        for (int y = 0; y < kMoves; ++y) {
+            const int i = i0 + y * step + at;
+            dst[y] = nullptr;
+            const uint16_t* src = base;
+            if (row[y] >= 0) {
+                if constexpr (PAGED) {
+                    if (from[y] < 0 || to[y] < 0) {
+                        report_bad_page(p.c.status);
+                    } else {
+                        const int B = (int)p.c.block.d;
+                        src = base + from[y] * sb + (row[y] - quotient(row[y], p.c.block) * B) * sn;
+                        dst[y] = base + to[y] * sb + (i - quotient(i, p.c.block) * B) * sn;
+                    }
+                } else {
+                    src = base + b * sb + row[y] * sn;
+                    dst[y] = base + b * sb + i * sn;
                 }
             }
+            if (row[y] == i) dst[y] = nullptr;
+            if (dst[y]) x[y] = *reinterpret_cast<const u32x4*>(src);
         }
-        if (good) {
-            const RowAt from = cache_row<PAGED>(p.c, b, row), to = cache_row<PAGED>(p.c, b, i);
-            src = base + (kind ? from.v : from.k);
-            dst = base + (kind ? to.v : to.k);
-        }
-        u32x4 x = {0u, 0u, 0u, 0u};
-        if (good && row != i) x = *reinterpret_cast<const u32x4*>(src);
-        __syncthreads();                       // the step's rows are read
-        if (good && row != i) *reinterpret_cast<u32x4*>(dst) = x;
-        __syncthreads();                       // and written before the next step reads
+        reads_done();
+#pragma unroll
+        for (int y = 0; y < kMoves; ++y)
+            if (dst[y]) *reinterpret_cast<u32x4*>(dst[y]) = x[y];
     }
 }
 
@@ -553,10 +611,11 @@ extern "C" int slimkv_compact_rows(const slimkv_compact_rows_args* a, void* stre
         return fail(SLIMKV_EUNSUP, "compact rows: element type must be bf16 or fp16");
     if (a->batch < 0 || a->batch > 65535 || a->kv_heads <= 0 || a->kv_heads > 4096 || a->keep < 0 ||
         a->keep > ((int64_t)1 << 30) || a->weight_keys < 0 || a->weight_keys > ((int64_t)1 << 30) ||
-        (a->weights && a->weight_heads != a->kv_heads && a->weight_heads != 1))
+        (a->weight_heads != 0 && a->weight_heads != a->kv_heads && a->weight_heads != 1))
         return fail(SLIMKV_EINVAL, "compact rows: invalid sizes");
     if (a->batch == 0 || (a->keep == 0 && !a->in_place)) return SLIMKV_OK;
-    if ((!a->rows && a->keep > 0) || !a->counts || (!a->in_place && (!a->out_k || !a->out_v || (a->weights && !a->out_weights))))
+    if ((!a->rows && a->keep > 0) || !a->counts || (a->weight_heads && a->weight_keys && !a->weights) ||
+        (!a->in_place && (!a->out_k || !a->out_v || (a->weight_heads && !a->out_weights))))
         return fail(SLIMKV_EINVAL, "compact rows: null pointer");
     CompactParams p{};
     const int view = cache_view(a->cache, a->batch, a->kv_heads, a->head_dim, true, "compact rows", &p.c);
@@ -574,20 +633,21 @@ extern "C" int slimkv_compact_rows(const slimkv_compact_rows_args* a, void* stre
     hipStream_t st = static_cast<hipStream_t>(stream);
     int64_t move, weights;
     if (a->in_place) {
-        move = a->kv_heads * 2 * (a->head_dim / 32);
-        weights = a->weights ? a->weight_heads : 0;
+        p.lanes_log = (int64_t)a->batch * a->kv_heads * 2 * (a->head_dim / 64) >= device_cu_count() ? 3 : 2;
+        move = a->kv_heads * 2 * (a->head_dim >> (p.lanes_log + 3));
+        weights = a->weight_heads;
     } else {
         const int64_t per = 256 / (a->head_dim / 8);
         move = (a->keep * a->kv_heads + per - 1) / per;
-        weights = a->weights ? (a->weight_heads * a->keep + 255) / 256 : 0;
+        weights = (a->weight_heads * a->keep + 255) / 256;
     }
     if (move + weights > 0x7fffffff) return fail(SLIMKV_EINVAL, "compact rows: too many rows for one call");
     p.move_blocks = (int)move;
     p.weight_blocks = (int)weights;
     const dim3 grid((unsigned)(move + weights), (unsigned)a->batch);
     if (a->in_place) {
-        if (p.c.table) hipLaunchKernelGGL(compact_in_place_kernel<true>, grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL(compact_in_place_kernel<false>, grid, dim3(256), 0, st, p);
+        if (p.c.table) hipLaunchKernelGGL(compact_in_place_kernel<true>, grid, dim3(kMoveThreads), 0, st, p);
+        else hipLaunchKernelGGL(compact_in_place_kernel<false>, grid, dim3(kMoveThreads), 0, st, p);
     } else {
         void (*kernel)(CompactParams);
         if (p.r_sh) kernel = p.c.table ? compact_kernel<true, true> : compact_kernel<false, true>;

@@ -407,6 +407,9 @@ COMPACT = [
     (2, 8, 128, 700, 257, False, 48, 'fp16'),
     (1, 1, 128, 300, 300, False, 1, 'bf16'),
     (3, 2, 64, 90, 33, True, 0, 'fp16'),
+    (1, 2, 128, 9000, 4500, False, 16, 'bf16'),
+    (8, 8, 128, 2900, 2300, False, 32, 'fp16'),
+    (1, 1, 64, 20000, 18001, False, 0, 'bf16'),
 ]
 
 
@@ -481,6 +484,26 @@ def test_compact_reports_bad_rows():
     with pytest.raises(IndexError):                    # out of order in place
         cache_ops.compact_rows(rows, counts, k, v, in_place=True)
     assert torch.equal(k[0, 3:], before[0][0, 3:])
+
+
+@pytest.mark.parametrize('in_place', [False, True])
+@pytest.mark.parametrize('held', [0, 4])
+def test_weights_shorter_than_the_choice(held, in_place):
+    from slimkv_amd import cache_ops
+    g = gen(35)
+    k, v, _ = make_cache(g, 1, 9, 2, 64, 0, torch.bfloat16)
+    w = torch.rand(1, 2, held, generator=g, device='cuda')
+    rows = torch.tensor([[[0, 2, 5, 8], [1, 2, 3, 4]]], dtype=torch.int32, device='cuda')
+    counts = torch.tensor([4], dtype=torch.int32, device='cuda')
+    before, kept = k.clone(), w.clone()
+    with pytest.raises(IndexError):
+        cache_ops.compact_rows(rows, counts, k, v, weights=w, in_place=in_place)
+    if in_place:                                       # rows that the cache has are moved all the same
+        assert torch.equal(k[0, :4, 0], before[0, [0, 2, 5, 8], 0])
+        if held:
+            assert torch.equal(w[0, 0, :2], kept[0, 0, [0, 2]]) and torch.equal(w[0, 1, :3], kept[0, 1, 1:4])
+    else:
+        assert torch.equal(k, before) and torch.equal(w, kept)
 
 
 def test_bad_pages_are_reported():
