@@ -6,9 +6,9 @@
 // the weight of the last row kept and how many rows of exactly that weight fit;
 // a last pass counts and writes the kept rows in ascending order.  All counts
 // are integers, so the result does not depend on the order of the LDS atomics.
-// Rows that one workgroup would take long over are cut into chunks: a launch
-// makes each chunk's histogram, and every workgroup of the next one adds them
-// up for itself, so no launch waits for another workgroup.
+// Up to 32768 rows one workgroup holds in registers.  More are cut into chunks: a
+// launch makes each chunk's histogram, and every workgroup of the next one adds
+// them up for itself, so no launch waits for another workgroup.
 //
 // compact: bytes moved.  Out of place a lane moves 16 bytes of K and V of one
 // row; in place a workgroup takes some columns of one head's K or V and
@@ -21,6 +21,8 @@ namespace slimkv {
 namespace {
 
 constexpr int kSelectThreads = 512, kSelectWaves = kSelectThreads / 64;
+constexpr int kHeldThreads = 1024, kHeldWaves = kHeldThreads / 64, kMostHeld = 32;   // values a thread keeps
+constexpr int kCopies = 4;        // of the first histogram, for lanes that meet in a bin
 constexpr int kBins = 2048, kLastBins = 1024;
 constexpr int kBatch = 8;         // loads a thread has open at once
 
@@ -36,13 +38,13 @@ struct SelectParams {
 
 // Order-preserving image of a weight: -0 as +0, NaN below everything.
 __device__ __forceinline__ uint32_t rank_of(float w) {
-    if (w != w) return 0u;
     const uint32_t u = __float_as_uint(w == 0.f ? 0.f : w);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    return w != w ? 0u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
-__device__ __forceinline__ int lanes_below(uint64_t mask, int lane) {
-    return __popcll(mask & (((uint64_t)1 << lane) - 1));
+// Set bits of a wave's mask below this lane's.
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
 // One (sequence, head): the ranked rows [first, last), of which `need` are
@@ -80,13 +82,14 @@ struct SelectRow {
     __device__ __forceinline__ void write_given(const SelectParams& p, int item) const {
         const int count = min(n, p.keep), tid = threadIdx.x;
         if (item % p.H == 0 && tid == 0) p.counts[item / p.H] = count;
-        for (int i = count + tid; i < p.keep; i += kSelectThreads) rows[i] = -1;
+        const int threads = blockDim.x;
+        for (int i = count + tid; i < p.keep; i += threads) rows[i] = -1;
         if (n <= p.keep) {
-            for (int i = tid; i < n; i += kSelectThreads) rows[i] = i;
+            for (int i = tid; i < n; i += threads) rows[i] = i;
             return;
         }
-        for (int i = tid; i < p.sink; i += kSelectThreads) rows[i] = i;
-        for (int i = tid; i < p.recent; i += kSelectThreads) rows[p.keep - p.recent + i] = n - p.recent + i;
+        for (int i = tid; i < p.sink; i += threads) rows[i] = i;
+        for (int i = tid; i < p.recent; i += threads) rows[p.keep - p.recent + i] = n - p.recent + i;
     }
 };
 
@@ -94,10 +97,18 @@ struct SelectRow {
 struct SelectLds {
     uint32_t hist[kBins];
     uint32_t bin, above;
-    uint32_t wave[2][kSelectWaves];
+    uint32_t wave[2][kHeldWaves];
 };
 
+// No row counted yet, once all threads are past what they read of s.
+__device__ __forceinline__ void clear_bins(SelectLds& s) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += blockDim.x) s.hist[i] = 0;
+    __syncthreads();
+}
+
 // Sum of x over the workgroup's threads below this one, and over all of them.
+template <int THREADS = kSelectThreads>
 __device__ __forceinline__ uint32_t block_before(uint32_t x, SelectLds& s, uint32_t* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t upto = x;
@@ -111,7 +122,7 @@ __device__ __forceinline__ uint32_t block_before(uint32_t x, SelectLds& s, uint3
     __syncthreads();
     uint32_t below = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kSelectWaves; ++i) {
+    for (int i = 0; i < THREADS / 64; ++i) {
         below += i < wave ? s.wave[0][i] : 0u;
         all += s.wave[0][i];
     }
@@ -121,13 +132,13 @@ __device__ __forceinline__ uint32_t block_before(uint32_t x, SelectLds& s, uint3
 
 // The bin, from the highest down, that holds row `left` (counted from 1):
 // s.bin, and s.above rows in the bins above it.
-template <int NB>
+template <int NB, int THREADS = kSelectThreads>
 __device__ __forceinline__ void find_bin(SelectLds& s, uint32_t left) {
-    constexpr int K = NB / kSelectThreads;
+    constexpr int K = NB / THREADS;
     uint32_t c[K], sum = 0, all;
 #pragma unroll
     for (int x = 0; x < K; ++x) sum += c[x] = s.hist[NB - 1 - (K * (int)threadIdx.x + x)];
-    uint32_t before = block_before(sum, s, &all);
+    uint32_t before = block_before<THREADS>(sum, s, &all);
 #pragma unroll
     for (int x = 0; x < K; ++x) {
         if (before < left && before + c[x] >= left) {
@@ -243,16 +254,105 @@ __device__ __forceinline__ void write_taken(const SelectRow& r, SelectLds& s, ui
             const int i = i0 + 64 * k + lane;
             const uint32_t u = rank_of(x[k]);
             const uint64_t eq = __ballot(i < to && u == least);
-            const bool take = i < to && (u > least || (u == least && same + lanes_below(eq, lane) < left));
+            const bool take = i < to && (u > least || (u == least && same + lanes_below(eq) < left));
             const uint64_t all = __ballot(take);
-            if (take) dst[lanes_below(all, lane)] = i;
+            if (take) dst[lanes_below(all)] = i;
             dst += __popcll(all);
             same += __popcll(eq);
         }
     }
 }
 
-// A row in one workgroup.
+// A row whose values one workgroup holds, VALUES a thread: read once, ranked and
+// written from registers.  A wave owns a contiguous part.  What lies behind the
+// ranked rows has rank 0, the lowest, and the highest places: it is never taken.
+// Bound by its instructions, some 85 for 64 values, and the LDS atomics.  Against
+// chunks over four launches: 8 rows of 32768 values 18 us (26), 128 rows of 16384
+// 12.5 (27.6) and of 32768 18 (37), 512 of 32768 41 (80).  Weights lie in few bins
+// of the first level, zeros in one: rows of which half are zero take 29 us with
+// one copy of its histogram, 20 with four, eight or sixteen.
+template <int VALUES>
+__global__ void __launch_bounds__(kHeldThreads) select_held_kernel(SelectParams p) {
+    __shared__ SelectLds s;
+    __shared__ uint32_t copies[kBins * kCopies];
+    const SelectRow r(p, blockIdx.x, 0);
+    r.write_given(p, blockIdx.x);
+    if (r.trivial) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int first = r.first + 64 * VALUES * wave + lane;
+    uint32_t u[VALUES], left = r.need;
+    {
+        float x[VALUES];
+#pragma unroll
+        for (int k = 0; k < VALUES; ++k) x[k] = r.w[min(first + 64 * k, r.last - 1)];
+        for (int i = tid; i < kBins * kCopies; i += kHeldThreads) copies[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < VALUES; ++k) u[k] = first + 64 * k < r.last ? rank_of(x[k]) : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k) atomicAdd(&copies[(u[k] >> 21) * kCopies + lane % kCopies], 1u);
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kHeldThreads) {
+        uint32_t sum = 0;
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) sum += copies[i * kCopies + c];
+        s.hist[i] = sum;
+    }
+    __syncthreads();
+    find_bin<kBins, kHeldThreads>(s, left);
+    uint32_t prefix = s.bin << 21;
+    left -= s.above;
+    clear_bins(s);
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k)
+        if (u[k] - prefix < 1u << 21) atomicAdd(&s.hist[(u[k] - prefix) >> 10], 1u);
+    __syncthreads();
+    find_bin<kBins, kHeldThreads>(s, left);
+    prefix |= s.bin << 10;
+    left -= s.above;
+    clear_bins(s);
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k)
+        if (u[k] - prefix < 1u << 10) atomicAdd(&s.hist[u[k] - prefix], 1u);
+    __syncthreads();
+    find_bin<kLastBins, kHeldThreads>(s, left);
+    const uint32_t least = prefix | s.bin;
+    const int wanted = (int)(left - s.above);
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k) {
+        above += __popcll(__ballot(u[k] > least));
+        equal += __popcll(__ballot(u[k] == least));
+    }
+    __syncthreads();
+    if (lane == 0) {
+        s.wave[0][wave] = above;
+        s.wave[1][wave] = equal;
+    }
+    __syncthreads();
+    int at = p.sink, same = 0;
+    for (int x = 0; x < wave; ++x) {
+        at += (int)s.wave[0][x] + min((int)s.wave[1][x], max(0, wanted - same));
+        same += (int)s.wave[1][x];
+    }
+    int32_t* dst = r.rows + uniform(at);
+    same = uniform(same);
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k) {
+        asm volatile("" : "+v"(u[k]));                     // compared anew: the masks of the counting are too many to keep
+        const uint64_t eq = __ballot(u[k] == least);
+        uint64_t all = __ballot(u[k] > least);
+        if (eq && same < wanted) {
+            all |= __ballot(u[k] == least && same + lanes_below(eq) < wanted);
+            same += __popcll(eq);
+        }
+        if (__builtin_amdgcn_inverse_ballot_w64(all)) dst[lanes_below(all)] = first + 64 * k;
+        dst += __popcll(all);
+    }
+}
+
+// A longer row in one workgroup, where rows are many.
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(SelectParams p) {
     __shared__ SelectLds s;
     const SelectRow r(p, blockIdx.x, 0);
@@ -344,9 +444,10 @@ __global__ void __launch_bounds__(kSelectThreads) select_chunk_kernel(SelectPara
     }
 }
 
-// Chunks of a row: of 8192 values, at most 32, and no more than give four
-// workgroups a CU over all rows.
+// Chunks of a row that no workgroup holds: of 8192 values, at most 32, and no more
+// than give four workgroups a CU over all rows.
 int select_chunks(const slimkv_select_rows_args* a) {
+    if (a->keys <= kMostHeld * kHeldThreads) return 1;
     const int64_t rows = std::max<int64_t>(1, a->batch * a->heads), most = 4 * device_cu_count() / rows;
     return (int)std::max<int64_t>(1, std::min<int64_t>({(a->keys + 8191) / 8192, 32, most}));
 }
@@ -589,7 +690,13 @@ extern "C" int slimkv_select_rows(const slimkv_select_rows_args* a, void* worksp
     p.ws = static_cast<uint32_t*>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const unsigned rows = (unsigned)(a->batch * a->heads);
-    if (p.chunks == 1) {
+    if (a->keys <= kMostHeld * kHeldThreads) {
+        void (*kernel)(SelectParams) = a->keys <= 4 * kHeldThreads    ? select_held_kernel<4>
+                                       : a->keys <= 8 * kHeldThreads  ? select_held_kernel<8>
+                                       : a->keys <= 16 * kHeldThreads ? select_held_kernel<16>
+                                                                      : select_held_kernel<kMostHeld>;
+        hipLaunchKernelGGL(kernel, dim3(rows), dim3(kHeldThreads), 0, st, p);
+    } else if (p.chunks == 1) {
         hipLaunchKernelGGL(select_kernel, dim3(rows), dim3(kSelectThreads), 0, st, p);
     } else {
         if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) || workspace_bytes < select_bytes(a))

@@ -378,6 +378,9 @@ SELECT = [
     (2, 1, 20000, 3000, [20000, 9001], 5, 40),
     (1, 3, 40007, 20001, [40000], 0, 0),
     (130, 2, 9001, 100, [(97 * i) % 9002 for i in range(130)], 2, 3),
+    (2, 2, 32768, 30000, [32768, 30001], 0, 1),
+    (1, 2, 32769, 8000, None, 1, 0),
+    (1030, 1, 33001, 100, [33001 - i if i % 103 == 0 else (7 * i) % 400 for i in range(1030)], 4, 8),
 ]
 
 
