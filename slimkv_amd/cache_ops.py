@@ -104,6 +104,10 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
+def _expanded(t):
+    return any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))
+
+
 def _lengths(name, lengths, batch):
     if lengths is None:
         return None
@@ -255,11 +259,14 @@ def tree_attention(q, draft_k, draft_v, scale, k=None, v=None, *, pages=None, ta
         if mask.stride(-1) != 1:
             mask = mask.contiguous()
         m = (mask.data_ptr(), mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
-    if out is not None and (out.shape != q.shape or out.stride(3) != 1 or
-                            any(t is not None and _overlap(out, t) for t in (q, draft_k, draft_v, k, v, pages))):
-        raise ValueError(f'{name}: out must have the shape of q with contiguous features, apart from the inputs')
-    if lse is not None and (lse.shape != (B, Hq, T) or lse.dtype is not torch.float32 or not lse.is_contiguous()):
-        raise ValueError(f'{name}: lse must be a contiguous float32 [{B}, {Hq}, {T}]')
+    inputs = (q, draft_k, draft_v, k, v, pages, table, lengths, mask)
+    if out is not None and (out.shape != q.shape or out.stride(3) != 1 or _expanded(out) or
+                            any(t is not None and _overlap(out, t) for t in inputs)):
+        raise ValueError(f'{name}: out must have the shape of q with contiguous features, no expanded view and apart '
+                         'from the inputs')
+    if lse is not None and (lse.shape != (B, Hq, T) or lse.dtype is not torch.float32 or not lse.is_contiguous() or
+                            any(t is not None and _overlap(lse, t) for t in (*inputs, out))):
+        raise ValueError(f'{name}: lse must be a contiguous float32 [{B}, {Hq}, {T}], apart from the other tensors')
     device = _common(name, q, draft_k, draft_v, k, v, pages, table, lengths, mask, out, lse)
     q, draft_k, draft_v = _rows16(q), _rows16(draft_k), _rows16(draft_v)
     if out is None:
@@ -306,8 +313,9 @@ def attention_weights(q, lse, scale, k=None, *, pages=None, table=None, lengths=
     if out is not None and previous is not None and _overlap(out, previous) and \
             (out.data_ptr() != previous.data_ptr() or out.stride() != previous.stride()):
         raise ValueError(f'{name}: out must be previous itself or lie apart from it')
-    if out is not None and (any(n > 1 and s == 0 for n, s in zip(shape, out.stride())) or _overlap(out, lse)):
-        raise ValueError(f'{name}: out must not be an expanded view and lie apart from lse')
+    if out is not None and (_expanded(out) or any(t is not None and _overlap(out, t)
+                                                  for t in (lse, q, k, pages, table, lengths))):
+        raise ValueError(f'{name}: out must not be an expanded view and lie apart from lse and the other inputs')
     device = _common(name, q, lse, k, pages, table, lengths, previous, out)
     if out is None:
         out = _new(torch.float32, device, *shape)
@@ -383,15 +391,16 @@ def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weight
         if out_k is not None or out_v is not None:
             raise ValueError(f'{name}: in place there are no outputs')
         for t in (k, v, pages, weights):
-            if t is not None and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+            if t is not None and _expanded(t):
                 raise ValueError(f'{name}: in place the cache must not be an expanded view')
         if k is not None and k.numel() and k.data_ptr() == v.data_ptr():
             raise ValueError(f'{name}: in place k and v must be two tensors')
     sources = [t for t in (k, v, pages) if t is not None]
     for t in (out_k, out_v):
-        if t is not None and (t.shape != (B, keep, H, D) or t.stride(3) != 1 or any(_overlap(t, s) for s in sources)):
-            raise ValueError(f'{name}: outputs must be [{B}, {keep}, {H}, {D}] with contiguous features, apart from '
-                             'the cache')
+        if t is not None and (t.shape != (B, keep, H, D) or t.stride(3) != 1 or _expanded(t) or
+                              any(_overlap(t, s) for s in sources)):
+            raise ValueError(f'{name}: outputs must be [{B}, {keep}, {H}, {D}] with contiguous features, no expanded '
+                             'views and apart from the cache')
     if out_k is not None and out_v is not None and _overlap(out_k, out_v):
         raise ValueError(f'{name}: out_k and out_v must lie apart')
     device = _common(name, rows, counts, k, v, pages, table, weights, out_k, out_v)

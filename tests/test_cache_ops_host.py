@@ -74,6 +74,7 @@ def tree(**over):
 
 PAGED = dict(k=None, v=None, pages=z(6, 4, 2, 2, 64), table=z(2, 3, dtype=torch.int64))
 shared = z(2 * 3 * 8 * 64 + 8)
+floats = z(3 * 8 * 64, dtype=torch.float32)
 
 
 @pytest.mark.parametrize('over,match', [
@@ -97,6 +98,9 @@ shared = z(2 * 3 * 8 * 64 + 8)
     (dict(out=z(2, 3, 8, 32)), 'out must have'),
     (dict(q=shared[:-8].view(2, 3, 8, 64), out=shared[8:].view(2, 3, 8, 64)), 'apart from the inputs'),
     (dict(lse=z(2, 8, 3)), 'lse must be'),
+    (dict(out=z(1, 3, 8, 64).expand(2, 3, 8, 64)), 'no expanded view'),
+    (dict(lse=floats[:48].view(2, 8, 3), out=floats.view(BF16).view(2, 3, 8, 64)), 'lse must be .* apart'),
+    (dict(lse=floats[8:56].view(2, 8, 3), lengths=floats.view(torch.int32)[55:57]), 'lse must be .* apart'),
     (dict(keys=9), 'belong to pages'),
     (dict(PAGED, keys=13), 'keys must lie'),
     (dict(PAGED, table=z(2, 3, dtype=torch.int32)), 'int64 block table'),
@@ -128,6 +132,8 @@ line = z(2 * 2 * 9 + 4, dtype=torch.float32)
     (dict(previous=line[:36].view(2, 2, 9), out=line[4:].view(2, 2, 9)), 'previous itself'),
     (dict(k=z(2, 9, 3, 64)), 'multiple of 3'),
     (dict(lse=line[:36].view(2, 6, 3), q=z(2, 3, 6, 64), out=line[4:].view(2, 2, 9)), 'apart from lse'),
+    (dict(out=z(1, 2, 9, dtype=torch.float32).expand(2, 2, 9)), 'expanded view'),
+    (dict(q=floats.view(BF16).view(2, 3, 8, 64), out=floats[:36].view(2, 2, 9)), 'apart from lse and the other'),
 ])
 def test_attention_weights_refuses(over, match):
     with pytest.raises(ValueError, match=match):
@@ -169,6 +175,7 @@ cache = z(2 * 9 * 2 * 64)
     (dict(in_place=True, k=cache.view(2, 9, 2, 64), v=cache.view(2, 9, 2, 64)), 'two tensors'),
     (dict(out_k=z(2, 4, 2, 32)), 'outputs must be'),
     (dict(k=cache.view(2, 9, 2, 64), out_k=cache[:1024].view(2, 4, 2, 64)), 'apart from the cache'),
+    (dict(out_v=z(1, 4, 2, 64).expand(2, 4, 2, 64)), 'no expanded'),
 ])
 def test_compact_rows_refuses(over, match):
     with pytest.raises(ValueError, match=match):
