@@ -70,6 +70,9 @@ inline FastDiv fast_div(int64_t d) {
 
 __device__ __forceinline__ int quotient(int n, const FastDiv& f) { return (int)(((uint64_t)(uint32_t)n * f.m) >> f.shift); }
 
+// A softmax scale whose fp32 image times a score of -inf stays -inf.
+inline bool scale_usable(double scale) { return scale >= 1e-18 && scale <= 1e18; }
+
 struct CacheView {
     const uint16_t* k; int64_t k_sb, k_sn, k_sh;
     const uint16_t* v; int64_t v_sb, v_sn, v_sh;

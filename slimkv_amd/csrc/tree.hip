@@ -990,7 +990,7 @@ int check_tree(const slimkv_tree_attention_args* a) {
     if (a->batch < 0 || a->batch > 65535 || a->drafted < 0 || a->drafted > kMaxDrafted || a->heads <= 0 || a->kv_heads <= 0 ||
         a->heads % a->kv_heads || a->heads > 4096 || a->heads / a->kv_heads > 256)
         return fail(SLIMKV_EINVAL, "tree attention: invalid sizes");
-    if (!(a->scale > 0.0)) return fail(SLIMKV_EINVAL, "tree attention: the softmax scale must be positive");
+    if (!scale_usable(a->scale)) return fail(SLIMKV_EINVAL, "tree attention: the softmax scale must lie in [1e-18, 1e18]");
     return SLIMKV_OK;
 }
 

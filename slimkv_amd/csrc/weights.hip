@@ -385,7 +385,7 @@ int check_weights(const slimkv_attention_weights_args* a) {
     if (a->batch < 0 || a->batch > 65535 || a->queries < 0 || a->queries > (1 << 20) || a->heads <= 0 ||
         a->kv_heads <= 0 || a->heads % a->kv_heads || a->heads > 4096 || a->heads / a->kv_heads > 256)
         return fail(SLIMKV_EINVAL, "attention weights: invalid sizes");
-    if (!(a->scale > 0.0)) return fail(SLIMKV_EINVAL, "attention weights: the softmax scale must be positive");
+    if (!scale_usable(a->scale)) return fail(SLIMKV_EINVAL, "attention weights: the softmax scale must lie in [1e-18, 1e18]");
     if (a->cache.keys < 0 || a->cache.keys > ((int64_t)1 << 30))
         return fail(SLIMKV_EINVAL, "attention weights: invalid cache length");
     return SLIMKV_OK;

@@ -195,7 +195,8 @@ def test_the_c_entry_points_refuse_bad_sizes():
     assert lib.slimkv_tree_attention(ref(a), 4096, need - 1, None) == -3
     assert lib.slimkv_tree_attention(ref(a), None, need, None) == -3
     for field, value, code in (('head_dim', 96, -2), ('dtype', 2, -2), ('drafted', 1025, -1), ('heads', 9, -1),
-                               ('scale', 0.0, -1), ('batch', -1, -1), ('q', 4098, -1), ('draft_k', 0, -1)):
+                               ('scale', 0.0, -1), ('scale', float('inf'), -1), ('scale', 1e-60, -1), ('scale', float('nan'), -1),
+                               ('batch', -1, -1), ('q', 4098, -1), ('draft_k', 0, -1)):
         old = getattr(a, field)
         setattr(a, field, value)
         assert lib.slimkv_tree_attention(ref(a), 4096, need, None) == code, field
@@ -211,6 +212,10 @@ def test_the_c_entry_points_refuse_bad_sizes():
     assert b'16-byte' in lib.slimkv_last_error()
     w = _lib.AttentionWeightsArgs()
     assert lib.slimkv_attention_weights(ref(w), None, 0, None) < 0
+    w = _lib.AttentionWeightsArgs(batch=1, queries=1, heads=2, kv_heads=1, head_dim=64)
+    for scale in (0.0, float('inf'), 1e-60, float('nan')):
+        w.scale = scale
+        assert lib.slimkv_attention_weights(ref(w), None, 0, None) == -1 and b'scale' in lib.slimkv_last_error()
     s = _lib.SelectRowsArgs()
     s.batch, s.heads, s.keys, s.keep, s.sink = 1, 1, 10, 4, 5
     assert lib.slimkv_select_rows(ref(s), None, 0, None) == -1
