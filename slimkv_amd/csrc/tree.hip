@@ -175,6 +175,21 @@ __device__ __forceinline__ void load_queries(const TreeParams& p, int64_t b, int
     }
 }
 
+// A score's exponent against the row's base.  Fused, it is rounded once, but the
+// largest score then ends at the rounding of its product, which is in the base: up
+// to half a step of it either way, past the exponents of fp16 from 2^28 on and of
+// fp32 from 2^31.  From kFarBase on the products are rounded before the
+// difference, as they were for the base, and the largest ends at zero.
+constexpr float kFarBase = 1048576.f;
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+__device__ __forceinline__ float far_exponent(float s, float scale_log2, float base) {
+#pragma clang fp contract(off)
+    return __builtin_fabsf(base) >= kFarBase ? rounded_product(s, scale_log2) - base : __builtin_fmaf(s, scale_log2, -base);
+}
+
 // One online-softmax step of a column's scores: the scores become weights, the
 // state moves to the new maximum.  The weights' sum is fp32 and of the
 // unrounded weights; a lane keeps the sum of its own keys.
@@ -186,18 +201,22 @@ __device__ __forceinline__ void softmax_step(v4f (&s)[MT], float scale_log2, flo
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][i]);
     mx = rows_max(mx);
-    const float m_new = fmaxf(m, mx * scale_log2);
+    const float m_new = fmaxf(m, rounded_product(mx, scale_log2));
     const float base = m_new == kNegInf ? 0.f : m_new;
     const float alpha = fast_exp2(m - base);
     m = m_new;
     float sum = 0.f;
+    auto weigh = [&](auto exponent) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[mt][i] = fast_exp2(__builtin_fmaf(s[mt][i], scale_log2, -base));
-            sum += s[mt][i];
-        }
+            for (int i = 0; i < 4; ++i) {
+                s[mt][i] = fast_exp2(exponent(s[mt][i]));
+                sum += s[mt][i];
+            }
+    };
+    if (__ballot(__builtin_fabsf(base) >= kFarBase)) weigh([&](float x) { return far_exponent(x, scale_log2, base); });
+    else weigh([&](float x) { return __builtin_fmaf(x, scale_log2, -base); });
     if (__ballot(alpha != 1.f)) {
 #pragma unroll
         for (int md = 0; md < MD; ++md) o[md] *= alpha;

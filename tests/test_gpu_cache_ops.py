@@ -682,3 +682,24 @@ def test_torch_operators():
     got = (out, lse, w, rows, counts, *ops.compact_rows(*move))
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('T', [2, 30, 70])
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+def test_scores_of_a_thousand_million_and_more(T, dtype):
+    """Scores whose products with the scale are rounded to steps of 64 to 2^24: two equal ones in different tiles share
+    the row, all others are nothing.  The LSE takes four roundings: of the scale and of ln 2, of the products with
+    them."""
+    from slimkv_amd import cache_ops
+    D, N, dt = 128, 300, TYPES[dtype]
+    q = torch.full((1, T, 2, D), 3001.0, dtype=dt, device='cuda')
+    k = torch.zeros(1, N, 2, D, dtype=dt, device='cuda')
+    k[:, 7], k[:, 100], k[:, 200] = 2999.0, -2999.0, 2999.0
+    v = torch.full((1, N, 2, D), 100.0, dtype=dt, device='cuda')
+    v[:, 7], v[:, 200] = 1.5, 4.5
+    nothing = torch.zeros(T, T, dtype=torch.bool, device='cuda')
+    for scale in (1.0, 1.7, 0.0931, 1e5):
+        out, lse = cache_ops.tree_attention(q, k[:, :T], v[:, :T], scale, k, v, mask=nothing)
+        assert (out == 3.0).all(), scale
+        s = D * float(q[0, 0, 0, 0]) * float(k[0, 7, 0, 0]) * scale
+        assert (lse.double() - s).abs().max() <= s * 2.0 ** -22 + 1.0, scale
