@@ -190,10 +190,22 @@ __device__ __forceinline__ float far_exponent(float s, float scale_log2, float b
     return __builtin_fabsf(base) >= kFarBase ? rounded_product(s, scale_log2) - base : __builtin_fmaf(s, scale_log2, -base);
 }
 
+// The base of a maximum, in log2.  fp16 weights against the maximum itself would be
+// subnormal from 2^-14 of it on and nothing from 2^-25, while their sum kept them:
+// 15 less, weights of up to 2^15 go down to 2^-39 of the largest in what the type
+// holds.  The sum and the output carry the same factor, and base + log2 of the sum
+// is the LSE for any base.  Maxima whose rounding could take a weight past the type
+// stay their own base.
+template <bool F16>
+__device__ __forceinline__ float base_of(float top) {
+    if constexpr (F16) return __builtin_fabsf(top) < kFarBase ? top - 15.f : top;
+    return top;
+}
+
 // One online-softmax step of a column's scores: the scores become weights, the
-// state moves to the new maximum.  The weights' sum is fp32 and of the
-// unrounded weights; a lane keeps the sum of its own keys.
-template <int MT, int MD>
+// state moves to the new base.  The weights' sum is fp32 and of the unrounded
+// weights; a lane keeps the sum of its own keys.
+template <int MT, int MD, bool F16>
 __device__ __forceinline__ void softmax_step(v4f (&s)[MT], float scale_log2, float& m, float& l, v4f (&o)[MD]) {
     float mx = kNegInf;
 #pragma unroll
@@ -201,7 +213,7 @@ __device__ __forceinline__ void softmax_step(v4f (&s)[MT], float scale_log2, flo
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][i]);
     mx = rows_max(mx);
-    const float m_new = fmaxf(m, rounded_product(mx, scale_log2));
+    const float m_new = fmaxf(m, base_of<F16>(rounded_product(mx, scale_log2)));
     const float base = m_new == kNegInf ? 0.f : m_new;
     const float alpha = fast_exp2(m - base);
     m = m_new;
@@ -588,7 +600,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[nt][0][i] = visible(nt, i) ? s[nt][0][i] : kNegInf;
-                softmax_step<1, MD>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
+                softmax_step<1, MD, F16>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
             }
 #pragma unroll
             for (int md = 0; md < MD; ++md) {
@@ -774,7 +786,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
         auto softmax = [&](v4f(&s)[NT][MT], u32x4(&pb)[MT / 2][NT]) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                softmax_step<MT, MD>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
+                softmax_step<MT, MD, F16>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
 #pragma unroll
                 for (int ss = 0; ss < MT / 2; ++ss)
                     pb[ss][nt] =

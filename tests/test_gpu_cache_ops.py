@@ -703,3 +703,33 @@ def test_scores_of_a_thousand_million_and_more(T, dtype):
         assert (out == 3.0).all(), scale
         s = D * float(q[0, 0, 0, 0]) * float(k[0, 7, 0, 0]) * scale
         assert (lse.double() - s).abs().max() <= s * 2.0 ** -22 + 1.0, scale
+
+
+@pytest.mark.parametrize('T', [1, 20, 40, 70])
+@pytest.mark.parametrize('ahead', [12.0, 17.5, 22.0])
+def test_fp16_rows_far_behind_the_first_keep_their_weight(T, ahead):
+    """One row `ahead` nats before thousands of equal ones whose values alone are not zero, every item in one run.
+    Weights are held 2^15 times as large as their share of the row's largest, so the half step 2^-25 of fp16's
+    subnormals is 2^-40 of it: 2^-40 max|v| a key, divided by the row's sum.  The output may be subnormal too."""
+    from slimkv_amd import cache_ops
+    B, H, D, N, g, dt = 64, 8, 128, 2003, gen(73), torch.float16
+    scale = D ** -0.5
+    q = torch.full((1, T, H, D), 2.0, dtype=dt, device='cuda')
+    k = torch.zeros(1, N, H, D, dtype=dt, device='cuda')
+    k[:, 0] = ahead / (2.0 * D * scale)
+    v = (500.0 + 50.0 * torch.randn(1, N, H, D, generator=g, device='cuda')).to(dt)
+    v[:, 0] = 0.0
+    dk, dv = torch.zeros(1, T, H, D, dtype=dt, device='cuda'), v[:, 1:T + 1].clone()
+    every = lambda x: x.expand(B, -1, -1, -1)
+    out, lse = cache_ops.tree_attention(every(q), every(dk), every(dv), scale, every(k), every(v))
+    eo, el, terms, top, mass, total = oc.tree_attention(f64(q), f64(k), f64(v), [N], f64(dk), f64(dv), None, scale)
+    d = 2.0 ** -24 * (D + 8) * mass + 2.0 ** -22 * (1 + top)
+    of_rows = lambda x: x.transpose(0, 2, 1)[..., None]
+    u = HALF[dt]
+    tol = (2 * of_rows(d) + u) * terms + u * np.abs(eo) * (1 + u) + 2.0 ** -25 + \
+        2.0 ** -40 * (N + T) * np.abs(f64(v)).max() / of_rows(total)
+    err = np.abs(f64(out) - eo)
+    print('expected', eo.min(), eo.max(), 'worst error over its bound', (err / tol).max(), flush=True)
+    assert (err <= tol).all()
+    tl = d + 2.0 ** -24 * ((N + T) / 4 + 64) + 2.0 ** -21 * (1 + np.abs(el))
+    assert (np.abs(lse.double().cpu().numpy() - el) <= tl).all()
