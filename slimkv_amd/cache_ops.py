@@ -20,12 +20,14 @@ and compact_rows bring it back.  Rows read through a block table follow torch's
 indexing rules: an entry outside the pool raises IndexError after the call (one
 host synchronisation), or is left in the caller's device int32 `status` word
 (graph capture, serving loops; kernels.check_status).  The operators have no
-gradients and raise ValueError where one would be recorded.
+gradients: they raise ValueError where one would be recorded or a forward-mode
+tangent lost, and for negative views, whose memory holds other values.
 """
 import struct
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
@@ -53,19 +55,25 @@ _pack_compact = _packer(_lib.CompactRowsArgs)
 
 
 def _common(name, *tensors):
-    """The device that holds every tensor; no gradient to record."""
-    index = tensors[0].get_device()
-    grad = torch.is_grad_enabled()
+    """The device that holds every tensor; no gradient to record, no tangent to carry, memory that holds the values."""
+    index = lowest = highest = tensors[0].get_device()
+    grad, dual = torch.is_grad_enabled(), forward_ad._current_level >= 0
     for t in tensors:
         if t is None:
             continue
-        at = t.get_device()
-        if at < 0:
-            raise ValueError(f'{name} needs device tensors (no CPU path)')
-        if at != index:
-            raise ValueError(f'{name}: tensors on devices {index} and {at}')
+        if t.is_neg():
+            raise ValueError(f'{name} reads memory as it is: resolve negative views (resolve_neg)')
+        if dual and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f'{name} carries no tangent: detach the inputs')
         if grad and t.requires_grad:
             raise ValueError(f'{name} records no gradient: detach the inputs or run it under torch.no_grad()')
+        at = t.get_device()
+        if at != index:
+            lowest, highest = min(lowest, at), max(highest, at)
+    if lowest < 0:
+        raise ValueError(f'{name} needs device tensors (no CPU path)')
+    if lowest != highest:
+        raise ValueError(f'{name}: tensors on devices {lowest} and {highest}')
     return tensors[0].device
 
 

@@ -261,3 +261,34 @@ def test_oracle_weights_and_rows_by_hand():
     assert rows.tolist() == [[[1, 2]]]
     rows, counts = oc.select_rows(np.array([[[0.0, 1, 1]]]), 4, [2], 1, 1)
     assert rows.tolist() == [[[0, 1, -1, -1]]] and counts.tolist() == [2]
+
+
+def operator_calls():
+    """Each operator with one of its tensors replaced: (name, argument, call of the replacement)."""
+    lse, line = z(2, 8, 3, dtype=torch.float32), z(2, 2, 9, dtype=torch.float32)
+    rows = (z(2, 3, 8, 64), z(2, 3, 2, 64), z(2, 9, 2, 64))
+    calls = [('tree', x, rows[i], lambda t, x=x: tree(**{x: t})) for x, i in
+             (('q', 0), ('draft_k', 1), ('draft_v', 1), ('k', 2), ('v', 2), ('out', 0))]
+    calls += [('tree', 'lse', lse, lambda t: tree(lse=t)),
+              ('tree', 'pages', PAGED['pages'], lambda t: tree(**dict(PAGED, pages=t)))]
+    calls += [('weights', x, t0, lambda t, x=x: weights(**{x: t})) for x, t0 in
+              (('q', rows[0]), ('lse', lse), ('k', rows[2]), ('previous', line), ('out', line))]
+    from slimkv_amd import cache_ops
+    calls += [('select', 'weights', line, lambda t: cache_ops.select_rows(t, 4))]
+    calls += [('compact', x, t0, lambda t, x=x: compact(**{x: t})) for x, t0 in
+              (('k', rows[2]), ('v', rows[2]), ('weights', line), ('out_k', z(2, 4, 2, 64)), ('out_v', z(2, 4, 2, 64)))]
+    return calls
+
+
+@pytest.mark.parametrize('call', operator_calls(), ids=lambda c: f'{c[0]}-{c[1]}')
+def test_tangents_and_negative_views_are_refused(call):
+    _, _, t, run = call
+    with pytest.raises(ValueError, match='negative'):
+        run(torch._neg_view(t))
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(ValueError, match='tangent'):
+            run(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+        with torch.no_grad(), pytest.raises(ValueError, match='tangent'):
+            run(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(ValueError, match='device tensors'):
+            run(t)
