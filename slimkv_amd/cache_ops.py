@@ -101,15 +101,49 @@ def _rows16(t):
 
 def _span(t):
     """First and last byte address of t's elements."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + last * t.element_size() + t.element_size()
+    size = t.element_size()
+    last = t.numel() - 1 if t.is_contiguous() else sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    start = t.data_ptr()
+    return start, start + last * size + size
+
+
+def _reaches(target, terms, budget):
+    """Whether 0 <= x_i <= n_i give sum x_i s_i = target, for terms (s_i, n_i) with s_i falling; true as well where that
+    takes more than budget[0] steps to find out."""
+    if not terms:
+        return target == 0
+    (step, most), rest = terms[0], terms[1:]
+    reach = sum(s * n for s, n in rest)
+    for x in range(max(0, -((reach - target) // step)), min(most, target // step) + 1):
+        budget[0] -= 1
+        if budget[0] < 0 or _reaches(target - x * step, rest, budget):
+            return True
+    return False
 
 
 def _overlap(a, b):
+    """Whether a byte belongs to elements of both a and b (views may lie interleaved and apart: the halves of one
+    tensor): an element of a at a0 + x and one of b at b0 + y share one if the distance b0 - a0 is a sum of steps of
+    both."""
     if a.numel() == 0 or b.numel() == 0:
         return False
     (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+    if a1 <= b0 or b1 <= a0:
+        return False
+    steps = {1: a.element_size() + b.element_size() - 2}
+    for t in (a, b):
+        for n, s in zip(t.shape, t.stride()):
+            if s and n > 1:
+                s *= t.element_size()
+                steps[s] = steps.get(s, 0) + n - 1
+    terms = []
+    for s, n in sorted(steps.items()):
+        if terms and s % terms[-1][0] == 0 and s // terms[-1][0] <= terms[-1][1] + 1:
+            terms[-1] = (terms[-1][0], terms[-1][1] + s // terms[-1][0] * n)      # the steps below reach up to this one
+        elif n:
+            terms.append((s, n))
+    # y counted down from b's last byte, so that all steps add up
+    return _reaches(b1 - 1 - a0, terms[::-1], [1000])
 
 
 def _expanded(t):

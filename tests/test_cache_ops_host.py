@@ -292,3 +292,38 @@ def test_tangents_and_negative_views_are_refused(call):
             run(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
         with pytest.raises(ValueError, match='device tensors'):
             run(t)
+
+
+def test_overlap_is_that_of_the_elements():
+    """Random views of one buffer, interleaved, nested and expanded ones among them, against the bytes they name."""
+    import random
+    from slimkv_amd.cache_ops import _overlap
+    rng, seen = random.Random(5), [0, 0]
+    room = torch.zeros(128, dtype=torch.float32)
+    for _ in range(4000):
+        views, named = [], []
+        for dtype in rng.choices((torch.float32, torch.bfloat16), k=2):
+            shape = [rng.randint(1, 4) for _ in range(rng.randint(1, 3))]
+            step = [rng.choice((0, 1, 2, 3, 4, 6, 8, 12)) for _ in shape]
+            at, size = rng.randint(0, 20), dtype.itemsize
+            views.append(torch.as_strided(room.view(dtype), shape, step, at))
+            named.append({(at + sum(i * s for i, s in zip(index, step))) * size + byte
+                          for index in np.ndindex(*shape) for byte in range(size)})
+        meets = bool(named[0] & named[1])
+        assert _overlap(*views) == meets, [(x.dtype, x.shape, x.stride(), x.storage_offset()) for x in views]
+        seen[meets] += 1
+    assert min(seen) > 500
+
+
+def test_interleaved_views_are_taken():
+    """K and V, or q and the output, as halves of one tensor: refused for nothing but the device."""
+    both, qo = z(2, 4, 2, 2, 64), z(2, 3, 8, 2, 64)
+    with pytest.raises(ValueError, match='device tensors'):
+        compact(out_k=both[:, :, 0], out_v=both[:, :, 1])
+    with pytest.raises(ValueError, match='device tensors'):
+        tree(q=qo[:, :, :, 0], out=qo[:, :, :, 1])
+    with pytest.raises(ValueError, match='apart'):
+        tree(q=qo[:, :, :, 0], out=qo.view(2, 3, 8, 128)[..., 32:96])
+    wide = z(2, 2, 2, 9, dtype=torch.float32)
+    with pytest.raises(ValueError, match='device tensors'):
+        weights(previous=wide[:, :, 0], out=wide[:, :, 1])

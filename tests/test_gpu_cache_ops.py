@@ -733,3 +733,25 @@ def test_fp16_rows_far_behind_the_first_keep_their_weight(T, ahead):
     assert (err <= tol).all()
     tl = d + 2.0 ** -24 * ((N + T) / 4 + 64) + 2.0 ** -21 * (1 + np.abs(el))
     assert (np.abs(lse.double().cpu().numpy() - el) <= tl).all()
+
+
+def test_outputs_interleaved_with_other_tensors():
+    """The output beside q, the moved K and V as halves of one tensor, the sums beside what they are added to."""
+    from slimkv_amd import cache_ops
+    B, T, Hq, H, D, N, keep, g = 2, 3, 8, 2, 64, 40, 16, gen(75)
+    k, v, _ = make_cache(g, B, N, H, D, 0, torch.bfloat16)
+    both, sums = randn(g, B, T, Hq, 2, D), torch.rand(B, H, 2, N, generator=g, device='cuda')
+    dk, dv = randn(g, B, T, H, D), randn(g, B, T, H, D)
+    q, before = both[:, :, :, 0], both.clone()
+    want, lse = cache_ops.tree_attention(q.contiguous(), dk, dv, 0.125, k, v)
+    got, _ = cache_ops.tree_attention(q, dk, dv, 0.125, k, v, out=both[:, :, :, 1])
+    assert torch.equal(got, want) and torch.equal(q, before[:, :, :, 0])
+    kept = sums[:, :, 0].clone()
+    want = cache_ops.attention_weights(q, lse, 0.125, k, previous=kept, causal=False)
+    w = cache_ops.attention_weights(q, lse, 0.125, k, previous=sums[:, :, 0], out=sums[:, :, 1], causal=False)
+    assert torch.equal(w, want) and torch.equal(sums[:, :, 0], kept)
+    rows, counts = cache_ops.select_rows(w, keep)
+    halves = torch.empty(B, keep, 2, H, D, dtype=torch.bfloat16, device='cuda')
+    want = cache_ops.compact_rows(rows, counts, k, v)
+    cache_ops.compact_rows(rows, counts, k, v, out_k=halves[:, :, 0], out_v=halves[:, :, 1])
+    assert torch.equal(halves[:, :, 0], want[0]) and torch.equal(halves[:, :, 1], want[1])
