@@ -437,12 +437,11 @@ def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weight
                 raise ValueError(f'{name}: in place the cache must not be an expanded view')
         if k is not None and k.numel() and k.data_ptr() == v.data_ptr():
             raise ValueError(f'{name}: in place k and v must be two tensors')
-    sources = [t for t in (k, v, pages) if t is not None]
     for t in (out_k, out_v):
         if t is not None and (t.shape != (B, keep, H, D) or t.stride(3) != 1 or _expanded(t) or
-                              any(_overlap(t, s) for s in sources)):
+                              any(s is not None and _overlap(t, s) for s in (k, v, pages, table, rows, counts, weights))):
             raise ValueError(f'{name}: outputs must be [{B}, {keep}, {H}, {D}] with contiguous features, no expanded '
-                             'views and apart from the cache')
+                             'views and apart from the cache and the other inputs')
     if out_k is not None and out_v is not None and _overlap(out_k, out_v):
         raise ValueError(f'{name}: out_k and out_v must lie apart')
     device = _common(name, rows, counts, k, v, pages, table, weights, out_k, out_v)

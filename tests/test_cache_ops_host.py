@@ -327,3 +327,19 @@ def test_interleaved_views_are_taken():
     wide = z(2, 2, 2, 9, dtype=torch.float32)
     with pytest.raises(ValueError, match='device tensors'):
         weights(previous=wide[:, :, 0], out=wide[:, :, 1])
+
+
+moved = z(4 * 2 * 4 * 2 * 64)
+
+
+@pytest.mark.parametrize('out', ['out_k', 'out_v'])
+@pytest.mark.parametrize('over', [
+    dict(rows=moved.view(torch.int32)[:16].view(2, 2, 4)),
+    dict(counts=moved.view(torch.int32)[500:502]),
+    dict(weights=moved.view(torch.float32)[100:136].view(2, 2, 9)),
+    dict(PAGED, table=moved.view(torch.int64)[:6].view(2, 3)),
+    dict(k=moved[1000:3304].view(2, 9, 2, 64)),
+], ids=['rows', 'counts', 'weights', 'table', 'k'])
+def test_compact_rows_refuses_outputs_over_its_inputs(out, over):
+    with pytest.raises(ValueError, match='apart from the cache and the other inputs'):
+        compact(**over, **{out: moved[:1024].view(2, 4, 2, 64)})
