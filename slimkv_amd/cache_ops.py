@@ -146,8 +146,17 @@ def _overlap(a, b):
     return _reaches(b1 - 1 - a0, terms[::-1], [1000])
 
 
-def _expanded(t):
-    return any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))
+def _folded(t):
+    """Whether elements of t share memory (expanded views), or its steps do not show that none do: each past all that
+    the smaller ones reach."""
+    if t.numel() < 2 or t.is_contiguous():
+        return False
+    reach = 0
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s <= reach:
+            return True
+        reach += s * (n - 1)
+    return False
 
 
 def _lengths(name, lengths, batch):
@@ -302,7 +311,7 @@ def tree_attention(q, draft_k, draft_v, scale, k=None, v=None, *, pages=None, ta
             mask = mask.contiguous()
         m = (mask.data_ptr(), mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
     inputs = (q, draft_k, draft_v, k, v, pages, table, lengths, mask)
-    if out is not None and (out.shape != q.shape or out.stride(3) != 1 or _expanded(out) or
+    if out is not None and (out.shape != q.shape or out.stride(3) != 1 or _folded(out) or
                             any(t is not None and _overlap(out, t) for t in inputs)):
         raise ValueError(f'{name}: out must have the shape of q with contiguous features, no expanded view and apart '
                          'from the inputs')
@@ -355,7 +364,7 @@ def attention_weights(q, lse, scale, k=None, *, pages=None, table=None, lengths=
     if out is not None and previous is not None and _overlap(out, previous) and \
             (out.data_ptr() != previous.data_ptr() or out.stride() != previous.stride()):
         raise ValueError(f'{name}: out must be previous itself or lie apart from it')
-    if out is not None and (_expanded(out) or any(t is not None and _overlap(out, t)
+    if out is not None and (_folded(out) or any(t is not None and _overlap(out, t)
                                                   for t in (lse, q, k, pages, table, lengths))):
         raise ValueError(f'{name}: out must not be an expanded view and lie apart from lse and the other inputs')
     device = _common(name, q, lse, k, pages, table, lengths, previous, out)
@@ -433,12 +442,12 @@ def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weight
         if out_k is not None or out_v is not None:
             raise ValueError(f'{name}: in place there are no outputs')
         for t in (k, v, pages, weights):
-            if t is not None and _expanded(t):
-                raise ValueError(f'{name}: in place the cache must not be an expanded view')
+            if t is not None and _folded(t):
+                raise ValueError(f'{name}: in place the cache and the weights must not be expanded or overlapping views')
         if k is not None and k.numel() and k.data_ptr() == v.data_ptr():
             raise ValueError(f'{name}: in place k and v must be two tensors')
     for t in (out_k, out_v):
-        if t is not None and (t.shape != (B, keep, H, D) or t.stride(3) != 1 or _expanded(t) or
+        if t is not None and (t.shape != (B, keep, H, D) or t.stride(3) != 1 or _folded(t) or
                               any(s is not None and _overlap(t, s) for s in (k, v, pages, table, rows, counts, weights))):
             raise ValueError(f'{name}: outputs must be [{B}, {keep}, {H}, {D}] with contiguous features, no expanded '
                              'views and apart from the cache and the other inputs')

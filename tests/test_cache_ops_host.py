@@ -343,3 +343,40 @@ moved = z(4 * 2 * 4 * 2 * 64)
 def test_compact_rows_refuses_outputs_over_its_inputs(out, over):
     with pytest.raises(ValueError, match='apart from the cache and the other inputs'):
         compact(**over, **{out: moved[:1024].view(2, 4, 2, 64)})
+
+
+def test_views_that_overlap_themselves():
+    """Never taken for plain where two indices name one element; ordinary, permuted, sliced and empty views pass."""
+    from slimkv_amd.cache_ops import _folded
+    import random
+    rng, room, seen = random.Random(6), torch.zeros(128), 0
+    for _ in range(3000):
+        shape = [rng.randint(1, 4) for _ in range(rng.randint(1, 3))]
+        step = [rng.choice((0, 1, 2, 3, 4, 6, 8, 12)) for _ in shape]
+        t = torch.as_strided(room, shape, step)
+        named = [sum(i * s for i, s in zip(index, step)) for index in np.ndindex(*shape)]
+        if len(set(named)) < len(named):
+            assert _folded(t), (shape, step)
+            seen += 1
+    assert seen > 500
+    for t in (z(2, 3, 4), z(2, 3, 4).transpose(0, 2), z(2, 6, 8)[:, ::2, :4], z(2, 3, 4)[:, :0], z(4, 2, 8, 64)[:, 0],
+              z(1, 3, 4).as_strided((1, 3, 4), (0, 4, 1)), torch.zeros(())):
+        assert not _folded(t)
+
+
+windows = dict(size=(2, 4, 2, 64), stride=(512, 64, 64, 1))          # row 1 of head 0 is row 0 of head 1
+
+
+@pytest.mark.parametrize('run', [
+    lambda: tree(out=z(4000).as_strided((2, 3, 8, 64), (1536, 64, 64, 1))),
+    lambda: weights(out=z(100, dtype=torch.float32).as_strided((2, 2, 9), (18, 8, 1))),
+    lambda: compact(out_k=z(4000).as_strided(**windows)),
+    lambda: compact(out_v=z(4000).as_strided(**windows)),
+    lambda: compact(in_place=True, k=z(4000).as_strided((2, 9, 2, 64), (1152, 64, 64, 1))),
+    lambda: compact(in_place=True, v=z(4000).as_strided((2, 9, 2, 64), (1152, 64, 64, 1))),
+    lambda: compact(in_place=True, weights=z(100, dtype=torch.float32).as_strided((2, 2, 9), (18, 8, 1))),
+    lambda: compact(**dict(PAGED, pages=z(9000).as_strided((6, 4, 2, 2, 64), (512, 128, 64, 64, 1))), in_place=True),
+])
+def test_tensors_written_that_overlap_themselves_are_refused(run):
+    with pytest.raises(ValueError, match='expanded'):
+        run()
