@@ -125,7 +125,10 @@ int slimkv_select_rows(const slimkv_select_rows_args* a, void* workspace, size_t
  *  in_place 0: into out_k / out_v [B, keep, Hkv, D]; rows from counts[b] on are
  *    zero.  Rows may repeat and come in any order.
  *  in_place 1: within the cache (dense or pages, out_k / out_v unused); each
- *    choice strictly ascending, rows from counts[b] on stay as they are.
+ *    choice strictly ascending, rows from counts[b] on stay as they are.  K and
+ *    V of every sequence and head, and the weights, lie apart; no two sequences
+ *    share a page that one of them writes.  Strides of 0 over sequences or heads
+ *    (t_sb among them), and k = v, are refused.
  * weights (optional) [B, weight_heads, weight_keys] fp32 move along into
  * out_weights [B, weight_heads, keep], zero from counts[b] on; in place within
  * weights, whose entries from counts[b] on become zero.  weight_heads is the

@@ -146,6 +146,14 @@ def _overlap(a, b):
     return _reaches(b1 - 1 - a0, terms[::-1], [1000])
 
 
+def _apart(written, read):
+    """Whether no tensor written shares memory with another one (None: not there)."""
+    written = [(*_span(t), t) for t in written if t is not None and t.numel()]
+    spans = written + [(*_span(t), t) for t in read if t is not None and t.numel()]
+    return not any(a0 < b1 and b0 < a1 and _overlap(a, b)
+                   for i, (a0, a1, a) in enumerate(written) for b0, b1, b in spans[i + 1:])
+
+
 def _folded(t):
     """Whether elements of t share memory (expanded views), or its steps do not show that none do: each past all that
     the smaller ones reach."""
@@ -421,7 +429,8 @@ def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weight
     None for pages).  weights [B, rows' head count, N] fp32 move along.  A row
     outside the cache (in place: or out of order) moves nothing and raises
     IndexError after the call, or is left in `status`.  In place, no other
-    sequence's table may name the pages a sequence writes."""
+    sequence's table may name the pages a sequence writes (an expanded table
+    is refused), and k, v, weights and the index tensors share no memory."""
     name = 'compact_rows'
     if rows.dim() != 3 or rows.dtype is not torch.int32 or counts.dtype is not torch.int32 or \
             counts.shape != rows.shape[:1]:
@@ -444,8 +453,11 @@ def compact_rows(rows, counts, k=None, v=None, *, pages=None, table=None, weight
         for t in (k, v, pages, weights):
             if t is not None and _folded(t):
                 raise ValueError(f'{name}: in place the cache and the weights must not be expanded or overlapping views')
-        if k is not None and k.numel() and k.data_ptr() == v.data_ptr():
-            raise ValueError(f'{name}: in place k and v must be two tensors')
+        if not _apart((k, v, pages, weights), (rows, counts, table)):
+            raise ValueError(f'{name}: in place k and v must be two tensors, and they, the weights and the index tensors '
+                             'must share no memory')
+        if table is not None and _folded(table):
+            raise ValueError(f'{name}: in place each table entry names pages of its own: no expanded or overlapping table')
     for t in (out_k, out_v):
         if t is not None and (t.shape != (B, keep, H, D) or t.stride(3) != 1 or _folded(t) or
                               any(s is not None and _overlap(t, s) for s in (k, v, pages, table, rows, counts, weights))):

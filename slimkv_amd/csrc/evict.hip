@@ -727,6 +727,14 @@ extern "C" int slimkv_compact_rows(const slimkv_compact_rows_args* a, void* stre
     CompactParams p{};
     const int view = cache_view(a->cache, a->batch, a->kv_heads, a->head_dim, true, "compact rows", &p.c);
     if (view != SLIMKV_OK) return view;
+    if (a->in_place && a->cache.keys > 0) {
+        const slimkv_cache_rows& c = a->cache;
+        const bool many = a->batch > 1, pages = c.table != nullptr;
+        if (c.k == c.v || (many && (pages ? c.t_sb == 0 : c.k_sb == 0 || c.v_sb == 0)) ||
+            (a->kv_heads > 1 && (c.k_sh == 0 || c.v_sh == 0)) || (a->weight_heads > 1 && a->weight_keys > 0 && a->w_sh == 0) ||
+            (many && a->weight_heads && a->weight_keys > 0 && a->w_sb == 0))
+            return fail(SLIMKV_EINVAL, "compact rows: in place every sequence and head needs rows of its own");
+    }
     if (!a->in_place && (!rows_aligned(a->out_k, {{a->batch, a->ok_sb}, {a->keep, a->ok_sn}, {a->kv_heads, a->ok_sh}}) ||
                          !rows_aligned(a->out_v, {{a->batch, a->ov_sb}, {a->keep, a->ov_sn}, {a->kv_heads, a->ov_sh}})))
         return fail(SLIMKV_EINVAL, "compact rows: output rows must start on 16-byte boundaries");

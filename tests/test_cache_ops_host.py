@@ -380,3 +380,43 @@ windows = dict(size=(2, 4, 2, 64), stride=(512, 64, 64, 1))          # row 1 of 
 def test_tensors_written_that_overlap_themselves_are_refused(run):
     with pytest.raises(ValueError, match='expanded'):
         run()
+
+
+def test_in_place_refuses_what_shares_memory():
+    """Sequences on the same pages; K and V, weights or index tensors in each other's memory.  The halves of one tensor
+    are apart."""
+    room = z(6000)
+    f, i = room.view(torch.float32), room.view(torch.int32)
+    k = room[:2304].view(2, 9, 2, 64)
+    for over, match in (
+            (dict(PAGED, table=z(1, 3, dtype=torch.int64).expand(2, 3)), 'table'),
+            (dict(PAGED, table=z(2, 1, dtype=torch.int64).expand(2, 3)), 'table'),
+            (dict(PAGED, table=z(9, dtype=torch.int64).as_strided((2, 3), (2, 1))), 'table'),
+            (dict(k=k, v=room[128:2432].view(2, 9, 2, 64)), 'two tensors'),
+            (dict(k=k, weights=f[1000:1036].view(2, 2, 9)), 'share no memory'),
+            (dict(k=k, rows=i[1000:1016].view(2, 2, 4)), 'share no memory'),
+            (dict(v=k, counts=i[1151:1153]), 'share no memory'),
+            (dict(PAGED, pages=room[:3072].view(6, 4, 1, 2, 64).as_strided((3, 4, 2, 2, 64), (1024, 256, 128, 64, 1)),
+                  table=room.view(torch.int64)[700:706].view(2, 3)), 'share no memory'),
+            (dict(rows=i[:16].view(2, 2, 4), weights=f[8:44].view(2, 2, 9)), 'share no memory')):
+        with pytest.raises(ValueError, match=match):
+            compact(in_place=True, **over)
+    both = z(2, 9, 2, 2, 64)
+    for over in (dict(k=both[:, :, 0], v=both[:, :, 1]), dict(k=both[..., 0, :], v=both[..., 1, :]), PAGED,
+                 dict(k=k, v=room[2304:4608].view(2, 9, 2, 64), weights=f[2304:2340].view(2, 2, 9))):
+        with pytest.raises(ValueError, match='device tensors'):
+            compact(in_place=True, **over)
+
+
+def test_the_c_entry_refuses_shared_rows_in_place():
+    from slimkv_amd import _lib
+    sound = dict(k=4096, v=8192, k_sb=1152, k_sn=128, k_sh=64, v_sb=1152, v_sn=128, v_sh=64, keys=9)
+    paged = dict(sound, table=4096, t_sb=3, t_cols=3, num_blocks=6, block_size=3)
+    for cache, over in ((dict(sound, k_sb=0), {}), (dict(sound, v_sh=0), {}), (dict(sound, v=4096), {}),
+                        (dict(paged, t_sb=0), {}), (sound, dict(w_sb=0)), (sound, dict(w_sh=0))):
+        a = dict(rows=4096, r_sb=8, r_sh=4, counts=4096, weights=4096, w_sb=18, w_sh=9, weight_heads=2, weight_keys=9, batch=2,
+                 kv_heads=2, head_dim=64, keep=4, in_place=1)
+        a.update(over)
+        call = _lib.CompactRowsArgs(cache=_lib.CacheRows(**cache), **a)
+        assert _lib.lib().slimkv_compact_rows(ctypes.byref(call), None) == -1, (cache, over)
+        assert b'of its own' in _lib.lib().slimkv_last_error()
