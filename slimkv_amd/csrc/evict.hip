@@ -662,10 +662,11 @@ namespace {
 
 int check_select(const slimkv_select_rows_args* a) {
     if (!a) return fail(SLIMKV_EINVAL, "select rows: null pointer");
-    if (a->batch < 0 || a->heads <= 0 || a->keys < 0 || a->keys > ((int64_t)1 << 30) || a->keep <= 0 ||
-        a->keep > ((int64_t)1 << 30) || a->sink < 0 || a->recent < 0 || a->batch * a->heads > 0x7fffffff || a->batch > 0x7fffffff)
+    if (a->batch < 0 || a->batch > 0x7fffffff || a->heads <= 0 || a->heads > 0x7fffffff || a->batch * a->heads > 0x7fffffff ||
+        a->keys < 0 || a->keys > ((int64_t)1 << 30) || a->keep <= 0 || a->keep > ((int64_t)1 << 30) || a->sink < 0 ||
+        a->recent < 0)
         return fail(SLIMKV_EINVAL, "select rows: invalid sizes");
-    if (a->sink + a->recent > a->keep)
+    if (a->sink > a->keep || a->recent > a->keep - a->sink)
         return fail(SLIMKV_EINVAL, "select rows: the first and the recent rows exceed the rows kept");
     return SLIMKV_OK;
 }

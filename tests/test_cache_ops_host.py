@@ -420,3 +420,12 @@ def test_the_c_entry_refuses_shared_rows_in_place():
         call = _lib.CompactRowsArgs(cache=_lib.CacheRows(**cache), **a)
         assert _lib.lib().slimkv_compact_rows(ctypes.byref(call), None) == -1, (cache, over)
         assert b'of its own' in _lib.lib().slimkv_last_error()
+
+
+@pytest.mark.parametrize('over', [dict(sink=2 ** 62, recent=2 ** 62), dict(sink=2 ** 63 - 1, recent=1), dict(batch=2, heads=2 ** 63 - 1),
+                                  dict(batch=2 ** 32, heads=2 ** 32)])
+def test_row_selection_sizes_whose_sum_or_product_wraps(over):
+    from slimkv_amd import _lib
+    a = _lib.SelectRowsArgs(**{**dict(batch=1, heads=1, keys=10, keep=4), **over})
+    assert _lib.lib().slimkv_select_rows_workspace(ctypes.byref(a)) == 0
+    assert b'select rows' in _lib.lib().slimkv_last_error()
