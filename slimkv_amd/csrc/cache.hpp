@@ -73,6 +73,9 @@ __device__ __forceinline__ int quotient(int n, const FastDiv& f) { return (int)(
 // A softmax scale whose fp32 image times a score of -inf stays -inf.
 inline bool scale_usable(double scale) { return scale >= 1e-18 && scale <= 1e18; }
 
+// A grid dimension's threads are counted in 32 bits by the launch.
+inline bool launchable(int64_t workgroups, int64_t threads) { return workgroups <= 0xffffffff / threads; }
+
 struct CacheView {
     const uint16_t* k; int64_t k_sb, k_sn, k_sh;
     const uint16_t* v; int64_t v_sb, v_sn, v_sh;

@@ -691,7 +691,10 @@ extern "C" int slimkv_select_rows(const slimkv_select_rows_args* a, void* worksp
     p.ws = static_cast<uint32_t*>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const unsigned rows = (unsigned)(a->batch * a->heads);
-    if (a->keys <= kMostHeld * kHeldThreads) {
+    const bool held = a->keys <= kMostHeld * kHeldThreads;
+    if (!launchable(rows, held ? kHeldThreads : kSelectThreads))
+        return fail(SLIMKV_EINVAL, "select rows: too many rows for one call");
+    if (held) {
         void (*kernel)(SelectParams) = a->keys <= 4 * kHeldThreads    ? select_held_kernel<4>
                                        : a->keys <= 8 * kHeldThreads  ? select_held_kernel<8>
                                        : a->keys <= 16 * kHeldThreads ? select_held_kernel<16>
@@ -757,7 +760,8 @@ extern "C" int slimkv_compact_rows(const slimkv_compact_rows_args* a, void* stre
         move = (a->keep * a->kv_heads + per - 1) / per;
         weights = (a->weight_heads * a->keep + 255) / 256;
     }
-    if (move + weights > 0x7fffffff) return fail(SLIMKV_EINVAL, "compact rows: too many rows for one call");
+    if (!launchable(move + weights, a->in_place ? kMoveThreads : 256))
+        return fail(SLIMKV_EINVAL, "compact rows: too many rows for one call");
     p.move_blocks = (int)move;
     p.weight_blocks = (int)weights;
     const dim3 grid((unsigned)(move + weights), (unsigned)a->batch);

@@ -1032,6 +1032,19 @@ auto tree_kernel(const TreePlan& plan) -> void (*)(TreeParams) {
     return plan.nt == 2 ? tree_few_kernel<D, F16, 2, PAGED> : tree_few_kernel<D, F16, 1, PAGED>;
 }
 
+// The merge's workgroups.  Runs an item has at most, on average: every group of
+// lanes its own row where they are few, all groups one row where they are many.
+struct MergePlan {
+    bool shared;
+    int chunks;                    // workgroups an item
+};
+
+MergePlan plan_merge(const TreePlan& plan, int64_t items, int64_t M, int64_t D) {
+    const bool shared = plan.runs / items >= 8;
+    const int64_t rows = shared ? 1 : 256 / (D / 4);
+    return MergePlan{shared, (int)((M + rows - 1) / rows)};
+}
+
 template <int D, bool F16>
 void launch_tree(const TreeParams& p, const TreePlan& plan, hipStream_t st) {
     const dim3 grid((unsigned)((plan.slots + kXcdCount - 1) / kXcdCount * kXcdCount));
@@ -1040,14 +1053,13 @@ void launch_tree(const TreeParams& p, const TreePlan& plan, hipStream_t st) {
     else if (p.c.block.d % 16 == 0) kernel = tree_kernel<D, F16, kBlocks16>(plan);
     else kernel = tree_kernel<D, F16, kAnyBlocks>(plan);
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p);
-    // runs an item has at most, on average: every group of lanes its own row
-    // where they are few, all groups one row where they are many
-    const int64_t share = (int64_t)plan.runs / (p.B * p.Hk);
+    const MergePlan merge = plan_merge(plan, (int64_t)p.B * p.Hk, p.M, D);
+    const dim3 merge_grid((unsigned)(p.B * p.Hk * merge.chunks));
     constexpr int kGroups = 256 / (D / 4);
-    const int rows = share >= 8 ? 1 : kGroups, chunks = (p.M + rows - 1) / rows;
-    const dim3 merge_grid((unsigned)(p.B * p.Hk * chunks));
-    if (share >= 8) hipLaunchKernelGGL((tree_merge_kernel<D, F16, kGroups>), merge_grid, dim3(256), 0, st, p, plan.rows(), chunks);
-    else hipLaunchKernelGGL((tree_merge_kernel<D, F16, 1>), merge_grid, dim3(256), 0, st, p, plan.rows(), chunks);
+    if (merge.shared)
+        hipLaunchKernelGGL((tree_merge_kernel<D, F16, kGroups>), merge_grid, dim3(256), 0, st, p, plan.rows(), merge.chunks);
+    else
+        hipLaunchKernelGGL((tree_merge_kernel<D, F16, 1>), merge_grid, dim3(256), 0, st, p, plan.rows(), merge.chunks);
 }
 
 }  // namespace
@@ -1127,7 +1139,8 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     p.deal = Dealing{p.B, p.Hk, kKeys, (p.T + kKeys - 1) / kKeys, plan.runs};
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.part = static_cast<float*>(workspace);
-    if (B * Hk * p.M > 0x7fffffff || B * Hk * ((a->cache.keys + T) / kKeys + 2) > 0x7fffffff)
+    if (B * Hk * p.M > 0x7fffffff || !launchable(B * Hk * plan_merge(plan, B * Hk, p.M, a->head_dim).chunks, 256) ||
+        B * Hk * ((a->cache.keys + T) / kKeys + 2) > 0x7fffffff)
         return fail(SLIMKV_EINVAL, "tree attention: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->head_dim == 128) {

@@ -438,7 +438,7 @@ extern "C" int slimkv_attention_weights(const slimkv_attention_weights_args* a, 
     if (p.splits > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
                          workspace_bytes < slimkv_attention_weights_workspace(a)))
         return fail(SLIMKV_EWORKSPACE, "attention weights: workspace missing, misaligned or too small");
-    if ((int64_t)p.B * p.Hk * p.blocks > 0x7fffffff) return fail(SLIMKV_EINVAL, "attention weights: too many rows for one call");
+    if (!launchable((int64_t)p.B * p.Hk * p.blocks, 256)) return fail(SLIMKV_EINVAL, "attention weights: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->head_dim == 128) {
         if (a->dtype == SLIMKV_DTYPE_F16) launch_weights<128, true>(p, plan.few, st);

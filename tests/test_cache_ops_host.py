@@ -429,3 +429,28 @@ def test_row_selection_sizes_whose_sum_or_product_wraps(over):
     a = _lib.SelectRowsArgs(**{**dict(batch=1, heads=1, keys=10, keep=4), **over})
     assert _lib.lib().slimkv_select_rows_workspace(ctypes.byref(a)) == 0
     assert b'select rows' in _lib.lib().slimkv_last_error()
+
+
+def test_calls_past_what_one_launch_holds_are_refused():
+    """Threads of a grid dimension are counted in 32 bits: refused before anything is launched."""
+    from slimkv_amd import _lib
+    lib, ref = _lib.lib(), ctypes.byref
+    rows = dict(k=4096, v=8192, k_sb=0, k_sn=128, k_sh=64, v_sb=0, v_sn=128, v_sh=64)
+    tree = _lib.TreeAttentionArgs(cache=_lib.CacheRows(**rows, keys=9), q=4096, draft_k=4096, draft_v=4096, out=4096, batch=4096,
+                                  drafted=1024, heads=64, kv_heads=8, head_dim=128, scale=1.0, dk_sn=1024, dv_sn=1024, dk_sh=128,
+                                  dv_sh=128)
+    for s in ('q_sb', 'q_sl', 'q_sh', 'o_sb', 'o_sl', 'o_sh', 'dk_sb', 'dv_sb'):
+        setattr(tree, s, 128)
+    tree.cache.k_sn = tree.cache.v_sn = 1024
+    weights = _lib.AttentionWeightsArgs(cache=_lib.CacheRows(**rows, keys=33 * 128), q=4096, lse=4096, out=4096, batch=65535,
+                                        queries=1, heads=8, kv_heads=8, head_dim=64, scale=1.0)
+    select = _lib.SelectRowsArgs(weights=4096, rows=4096, counts=4096, batch=1 << 22, heads=1, keys=10, keep=4)
+    long_select = _lib.SelectRowsArgs(weights=4096, rows=4096, counts=4096, batch=1 << 23, heads=1, keys=1 << 16, keep=4)
+    compact = _lib.CompactRowsArgs(cache=_lib.CacheRows(**rows, keys=9), rows=4096, counts=4096, out_k=4096, out_v=4096, batch=1,
+                                   kv_heads=16, head_dim=64, keep=1 << 25)
+    for code in (lib.slimkv_tree_attention(ref(tree), 4096, 1 << 40, None),
+                 lib.slimkv_attention_weights(ref(weights), None, 0, None),
+                 lib.slimkv_select_rows(ref(select), None, 0, None), lib.slimkv_select_rows(ref(long_select), None, 0, None),
+                 lib.slimkv_compact_rows(ref(compact), None)):
+        assert code == -1, lib.slimkv_last_error()
+        assert b'too many rows' in lib.slimkv_last_error()
