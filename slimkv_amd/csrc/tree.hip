@@ -997,7 +997,8 @@ struct TreePlan {
     int rw, nt, row_blocks, runs;
     int64_t slots;
     int rows() const { return 16 * rw * nt; }
-    size_t bytes(int64_t D) const { return (size_t)slots * 2 * rows() * (D + 2) * sizeof(float); }
+    bool whole() const { return runs == 1; }      // no item lies in two runs: nothing to merge
+    size_t bytes(int64_t D) const { return whole() ? 0 : (size_t)slots * 2 * rows() * (D + 2) * sizeof(float); }
 };
 
 // Query rows a workgroup holds: the fewest of 16, 32, 64 and 128 that hold all
@@ -1053,6 +1054,7 @@ void launch_tree(const TreeParams& p, const TreePlan& plan, hipStream_t st) {
     else if (p.c.block.d % 16 == 0) kernel = tree_kernel<D, F16, kBlocks16>(plan);
     else kernel = tree_kernel<D, F16, kAnyBlocks>(plan);
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p);
+    if (plan.whole()) return;
     const MergePlan merge = plan_merge(plan, (int64_t)p.B * p.Hk, p.M, D);
     const dim3 merge_grid((unsigned)(p.B * p.Hk * merge.chunks));
     constexpr int kGroups = 256 / (D / 4);
@@ -1125,7 +1127,8 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
         if (T > 1 && (s < a->head_dim || s >= (1 << 23)))
             return fail(SLIMKV_EUNSUP, "tree attention: drafted rows must lie [head_dim, 2^23) elements apart");
     const TreePlan plan = plan_tree(a);
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes(a->head_dim))
+    if (!plan.whole() &&
+        (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes(a->head_dim)))
         return fail(SLIMKV_EWORKSPACE, "tree attention: workspace missing, misaligned or too small");
     p.q = static_cast<const uint16_t*>(a->q); p.q_sb = a->q_sb; p.q_sl = a->q_sl; p.q_sh = a->q_sh;
     p.dk = static_cast<const uint16_t*>(a->draft_k); p.dk_sb = a->dk_sb; p.dk_sn = a->dk_sn; p.dk_sh = a->dk_sh;
@@ -1139,7 +1142,7 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     p.deal = Dealing{p.B, p.Hk, kKeys, (p.T + kKeys - 1) / kKeys, plan.runs};
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.part = static_cast<float*>(workspace);
-    if (B * Hk * p.M > 0x7fffffff || !launchable(B * Hk * plan_merge(plan, B * Hk, p.M, a->head_dim).chunks, 256) ||
+    if (B * Hk * p.M > 0x7fffffff || (!plan.whole() && !launchable(B * Hk * plan_merge(plan, B * Hk, p.M, a->head_dim).chunks, 256)) ||
         B * Hk * ((a->cache.keys + T) / kKeys + 2) > 0x7fffffff)
         return fail(SLIMKV_EINVAL, "tree attention: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);

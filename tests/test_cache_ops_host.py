@@ -454,3 +454,15 @@ def test_calls_past_what_one_launch_holds_are_refused():
                  lib.slimkv_compact_rows(ref(compact), None)):
         assert code == -1, lib.slimkv_last_error()
         assert b'too many rows' in lib.slimkv_last_error()
+
+
+def test_trees_of_one_run_ask_for_no_workspace():
+    """Past half as many blocks of 128 query rows as two workgroups a CU (256 CUs) an item lies in one run: no partial
+    results, however many blocks there are."""
+    from slimkv_amd import _lib
+    a = _lib.TreeAttentionArgs(q=4096, batch=1, drafted=1024, kv_heads=1, head_dim=128, scale=1.0)
+    need = {}
+    for a.heads in (1, 4, 16, 32, 33, 64, 128, 256):
+        need[a.heads] = _lib.lib().slimkv_tree_attention_workspace(ctypes.byref(a))
+    assert need[1] == need[4] == need[16] == need[32] == 512 * 2 * 128 * 130 * 4
+    assert all(need[heads] == 16 for heads in (33, 64, 128, 256))

@@ -755,3 +755,28 @@ def test_outputs_interleaved_with_other_tensors():
     want = cache_ops.compact_rows(rows, counts, k, v)
     cache_ops.compact_rows(rows, counts, k, v, out_k=halves[:, :, 0], out_v=halves[:, :, 1])
     assert torch.equal(halves[:, :, 0], want[0]) and torch.equal(halves[:, :, 1], want[1])
+
+
+def test_more_query_rows_than_runs():
+    """Blocks of query rows past two workgroups a CU: one run, no partial results, no workspace."""
+    from slimkv_amd import _lib, cache_ops
+    B, T, Hq, D, N, g = 2, 1024, 40, 64, 150, gen(76)
+    assert _lib.lib().slimkv_tree_attention_workspace(_lib.ctypes.byref(_lib.TreeAttentionArgs(
+        q=16, batch=B, drafted=T, heads=Hq, kv_heads=1, head_dim=D, scale=1.0))) == 16
+    k, v = randn(g, B, N, 1, D), randn(g, B, N, 1, D)
+    q, dk, dv = randn(g, B, T, Hq, D), randn(g, B, T, 1, D), randn(g, B, T, 1, D)
+    mask = tree_mask(g, B, T, 'rows')
+    out, lse = cache_ops.tree_attention(q, dk, dv, 0.125, k, v, lengths=lengths_of([N, 0]), mask=mask)
+    for b, n in enumerate((N, 0)):
+        for t in (0, 1, 333, 700, 1023):
+            sees = mask[b, t].cpu().numpy()
+            eo, el, terms, top, mass, total = oc.tree_attention(
+                f64(q[b:b + 1, t:t + 1]), f64(k[b:b + 1]), f64(v[b:b + 1]), [n], f64(dk[b:b + 1])[:, sees],
+                f64(dv[b:b + 1])[:, sees], np.ones((1, int(sees.sum())), bool), 0.125)
+            u = HALF[q.dtype]
+            d = (2.0 ** -24 * (D + 8) * mass + 2.0 ** -22 * (1 + top)).transpose(0, 2, 1)[..., None]
+            assert (np.abs(f64(out[b:b + 1, t:t + 1]) - eo) <= (2 * d + u) * terms + u * np.abs(eo) * (1 + u) + 1e-30).all()
+            got = lse[b, :, t].double().cpu().numpy()
+            assert (np.isneginf(got) == np.isneginf(el[0, :, 0])).all()
+            seen = ~np.isneginf(got)
+            assert (np.abs(got[seen] - el[0, seen, 0]) <= 1e-4).all()
