@@ -408,15 +408,16 @@ def lib():
         raise ImportError(f'{path} is missing: build it with `python -m slimkv_amd.build` '
                           '(slimkv_amd has no fallback compute path)')
     handle = ctypes.CDLL(str(path))
+    # the interface numbers first: a library of another one may lack entry points
+    for query, what, expected in (('slimkv_abi_version', 'ABI', ABI_VERSION),
+                                  ('slimkv_cache_abi_version', 'cache operator ABI', CACHE_ABI_VERSION)):
+        found = getattr(handle, query)() if hasattr(handle, query) else 'none'
+        if found != expected:
+            raise ImportError(f'{path} has {what} {found}, expected {expected}')
     for name, (restype, argtypes) in SIGNATURES.items():
         fn = getattr(handle, name)
         fn.restype = restype
         fn.argtypes = argtypes
-    if handle.slimkv_abi_version() != ABI_VERSION:
-        raise ImportError(f'{path} has ABI {handle.slimkv_abi_version()}, expected {ABI_VERSION}')
-    if handle.slimkv_cache_abi_version() != CACHE_ABI_VERSION:
-        raise ImportError(f'{path} has cache operator ABI {handle.slimkv_cache_abi_version()}, '
-                          f'expected {CACHE_ABI_VERSION}')
     return handle
 
 

@@ -466,3 +466,22 @@ def test_trees_of_one_run_ask_for_no_workspace():
         need[a.heads] = _lib.lib().slimkv_tree_attention_workspace(ctypes.byref(a))
     assert need[1] == need[4] == need[16] == need[32] == 512 * 2 * 128 * 130 * 4
     assert all(need[heads] == 16 for heads in (33, 64, 128, 256))
+
+
+@pytest.mark.parametrize('source,message', [
+    ('int slimkv_abi_version(void) { return 16; }', 'cache operator ABI none, expected 1'),
+    ('int slimkv_abi_version(void) { return 16; } int slimkv_cache_abi_version(void) { return 7; }',
+     'cache operator ABI 7, expected 1'),
+    ('int slimkv_abi_version(void) { return 9; }', 'ABI 9, expected 16'),
+    ('int unrelated(void) { return 0; }', 'ABI none, expected 16'),
+], ids=['before the cache operators', 'another number', 'older', 'another library'])
+def test_an_override_library_of_another_interface_is_named(source, message, tmp_path, monkeypatch):
+    if shutil.which('gcc') is None:
+        pytest.skip('gcc not available')
+    from slimkv_amd import _lib
+    (tmp_path / 'old.c').write_text(source)
+    path = tmp_path / 'old.so'
+    subprocess.run(['gcc', '-shared', '-fPIC', str(tmp_path / 'old.c'), '-o', str(path)], check=True)
+    monkeypatch.setenv('SLIMKV_HIP_LIBRARY', str(path))
+    with pytest.raises(ImportError, match=message):
+        _lib.lib.__wrapped__()
