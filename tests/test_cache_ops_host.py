@@ -468,18 +468,21 @@ def test_trees_of_one_run_ask_for_no_workspace():
     assert all(need[heads] == 16 for heads in (33, 64, 128, 256))
 
 
-@pytest.mark.parametrize('source,message', [
-    ('int slimkv_abi_version(void) { return 16; }', 'cache operator ABI none, expected 1'),
-    ('int slimkv_abi_version(void) { return 16; } int slimkv_cache_abi_version(void) { return 7; }',
-     'cache operator ABI 7, expected 1'),
-    ('int slimkv_abi_version(void) { return 9; }', 'ABI 9, expected 16'),
-    ('int unrelated(void) { return 0; }', 'ABI none, expected 16'),
+@pytest.mark.parametrize('numbers,message', [
+    ((16, None), 'cache operator ABI none, expected 1'),
+    ((16, 7), 'cache operator ABI 7, expected 1'),
+    ((9, None), 'ABI 9, expected 16'),
+    ((None, None), 'ABI none, expected 16'),
 ], ids=['before the cache operators', 'another number', 'older', 'another library'])
-def test_an_override_library_of_another_interface_is_named(source, message, tmp_path, monkeypatch):
+def test_an_override_library_of_another_interface_is_named(numbers, message, tmp_path, monkeypatch):
     if shutil.which('gcc') is None:
         pytest.skip('gcc not available')
     from slimkv_amd import _lib
-    (tmp_path / 'old.c').write_text(source)
+    monkeypatch.setattr(_lib, 'ABI_VERSION', 16)
+    monkeypatch.setattr(_lib, 'CACHE_ABI_VERSION', 1)
+    (tmp_path / 'old.c').write_text('int unrelated;\n' + '\n'.join(
+        f'int {name}(void) {{ return {n}; }}' for name, n in zip(('slimkv_abi_version', 'slimkv_cache_abi_version'), numbers)
+        if n is not None))
     path = tmp_path / 'old.so'
     subprocess.run(['gcc', '-shared', '-fPIC', str(tmp_path / 'old.c'), '-o', str(path)], check=True)
     monkeypatch.setenv('SLIMKV_HIP_LIBRARY', str(path))

@@ -780,3 +780,106 @@ def test_more_query_rows_than_runs():
             assert (np.isneginf(got) == np.isneginf(el[0, :, 0])).all()
             seen = ~np.isneginf(got)
             assert (np.abs(got[seen] - el[0, seen, 0]) <= 1e-4).all()
+
+
+def long_step_inputs(seed):
+    """A step whose weights are split over query rows and whose selection cuts rows into chunks: both with workspaces."""
+    from slimkv_amd import cache_ops
+    B, T, Hq, H, D, N, g = 2, 128, 8, 2, 64, 33100, gen(seed)
+    pages, cols = randn(g, B * 2100, 16, 2, H, D), 2069
+    table = torch.randperm(B * 2100, generator=g, device='cuda')[:B * cols].view(B, cols)
+    lengths = lengths_of([N - seed, 32900 + seed])
+    s = dict(pages=pages, table=table, lengths=lengths, scale=D ** -0.5, keep=5000, q=randn(g, B, T, Hq, D),
+             dk=randn(g, B, T, H, D), dv=randn(g, B, T, H, D), mask=tree_mask(g, B, T, 'tree'),
+             weights=torch.rand(B, H, cols * 16, generator=g, device='cuda') * 1e-3)
+    index = torch.cuda.current_device()
+    assert cache_ops._tree_bytes(index, B, T, Hq, H, D) > 16 and cache_ops._weights_bytes(index, B, T, Hq, H, D, cols * 16) > 16
+    assert cache_ops._select_bytes(index, B, H, cols * 16, s['keep'], 2, 8) > 16
+    return s
+
+
+def same(got, want):
+    return all(torch.equal(a.view(torch.int16) if a.dtype is torch.bfloat16 else a,
+                           b.view(torch.int16) if b.dtype is torch.bfloat16 else b) for a, b in zip(got, want))
+
+
+def test_calls_with_workspaces_side_by_side():
+    from slimkv_amd import cache_ops
+    inputs = [long_step_inputs(81), long_step_inputs(82)]
+    want = [run_step(cache_ops, s) for s in inputs]
+    rows, counts = (x.cpu().numpy() for x in want[0][3:5])
+    er, ec = oc.select_rows(want[0][2].cpu().numpy(), 5000, inputs[0]['lengths'].tolist(), 2, 8)
+    assert (rows == er).all() and (counts == ec).all()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    words = [torch.zeros(1, dtype=torch.int32, device='cuda') for _ in streams]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, (s, st) in enumerate(zip(inputs, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(run_step(cache_ops, s, words[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(same(out, want[i]) for out in got[i]) and words[i].item() == 0
+
+
+def test_two_graphs_with_workspaces_replayed_side_by_side():
+    """Two captured steps, replayed on two streams at once with new inputs and eager work between the replays."""
+    from slimkv_amd import cache_ops
+    inputs = [long_step_inputs(83), long_step_inputs(84)]
+    words = [torch.zeros(1, dtype=torch.int32, device='cuda') for _ in inputs]
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s, word in zip(inputs, words):
+        run_step(cache_ops, s, word)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run_step(cache_ops, s, word))
+    for seed in (85, 87, 89):
+        for s, add in zip(inputs, (0, 1)):
+            fresh = long_step_inputs(seed + add)
+            for name in ('pages', 'table', 'lengths', 'q', 'dk', 'dv', 'mask', 'weights'):
+                s[name].copy_(fresh[name])
+        torch.cuda.synchronize()
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for s, out, word in zip(inputs, outs, words):
+            assert same(out, run_step(cache_ops, s, word)) and word.item() == 0
+
+
+@pytest.mark.parametrize('T', [30, 70, 130])
+@pytest.mark.parametrize('kind', [None, 'tree'])
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+def test_visible_infinities_and_nan_reach_the_rows_that_see_them(T, kind, dtype):
+    """Drafted values that are not finite, in several tiles: their rows' columns take them, all others are as if they
+    were 0."""
+    from slimkv_amd import cache_ops
+    B, Hq, H, D, N, dt, g = 2, 4, 2, 64, 100, TYPES[dtype], gen(91)
+    k, v, place = make_cache(g, B, N, H, D, 0, dt)
+    q, dk, dv = randn(g, B, T, Hq, D, dtype=dt), randn(g, B, T, H, D, dtype=dt), randn(g, B, T, H, D, dtype=dt)
+    mask = tree_mask(g, B, T, kind)
+    inf, nan = float('inf'), float('nan')
+    wild = [(0, 5, 0, 3, inf), (0, T - 2, 0, 3, -inf), (0, T // 2, 1, 17, nan), (1, T - 1, 1, 63, inf), (1, 0, 0, 0, -inf)]
+    clean = dv.clone()
+    for b, t, h, c, x in wild:
+        dv[b, t, h, c], clean[b, t, h, c] = x, 0.0
+    out, lse = cache_ops.tree_attention(q, dk, dv, 0.125, mask=mask, **place)
+    sees = torch.ones(B, T, T, dtype=torch.bool).tril() if mask is None else mask.cpu()
+    extra = np.zeros((B, T, Hq, D))
+    with np.errstate(invalid='ignore'):
+        for b, t, h, c, x in wild:
+            extra[b, sees[b, :, t].numpy(), h * 2:h * 2 + 2, c] += x
+    got = f64(out)
+    bad = ~np.isfinite(extra)
+    assert bad.sum() > T and np.array_equal(got[bad], extra[bad], equal_nan=True)
+    out = torch.where(torch.from_numpy(bad).cuda(), torch.zeros_like(out), out)
+    eo, el, terms, top, mass, total = oc.tree_attention(f64(q), f64(k), f64(v), [N] * B, f64(dk), f64(clean),
+                                                        None if mask is None else mask.cpu().numpy(), 0.125)
+    d = 2.0 ** -24 * (D + 8) * mass + 2.0 ** -22 * (1 + top)
+    u = HALF[dt]
+    tiny = 2.0 ** -40 * (N + T) * np.abs(f64(clean)).max() / total.transpose(0, 2, 1)[..., None] + 2.0 ** -25 if dt is torch.float16 else 0.0
+    tol = (2 * d.transpose(0, 2, 1)[..., None] + u) * terms + u * np.abs(eo) * (1 + u) + tiny
+    assert (np.abs(f64(out) - eo)[~bad] <= tol[~bad]).all()
+    assert np.isfinite(lse.double().cpu().numpy()).all()
