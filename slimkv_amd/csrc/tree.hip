@@ -361,18 +361,18 @@ __device__ __forceinline__ void load_to_lds(const char* base, uint32_t offset, c
     const uint32_t at = (uint32_t)uniform((int)(uintptr_t)(lds_void*)dst);
     if constexpr (ONCE)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(at), "v"(offset), "s"(base)
-                     : "memory");
+                     : "memory", "m0");
     else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base)
-                     : "memory");
+                     : "memory", "m0");
 }
 template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(const char* src, char* dst) {
     const uint32_t at = (uint32_t)uniform((int)(uintptr_t)(lds_void*)dst);
     if constexpr (ONCE)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(src) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(src) : "memory", "m0");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory", "m0");
 }
 
 __device__ __forceinline__ u32x2 read_transposed(const char* p) {
