@@ -466,8 +466,8 @@ struct CompactParams {
     uint16_t* ov; int64_t ov_sb, ov_sn, ov_sh;
     float* weights; int64_t w_sb, w_sh;
     float* ow; int64_t ow_sb, ow_sh;
-    int Hw, wkeys, B, Hk, D, keep;
-    int move_blocks, weight_blocks;               // workgroups a sequence: K/V rows, weights
+    int Hw, wkeys, Hk, D, keep;
+    int move_blocks;                              // workgroups a sequence that move K and V rows
     int lanes_log;                                // in place: log2 of the 16-byte lanes of a part
 };
 
@@ -748,7 +748,7 @@ extern "C" int slimkv_compact_rows(const slimkv_compact_rows_args* a, void* stre
     p.weights = a->weights; p.w_sb = a->w_sb; p.w_sh = a->w_sh;
     p.ow = a->out_weights; p.ow_sb = a->ow_sb; p.ow_sh = a->ow_sh;
     p.Hw = (int)a->weight_heads; p.wkeys = (int)a->weight_keys;
-    p.B = (int)a->batch; p.Hk = (int)a->kv_heads; p.D = (int)a->head_dim; p.keep = (int)a->keep;
+    p.Hk = (int)a->kv_heads; p.D = (int)a->head_dim; p.keep = (int)a->keep;
     hipStream_t st = static_cast<hipStream_t>(stream);
     int64_t move, weights;
     if (a->in_place) {
@@ -763,7 +763,6 @@ extern "C" int slimkv_compact_rows(const slimkv_compact_rows_args* a, void* stre
     if (!launchable(move + weights, a->in_place ? kMoveThreads : 256))
         return fail(SLIMKV_EINVAL, "compact rows: too many rows for one call");
     p.move_blocks = (int)move;
-    p.weight_blocks = (int)weights;
     const dim3 grid((unsigned)(move + weights), (unsigned)a->batch);
     if (a->in_place) {
         if (p.c.table) hipLaunchKernelGGL(compact_in_place_kernel<true>, grid, dim3(kMoveThreads), 0, st, p);

@@ -31,7 +31,7 @@ struct WeightsParams {
     const float* lse; int64_t l_sb, l_sh, l_sl;
     const float* previous; int64_t p_sb, p_sh;
     float* out; int64_t w_sb, w_sh;
-    int B, L, Hq, Hk, causal;
+    int B, L, Hk, causal;
     FastDiv G;
     int M, splits, blocks;                        // M = L * G query rows; blocks of keys a (sequence, head)
     float scale_log2;
@@ -427,7 +427,7 @@ extern "C" int slimkv_attention_weights(const slimkv_attention_weights_args* a, 
     p.lse = a->lse; p.l_sb = a->l_sb; p.l_sh = a->l_sh; p.l_sl = a->l_sl;
     p.previous = a->previous; p.p_sb = a->p_sb; p.p_sh = a->p_sh;
     p.out = a->out; p.w_sb = a->w_sb; p.w_sh = a->w_sh;
-    p.B = (int)a->batch; p.L = (int)a->queries; p.Hq = (int)a->heads; p.Hk = (int)a->kv_heads; p.causal = a->causal ? 1 : 0;
+    p.B = (int)a->batch; p.L = (int)a->queries; p.Hk = (int)a->kv_heads; p.causal = a->causal ? 1 : 0;
     p.G = fast_div(a->heads / a->kv_heads);
     p.M = p.L * (int)p.G.d;
     const WeightsPlan plan = plan_weights(a);
