@@ -13,7 +13,13 @@
  * and the outputs; head_dim 64 or 128; heads a multiple of kv_heads (query
  * head j reads KV head j / (heads / kv_heads)).  Rows start on 16-byte
  * boundaries: addresses aligned, strides multiples of 8 elements (strides of
- * dimensions of one element are not read).
+ * dimensions of one element are not read); rows of K, V and drafted tokens lie
+ * [head_dim, 2^23) elements apart.
+ *
+ * Sizes: batch up to 65535, heads up to 4096, heads / kv_heads up to 256, drafted
+ * up to 1024, keys up to 2^30.  `scale` lies in [1e-18, 1e18]: zero, negative,
+ * infinite and NaN scales are SLIMKV_EINVAL, as is a call whose launches would
+ * hold 2^32 threads or more.
  */
 #ifndef SLIMKV_CACHE_OPS_H
 #define SLIMKV_CACHE_OPS_H
@@ -54,7 +60,9 @@ typedef struct slimkv_cache_rows {
  * 0: one for all; NULL: j <= t), out [B, T, Hq, D], lse [B, Hq, T] fp32
  * contiguous.  A row that sees nothing gives output 0 and LSE -inf; what lies
  * in rows a query does not see (infinities and NaN included) has no influence.
- * T = 1 without a mask is the decode of a single token.
+ * T = 1 without a mask is the decode of a single token.  Softmax weights are
+ * rounded to the element type for the product with V (fp16: held 2^15 times as
+ * large, so that 2^-39 of a row's largest is not lost); sums and LSE are fp32.
  * ---------------------------------------------------------------------- */
 typedef struct slimkv_tree_attention_args {
     slimkv_cache_rows cache;

@@ -10,7 +10,9 @@ A cache is given as dense rows k, v [B, N, Hkv, D] or as raw pages
 [blocks, block, 2, Hkv, D] (RawPages' format) with a block table [B, cols] int64;
 `lengths` [B] int32 are the rows each sequence holds (default: all N).  Element
 types bf16 and fp16 (one for all tensors of a call), head_dim 64 or 128, keys
-rotated.  Cache rows start on 16-byte boundaries.
+rotated.  Cache rows start on 16-byte boundaries and lie less than 2^23 elements
+apart.  Up to 65535 sequences, 4096 query heads, 256 of them a KV head; softmax
+scales in [1e-18, 1e18] (zero, negative ones and NaN raise ValueError).
 
 A speculative step over a bounded cache: tree_attention gives the drafted
 tokens' outputs and LSEs; the accepted path's K/V rows are appended to the
@@ -300,7 +302,10 @@ def tree_attention(q, draft_k, draft_v, scale, k=None, v=None, *, pages=None, ta
     only if so marked); None is a chain (j <= t).  Every token sees all rows of
     its sequence's cache.  Returns (out [B, T, Hq, D], lse [B, Hq, T] fp32); a
     row that sees nothing gives 0 and -inf, and what lies in unseen rows has no
-    influence, infinities and NaN included.  T = 1 decodes a single token."""
+    influence, infinities and NaN included.  T = 1 decodes a single token.
+    Softmax weights are rounded to the element type for their product with v
+    (half a step of each weight; fp16 ones keep 2^-39 of the row's largest),
+    their sum and the LSE are fp32."""
     name = 'tree_attention'
     B = q.shape[0]
     place, rows, H, D, paged, keep = _cache(name, k, v, pages, table, lengths, keys, B)

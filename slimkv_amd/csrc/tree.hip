@@ -4,17 +4,20 @@
 // The T * G query rows of one KV head (row p = t * G + g) are the columns of
 // the score MFMA: S^T = K . Q^T with K rows as A and the query rows held in
 // registers as B, so the softmax statistics stay in a lane's column, and O^T =
-// V^T . P^T with P^T straight from the score registers (weights rounded once to
-// the element type, their sum fp32 and unrounded).  K and V rows go from memory
-// straight to LDS, row by row; V is transposed by the LDS read.
+// V^T . P^T with P^T straight from the score registers.  Weights are rounded once
+// to the element type, since the matrix instruction takes both operands in it: at
+// most half a step of sum p |v|, of either sign; their sum is fp32 and of the
+// unrounded ones.  K and V rows go from memory straight to LDS, row by row; V is
+// transposed by the LDS read.
 //
 // Up to 32 query rows a KV head the cache's bytes are the bound: tree_few_kernel,
 // whose waves share nothing but the end (16 sequences of 8-32K paged rows, a
-// token each: 222 us for 1.34 GB, 6.0 TB/s; a copy moves 4.9-5.3).  More rows
-// are bound by the matrix cores and by how well loads hide behind them:
-// tree_many_kernel, 64 or 128 rows a workgroup (26 tokens on the same cache 283
-// us, 4.8 TB/s; 63 tokens of 40 heads over 131071 rows 262 us, 640 TFLOP/s of
-// needed work, 785 with the rows that fill up the last block of 128).
+// token each: a call of 234 us for 1.34 GB, 5.7 TB/s; a copy moves 4.9-5.3).  More
+// rows are bound by the matrix cores and by how well loads hide behind them:
+// tree_many_kernel, 64 or 128 rows a workgroup (26 tokens on the same cache 293
+// us, 4.6 TB/s; 63 tokens of 40 heads over 131071 rows 255 us, 664 TFLOP/s of
+// needed work, 809 with the rows that fill up the last block of 128).  Figures
+// beside a choice compare its two sides as they were when it was made.
 //
 // Schedule.  The tiles of 64 rows of all (sequence, KV head) items -- the cache's
 // rows, then the drafted tokens' -- lie in a row and are dealt to two workgroups a

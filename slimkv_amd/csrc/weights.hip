@@ -15,7 +15,10 @@
 // read from LDS feeds four products (with 32 the LDS reads alone take as long
 // as the products), and the query rows pass through LDS 64 at a time.  Where
 // the key blocks do not fill the CUs evenly the query rows are split as well and
-// the parts are added by a second kernel in order.
+// the parts are added by a second kernel in order.  A 2048-query chunk over two
+// sequences of up to 10240 rows takes 231 us, the last 32 queries over 32771 rows
+// 25.6, a token over 16 x 8-32K rows 138 (5.0 TB/s of K).  Figures beside a choice
+// compare its two sides as they were when it was made.
 
 #include "cache.hpp"
 
@@ -38,8 +41,9 @@ struct WeightsParams {
     float* part;                                  // [splits][B][Hk][keys]
 };
 
-// Query row `row` (clamped to the last): its address, its LSE in log2 and the
-// last key it sees (-1: none, also for a row that counts nothing).
+// Query row `row` (clamped to the last): its address, its LSE in log2 (rounded to
+// fp32 once more, 2^-24 of it, as the scaled score is) and the last key it sees (-1:
+// none, also for a row that counts nothing).
 __device__ __forceinline__ const uint16_t* query_address(const WeightsParams& p, int64_t b, int h, int row) {
     const int r = min(row, p.M - 1), l = quotient(r, p.G), g = r - l * (int)p.G.d;
     return p.q + b * p.q_sb + l * p.q_sl + (int64_t)(h * (int)p.G.d + g) * p.q_sh;

@@ -883,3 +883,13 @@ def test_visible_infinities_and_nan_reach_the_rows_that_see_them(T, kind, dtype)
     tol = (2 * d.transpose(0, 2, 1)[..., None] + u) * terms + u * np.abs(eo) * (1 + u) + tiny
     assert (np.abs(f64(out) - eo)[~bad] <= tol[~bad]).all()
     assert np.isfinite(lse.double().cpu().numpy()).all()
+
+
+@pytest.mark.parametrize('scale', [0.0, -0.125, 1e19, 1e-19, float('inf'), float('nan')])
+def test_softmax_scales_outside_the_range_are_refused(scale):
+    from slimkv_amd import cache_ops
+    q, k = randn(gen(92), 1, 2, 4, 64), randn(gen(93), 1, 2, 2, 64)
+    with pytest.raises(ValueError, match='scale'):
+        cache_ops.tree_attention(q, k, k, scale, k, k)
+    with pytest.raises(ValueError, match='scale'):
+        cache_ops.attention_weights(q, torch.zeros(1, 4, 2, device='cuda'), scale, k)
