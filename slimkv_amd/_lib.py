@@ -279,6 +279,50 @@ CompactRowsArgs = _struct('slimkv_compact_rows_args', [
     ('in_place', c_i32), ('dtype', c_i32),
 ])
 
+# include/slimkv/quant_cache.h
+QuantPages = _struct('slimkv_quant_pages', [
+    ('pages', c_ptr), *_i64s('p_sb', 'p_sh'),
+    ('table', c_ptr), *_i64s('t_sb', 't_cols', 'num_pages', 'block_size'),
+    ('status', c_ptr),
+])
+
+_QUANT_ROWS = [
+    ('cache', QuantPages),
+    ('k', c_ptr), *_i64s('k_sb', 'k_sn', 'k_sh'),
+    ('v', c_ptr), *_i64s('v_sb', 'v_sn', 'v_sh'),
+    ('starts', c_ptr), ('counts', c_ptr),
+    *_i64s('batch', 'rows', 'kv_heads', 'head_dim'),
+    ('dtype', c_i32),
+]
+QuantizeRowsArgs = _struct('slimkv_quantize_rows_args', _QUANT_ROWS)
+DequantizeRowsArgs = _struct('slimkv_dequantize_rows_args', _QUANT_ROWS)
+
+QuantizedAttentionArgs = _struct('slimkv_quantized_attention_args', [
+    ('cache', QuantPages),
+    ('lengths', c_ptr), ('keys', c_i64),
+    ('q', c_ptr), *_i64s('q_sb', 'q_sl', 'q_sh'),
+    ('draft_k', c_ptr), *_i64s('dk_sb', 'dk_sn', 'dk_sh'),
+    ('draft_v', c_ptr), *_i64s('dv_sb', 'dv_sn', 'dv_sh'),
+    ('mask', c_ptr), *_i64s('m_sb', 'm_sl'),
+    ('out', c_ptr), *_i64s('o_sb', 'o_sl', 'o_sh'),
+    ('lse', c_ptr),
+    *_i64s('batch', 'tokens', 'heads', 'kv_heads', 'head_dim'),
+    ('scale', c_f64), ('dtype', c_i32),
+])
+
+NormRopeArgs = _struct('slimkv_norm_rope_args', [
+    ('q', c_ptr), *_i64s('q_sb', 'q_sl', 'q_sh'),
+    ('k', c_ptr), *_i64s('k_sb', 'k_sl', 'k_sh'),
+    ('q_weight', c_ptr), ('k_weight', c_ptr),
+    ('cos', c_ptr), ('sin', c_ptr), ('table_rows', c_i64),
+    ('positions', c_ptr), *_i64s('pos_sb', 'pos_sl'),
+    ('out_q', c_ptr), *_i64s('oq_sb', 'oq_sl', 'oq_sh'),
+    ('out_k', c_ptr), *_i64s('ok_sb', 'ok_sl', 'ok_sh'),
+    ('status', c_ptr),
+    *_i64s('batch', 'length', 'heads', 'kv_heads', 'head_dim'),
+    ('eps', c_f64), ('weight_f32', c_i32), ('dtype', c_i32),
+])
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     'slimkv_last_error': (ctypes.c_char_p, []),
@@ -336,10 +380,18 @@ SIGNATURES = {
     'slimkv_select_rows_workspace': (ctypes.c_size_t, [ctypes.POINTER(SelectRowsArgs)]),
     'slimkv_select_rows': (ctypes.c_int, [c_ptr, c_ptr, ctypes.c_size_t, c_ptr]),
     'slimkv_compact_rows': (ctypes.c_int, [c_ptr, c_ptr]),
+    # include/slimkv/quant_cache.h (likewise)
+    'slimkv_quant_abi_version': (ctypes.c_int, []),
+    'slimkv_quantize_rows': (ctypes.c_int, [c_ptr, c_ptr]),
+    'slimkv_dequantize_rows': (ctypes.c_int, [c_ptr, c_ptr]),
+    'slimkv_quantized_attention_workspace': (ctypes.c_size_t, [ctypes.POINTER(QuantizedAttentionArgs)]),
+    'slimkv_quantized_attention': (ctypes.c_int, [c_ptr, c_ptr, ctypes.c_size_t, c_ptr]),
+    'slimkv_norm_rope': (ctypes.c_int, [c_ptr, c_ptr]),
 }
 
 ABI_VERSION = 16
 CACHE_ABI_VERSION = 1          # include/slimkv/cache_ops.h
+QUANT_ABI_VERSION = 1          # include/slimkv/quant_cache.h
 
 STAGE_PROLOGUE, STAGE_ATTEND, STAGE_COMBINE, STAGE_ALL = 1, 2, 4, 7
 NOALLOC_SCRATCH_BYTES = 64 << 20
@@ -410,7 +462,8 @@ def lib():
     handle = ctypes.CDLL(str(path))
     # the interface numbers first: a library of another one may lack entry points
     for query, what, expected in (('slimkv_abi_version', 'ABI', ABI_VERSION),
-                                  ('slimkv_cache_abi_version', 'cache operator ABI', CACHE_ABI_VERSION)):
+                                  ('slimkv_cache_abi_version', 'cache operator ABI', CACHE_ABI_VERSION),
+                                  ('slimkv_quant_abi_version', '4-bit cache ABI', QUANT_ABI_VERSION)):
         found = getattr(handle, query)() if hasattr(handle, query) else 'none'
         if found != expected:
             raise ImportError(f'{path} has {what} {found}, expected {expected}')

@@ -14,7 +14,7 @@ PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / 'csrc'
 LIBRARY = PACKAGE / 'libslimkv_hip.so'
 SOURCES = ['attention.hip', 'rope.hip', 'recon.hip', 'paged.hip', 'prefill.hip', 'down.hip', 'project.hip',
-           'eager.hip', 'tree.hip', 'weights.hip', 'evict.hip']
+           'eager.hip', 'tree.hip', 'weights.hip', 'evict.hip', 'heads.hip', 'quant.hip', 'quant_attention.hip']
 # measurement probes: a library of their own (include/slimkv_probe.h)
 PROBE_LIBRARY = PACKAGE / 'libslimkv_probe.so'
 PROBE_SOURCES = ['probe.hip']

@@ -26,12 +26,16 @@ slimkv_amd.kernels and has no CPU implementation.
         the cache operators (slimkv_amd.cache_ops), out of place; index errors
         are left in `status`, which reads through block tables and row moves
         need
+    slimkv::quantized_attention, dequantize_rows, quantize_rows, norm_rope
+        a cache held in 4 bits (slimkv_amd.quant_cache); quantize_rows writes
+        `pages` and returns nothing, norm_rope takes queries and keys; index
+        errors as above
 """
 from typing import Optional
 
 import torch
 
-from . import cache_ops, kernels
+from . import cache_ops, kernels, quant_cache
 
 Tensor = torch.Tensor
 _NS = 'slimkv'
@@ -189,3 +193,57 @@ def _(rows, counts, k, v, pages, table, weights, status):
     first = k if k is not None else pages
     shape = (rows.shape[0], rows.shape[2], *first.shape[-2:])
     return first.new_empty(shape), first.new_empty(shape), weights.new_empty(rows.shape)
+
+
+@torch.library.custom_op(f'{_NS}::quantized_attention', mutates_args=('status',), device_types='cuda')
+def quantized_attention(q: Tensor, draft_k: Optional[Tensor], draft_v: Optional[Tensor], scale: float, pages: Tensor,
+                        table: Optional[Tensor], lengths: Optional[Tensor], keys: Optional[int], mask: Optional[Tensor],
+                        status: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """quant_cache.quantized_attention: q [B,T,Hq,D] -> (out [B,T,Hq,D], lse [B,Hq,T])."""
+    return quant_cache.quantized_attention(q, draft_k, draft_v, scale, pages, table, lengths=lengths, keys=keys, mask=mask,
+                                           status=status)
+
+
+@quantized_attention.register_fake
+def _(q, draft_k, draft_v, scale, pages, table, lengths, keys, mask, status):
+    B, T, Hq, D = q.shape
+    return q.new_empty((B, T, Hq, D)), _lse_like(q, B, Hq, T)
+
+
+@torch.library.custom_op(f'{_NS}::quantize_rows', mutates_args=('pages', 'status'), device_types='cuda')
+def quantize_rows(k: Tensor, v: Tensor, pages: Tensor, table: Optional[Tensor], starts: Optional[Tensor],
+                  counts: Optional[Tensor], status: Optional[Tensor]) -> None:
+    """quant_cache.quantize_rows: k, v [B,n,Hkv,D] written into pages."""
+    quant_cache.quantize_rows(k, v, pages, table, starts=starts, counts=counts, status=status)
+
+
+@quantize_rows.register_fake
+def _(k, v, pages, table, starts, counts, status):
+    return None
+
+
+@torch.library.custom_op(f'{_NS}::dequantize_rows', mutates_args=('status',), device_types='cuda')
+def dequantize_rows(pages: Tensor, rows: int, head_dim: int, table: Optional[Tensor], starts: Optional[Tensor],
+                    counts: Optional[Tensor], dtype: torch.dtype, status: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """quant_cache.dequantize_rows: -> (k, v [B,rows,Hkv,D])."""
+    return quant_cache.dequantize_rows(pages, rows, head_dim, table, starts=starts, counts=counts, dtype=dtype,
+                                       status=status)
+
+
+@dequantize_rows.register_fake
+def _(pages, rows, head_dim, table, starts, counts, dtype, status):
+    batch = next(t for t in (table, starts, counts, pages) if t is not None).shape[0]
+    shape = (batch, rows, pages.shape[1], head_dim)
+    return pages.new_empty(shape, dtype=dtype), pages.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op(f'{_NS}::norm_rope', mutates_args=('status',), device_types='cuda')
+def norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, q_weight: Optional[Tensor],
+              k_weight: Optional[Tensor], eps: float, status: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """quant_cache.norm_rope: q [B,L,Hq,D], k [B,L,Hkv,D] -> normalised and rotated."""
+    return quant_cache.norm_rope(q, k, cos, sin, positions, q_weight=q_weight, k_weight=k_weight, eps=eps, status=status)
+
+
+@norm_rope.register_fake
+def _(q, k, cos, sin, positions, q_weight, k_weight, eps, status):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
