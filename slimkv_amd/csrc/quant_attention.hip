@@ -29,6 +29,14 @@ struct QuantParams {
     PoolView z;
 };
 
+// The kernel's arguments, read where they are used: kept in scalar registers
+// over the whole kernel they push each other out.
+__device__ __forceinline__ const QuantParams& parameters() {
+    auto args = (const __attribute__((address_space(4))) QuantParams*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    return *(const QuantParams*)args;
+}
+
 // 16 rows of K and V as a lane holds them: K of row `col`, elements D / 4 grp on;
 // V of rows 4 grp .. 4 grp + 3, columns col + 16 md; their scales.
 template <int D>
@@ -51,42 +59,57 @@ struct GroupOffsets {
     }
 };
 
-typedef const __attribute__((address_space(4))) int64_t* table_entries;
+// Where groups of 16 rows lie, 64 of them at a time, one a lane: no load of codes
+// waits for the table, whose next 64 entries are on their way meanwhile.
+struct Places {
+    const int64_t* entries;           // the sequence's row of the table; none: one page
+    int64_t entry;                    // asked for
+    uint32_t page, slot;              // held
 
-// A wave's way to the groups of one item: the page numbers on the scalar unit.
-template <int D>
-struct GroupLoader {
-    GroupOffsets<D> off;
-    const uint8_t* head;              // page 0 of the item's head (no table: the sequence's page)
-    const int64_t* entries;
-
-    __device__ __forceinline__ void item(const PoolView& z, int64_t b, int h) {
-        head = z.pages + h * z.p_sh + (z.table ? 0 : b * z.p_sb);
-        entries = z.table ? z.table + b * z.t_sb : nullptr;
+    // The lane's next group begins at `row`.
+    __device__ __forceinline__ void ask(const PoolView& z, int row) {
+        entry = entries ? entries[quotient(row, z.block)] : 0;
     }
-    // The table entry of the page that holds row `row`, as it stands there.
-    __device__ __forceinline__ int64_t entry(const PoolView& z, int row) const {
-        return entries ? ((table_entries)(uintptr_t)entries)[quotient(row, z.block)] : 0;
-    }
-    // The group of rows row .. row + 15.
-    __device__ __forceinline__ void load(const PoolView& z, int64_t entry, int row, Group<D>& x) const {
-        typedef typename Group<D>::vec vec;
-        int64_t page = 0, slot = row;
+    __device__ __forceinline__ void take(const PoolView& z, int row) {
+        page = 0;
+        slot = row;
         if (entries) {
-            page = table_page(entry, z.num_pages);
-            if (page < 0) {
-                report_bad_page(z.status);
-                page = 0;
-            }
+            const int64_t at = table_page(entry, z.num_pages);
+            if (at < 0) report_bad_page(z.status);
+            page = at < 0 ? 0u : (uint32_t)at;
             slot = row - quotient(row, z.block) * (int)z.block.d;
         }
-        const uint8_t* base = head + page * z.p_sb;
-        const uint8_t* codes = base + slot * (D / 2);
-        const uint8_t* scales = base + slot * (D / 32);
-        x.k = *reinterpret_cast<const vec*>(codes + off.k);
-        x.v = *reinterpret_cast<const vec*>(codes + z.v_at + off.v);
-        x.ks = (scales + z.ks_at)[off.ks];
-        x.vs = *reinterpret_cast<const vec*>(scales + z.vs_at + off.vs);
+    }
+};
+
+// A wave's way to the groups of one item.
+template <int D>
+struct GroupLoader {
+    const uint8_t* head;              // page 0 of the item's head (no table: the sequence's page)
+    int64_t p_sb, v_at, ks_at, vs_at;
+    Places places;
+
+    __device__ __forceinline__ GroupLoader(const PoolView& z, int64_t b, int h)
+        : head(z.pages + h * z.p_sh + (z.table ? 0 : b * z.p_sb)), p_sb(z.p_sb), v_at(z.v_at), ks_at(z.ks_at),
+          vs_at(z.vs_at) {
+        places.entries = z.table ? z.table + b * z.t_sb : nullptr;
+    }
+    struct Parts {
+        const uint8_t *codes, *scales;
+    };
+    // K's codes and scales of the group that lane `at` holds the place of, but for the page's offsets.
+    __device__ __forceinline__ Parts parts(int at) const {
+        const uint32_t page = __builtin_amdgcn_readlane(places.page, at), slot = __builtin_amdgcn_readlane(places.slot, at);
+        const uint8_t* base = head + page * p_sb;
+        return Parts{base + (int64_t)slot * (D / 2), base + (int64_t)slot * (D / 32)};
+    }
+    __device__ __forceinline__ void load(const GroupOffsets<D>& off, int at, Group<D>& x) const {
+        typedef typename Group<D>::vec vec;
+        const Parts from = parts(at);
+        x.k = *reinterpret_cast<const vec*>(from.codes + off.k);
+        x.v = *reinterpret_cast<const vec*>(from.codes + v_at + off.v);
+        x.ks = (from.scales + ks_at)[off.ks];
+        x.vs = *reinterpret_cast<const vec*>(from.scales + vs_at + off.vs);
     }
 };
 
@@ -99,101 +122,55 @@ __device__ __forceinline__ u32x4 key_values(const Group<D>& x, int kk) {
 // The scales of the lane's four V rows behind `left` of the group's rows: none,
 // since a block behind the end may hold anything.
 template <int D>
-__device__ __forceinline__ void drop_scales(Group<D>& x, int left) {
+__device__ __forceinline__ void drop_scales(typename Group<D>::vec& scales, int left) {
     const int grp = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (4 * grp + j < left) continue;
-        if constexpr (D == 128) x.vs[j] = 0;
-        else x.vs[j / 2] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+        if constexpr (D == 128) scales[j] = 0;
+        else scales[j / 2] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
     }
 }
 
-// Value operands: the lane's four keys of column 16 md + col, two elements a
-// dword, for all md.
+// Value operands of columns 32 pr + col and 32 pr + 16 + col: the lane's four keys,
+// two elements a dword.
 template <int D, bool F16>
-__device__ __forceinline__ void value_values(const Group<D>& x, u32x2 (&out)[D / 16]) {
+__device__ __forceinline__ void value_values(const typename Group<D>::vec& codes, const typename Group<D>::vec& scales,
+                                             int pr, u32x2 (&out)[2]) {
     using C = Codes<F16>;
-    uint32_t pair[4][D / 32];           // key j: columns 32 pr + col (low) and 32 pr + 16 + col (high)
+    uint32_t pair[4];                   // key j: both columns
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        if constexpr (D == 128) {
-            const uint32_t w = x.v[j], f = x.vs[j];
-            pair[j][0] = C::template values<0>(w, f << 23);
-            pair[j][1] = C::template values<1>(w, f << 15);
-            pair[j][2] = C::template values<2>(w, f << 7);
-            pair[j][3] = C::template values<3>(w, f >> 1);
-        } else {
-            const uint32_t w = x.v[j / 2], f = x.vs[j / 2];
-            if (j & 1) {
-                pair[j][0] = C::template values<2>(w, f << 7);
-                pair[j][1] = C::template values<3>(w, f >> 1);
-            } else {
-                pair[j][0] = C::template values<0>(w, f << 23);
-                pair[j][1] = C::template values<1>(w, f << 15);
-            }
-        }
+        const int byte = D == 128 ? pr : 2 * (j & 1) + pr;
+        const uint32_t w = codes[D == 128 ? j : j / 2], f = scales[D == 128 ? j : j / 2];
+        pair[j] = byte == 0   ? C::template values<0>(w, f << 23)
+                  : byte == 1 ? C::template values<1>(w, f << 15)
+                  : byte == 2 ? C::template values<2>(w, f << 7)
+                              : C::template values<3>(w, f >> 1);
     }
-#pragma unroll
-    for (int pr = 0; pr < D / 32; ++pr) {
-        out[2 * pr] = u32x2{__builtin_amdgcn_perm(pair[1][pr], pair[0][pr], 0x05040100u),
-                            __builtin_amdgcn_perm(pair[3][pr], pair[2][pr], 0x05040100u)};
-        out[2 * pr + 1] = u32x2{__builtin_amdgcn_perm(pair[1][pr], pair[0][pr], 0x07060302u),
-                                __builtin_amdgcn_perm(pair[3][pr], pair[2][pr], 0x07060302u)};
-    }
+    out[0] = u32x2{__builtin_amdgcn_perm(pair[1], pair[0], 0x05040100u), __builtin_amdgcn_perm(pair[3], pair[2], 0x05040100u)};
+    out[1] = u32x2{__builtin_amdgcn_perm(pair[1], pair[0], 0x07060302u), __builtin_amdgcn_perm(pair[3], pair[2], 0x07060302u)};
 }
 
 // A workgroup's LDS: tiles or staged rows, joined states.
-template <int BYTES, int ROWS>
+template <int BYTES, int WAVES, int ROWS>
 struct alignas(1024) QuantLds {
     char rows[BYTES];
-    uint64_t seen[4][ROWS];       // drafted_seen's words, by wave
+    uint64_t seen[WAVES][ROWS];   // drafted_seen's words, by wave
     int wild;                     // drafted values that are not finite
 };
 
-// ---------------------------------------------------------------------------
-// up to 32 query rows a KV head
-// ---------------------------------------------------------------------------
+// The softmax of NT columns' scores, in two steps with one branch between them, so
+// that the exponentials lie in one block with the products that take them and
+// with the conversion of V.  First the maxima: where none moves (and none is so
+// large that products are rounded first, as in softmax_step) nothing else happens.
+template <int NT, int MT, int MD, bool F16>
+struct Softmax {
+    float factor[NT], base[NT];       // exponent of score s: factor s - base
+    float m[NT], l[NT];
+    v4f o[NT][MD];
 
-constexpr int kUnit = 4;                       // groups of 16 rows that a wave takes of a tile
-constexpr int kFewRows = 4 * 16 * kUnit;       // rows of a tile
-
-// A wave owns 64 rows of each tile and works for itself in its registers: the next
-// tile's codes are on their way while one is computed.
-template <int D, bool F16, int NT>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) quant_few_kernel(QuantParams qp) {
-    const TreeParams& p = qp.t;
-    const PoolView& z = qp.z;
-    using E = Elem<F16>;
-    using R = Rows16<D>;
-    constexpr int KS = D / 32, MD = D / 16, kRows = 16 * NT, kPart = kRows * (D + 2), kWave = 2 * R::kBytes;
-    constexpr int kBytes = 4 * kWave > 12 * kPart ? 4 * kWave : 12 * kPart;      // staged rows, or the join of three waves
-    __shared__ QuantLds<kBytes, kRows> sh;
-
-    const int run = slot_of_block();
-    const Deal deal(p.deal, total_tiles(p.c, p.deal));
-    if (run >= deal.runs) return;
-    int pos = deal.begin(run);
-    const int end = deal.begin(run + 1);
-    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
-    const int col = lane & 15, grp = lane >> 4;
-    char* staging = sh.rows + wave * kWave;
-    GroupLoader<D> loader;
-
-    while (pos < end) {
-        const Item it = item_at(p, pos, end);
-        const int64_t b = it.b;
-        const int cached = (it.n + kFewRows - 1) / kFewRows;
-        const int stop = max(it.t0, min(it.t1, cached));                 // tiles [t0, stop) of the cache
-        loader.item(z, b, it.h);
-        __syncthreads();                                                 // the item before is done with LDS
-        if (threadIdx.x == 0) sh.wild = 0;
-        __syncthreads();
-        u32x4 qr[NT][KS];
-        load_queries<KS, NT, true>(p, b, it.h, 0, qr);
-
-        v4f o[NT][MD];
-        float m[NT], l[NT];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt] = kNegInf;
@@ -201,19 +178,109 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
 #pragma unroll
             for (int md = 0; md < MD; ++md) o[nt][md] = v4f{0.f, 0.f, 0.f, 0.f};
         }
+    }
+    __device__ __forceinline__ void move(v4f (&s)[NT][MT], float scale_log2) {
+        float top[NT];
+        bool moves = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float mx = kNegInf;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[nt][mt][i]);
+            mx = rows_max(mx);
+            top[nt] = fmaxf(m[nt], base_of<F16>(rounded_product(mx, scale_log2)));
+            factor[nt] = scale_log2;
+            base[nt] = top[nt] == kNegInf ? 0.f : top[nt];
+            moves |= top[nt] != m[nt] || __builtin_fabsf(base[nt]) >= kFarBase;
+        }
+        if (!__ballot(moves)) return;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float alpha = fast_exp2(m[nt] - base[nt]);
+            m[nt] = top[nt];
+            l[nt] *= alpha;
+#pragma unroll
+            for (int md = 0; md < MD; ++md) o[nt][md] *= alpha;
+            if (__builtin_fabsf(base[nt]) >= kFarBase) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nt][mt][i] = far_exponent(s[nt][mt][i], scale_log2, base[nt]);
+                factor[nt] = 1.f;
+                base[nt] = 0.f;
+            }
+        }
+    }
+    // Two weights, rounded to the element type; their sum before that joins `sum`.
+    __device__ __forceinline__ uint32_t weigh(int nt, float a, float b, float& sum) const {
+        const float pa = fast_exp2(__builtin_fmaf(a, factor[nt], -base[nt]));
+        const float pb = fast_exp2(__builtin_fmaf(b, factor[nt], -base[nt]));
+        sum += pa + pb;
+        return Elem<F16>::pack(pa, pb);
+    }
+    // The weights of a column's scores as operands of two groups of 16 keys each.
+    __device__ __forceinline__ void weigh(const v4f (&s)[NT][MT], u32x4 (&pb)[MT / 2][NT]) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 2 * MT; ++x) pb[x / 4][nt][x % 4] = weigh(nt, s[nt][x / 2][2 * (x & 1)], s[nt][x / 2][2 * (x & 1) + 1], sum);
+            l[nt] += sum;
+        }
+    }
+};
 
-        // the wave's rows of tile t, those past the last group again the last one
-        const int last_row = (it.n - 1) & ~15;
-        auto row_of = [&](int t, int u) { return min(t * kFewRows + (wave * kUnit + u) * 16, last_row); };
+// ---------------------------------------------------------------------------
+// up to 32 query rows a KV head
+// ---------------------------------------------------------------------------
+
+// Groups of 16 rows that a wave takes of a tile: four with up to 16 query rows, two
+// with up to 32 (four spill 73 registers).
+constexpr int few_groups(int nt) { return nt == 1 ? 4 : 2; }
+
+// A wave owns 64 (32) rows of each tile and works for itself in its registers: the
+// next tile's codes are on their way while one is computed.
+template <int D, bool F16, int NT>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) quant_few_kernel(QuantParams) {
+    using E = Elem<F16>;
+    using R = Rows16<D>;
+    constexpr int KS = D / 32, MD = D / 16, kRows = 16 * NT, kPart = kRows * (D + 2), kWave = 2 * R::kBytes;
+    constexpr int kUnit = few_groups(NT), kFewRows = 64 * kUnit;                 // rows of a tile
+    constexpr int kBytes = 4 * kWave > 12 * kPart ? 4 * kWave : 12 * kPart;      // staged rows, or the join of three waves
+    __shared__ QuantLds<kBytes, 4, kRows> sh;
+
+    const int run = slot_of_block();
+    int pos, end;
+    {
+        const TreeParams& p = parameters().t;
+        const Deal deal(p.deal, total_tiles(p.c, p.deal));
+        if (run >= deal.runs) return;
+        pos = deal.begin(run);
+        end = deal.begin(run + 1);
+    }
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    char* staging = sh.rows + wave * kWave;
+
+    while (pos < end) {
+        const Item it = item_at(parameters().t, pos, end);
+        const int64_t b = it.b;
+        const int cached = (it.n + kFewRows - 1) / kFewRows;
+        const int stop = max(it.t0, min(it.t1, cached));                 // tiles [t0, stop) of the cache
+        __syncthreads();                                                 // the item before is done with LDS
+        if (threadIdx.x == 0) sh.wild = 0;
+        __syncthreads();
+        u32x4 qr[NT][KS];
+        load_queries<KS, NT, true>(parameters().t, b, it.h, 0, qr);
+        const float scale_log2 = parameters().t.scale_log2;
+
+        Softmax<NT, kUnit, MD, F16> x;
+        x.clear();
+
         struct Unit {
             Group<D> x[kUnit];
-        };
-        auto load = [&](int t, Unit& unit) {
-#pragma unroll
-            for (int u = 0; u < kUnit; ++u) {
-                const int row = row_of(t, u);
-                loader.load(z, loader.entry(z, row), row, unit.x[u]);
-            }
         };
         auto compute = [&](int t, Unit& unit) {
             const int left = it.n - (t * kFewRows + wave * kUnit * 16);
@@ -233,38 +300,52 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
             if (left < kUnit * 16) {
 #pragma unroll
                 for (int u = 0; u < kUnit; ++u) {
-                    drop_scales<D>(unit.x[u], left - 16 * u);
+                    drop_scales<D>(unit.x[u].vs, left - 16 * u);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[nt][u][i] = 16 * u + 4 * grp + i < left ? s[nt][u][i] : kNegInf;
                 }
             }
+            x.move(s, scale_log2);
             u32x4 pb[kUnit / 2][NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                softmax_step<kUnit, MD, F16>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
-#pragma unroll
-                for (int ss = 0; ss < kUnit / 2; ++ss)
-                    pb[ss][nt] =
-                        u32x4{E::pack(s[nt][2 * ss][0], s[nt][2 * ss][1]), E::pack(s[nt][2 * ss][2], s[nt][2 * ss][3]),
-                              E::pack(s[nt][2 * ss + 1][0], s[nt][2 * ss + 1][1]),
-                              E::pack(s[nt][2 * ss + 1][2], s[nt][2 * ss + 1][3])};
-            }
+            x.weigh(s, pb);
 #pragma unroll
             for (int ss = 0; ss < kUnit / 2; ++ss) {
-                u32x2 lo[MD], hi[MD];
-                value_values<D, F16>(unit.x[2 * ss], lo);
-                value_values<D, F16>(unit.x[2 * ss + 1], hi);
 #pragma unroll
-                for (int md = 0; md < MD; ++md)
+                for (int pr = 0; pr < MD / 2; ++pr) {
+                    u32x2 lo[2], hi[2];
+                    value_values<D, F16>(unit.x[2 * ss].v, unit.x[2 * ss].vs, pr, lo);
+                    value_values<D, F16>(unit.x[2 * ss + 1].v, unit.x[2 * ss + 1].vs, pr, hi);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        o[nt][md] = E::mma32(u32x4{lo[md].x, lo[md].y, hi[md].x, hi[md].y}, pb[ss][nt], o[nt][md]);
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            x.o[nt][2 * pr + i] = E::mma32(u32x4{lo[i].x, lo[i].y, hi[i].x, hi[i].y}, pb[ss][nt], x.o[nt][2 * pr + i]);
+                }
             }
         };
 
         if (it.t0 < stop) {
+            const PoolView& z = parameters().z;
+            GroupLoader<D> loader(z, b, it.h);
+            const GroupOffsets<D> off;
+            // the wave's groups of 16 tiles from `base` on, one a lane; those past the last group again the last one
+            const int last_row = (it.n - 1) & ~15;
+            int base = it.t0;
+            auto row_of = [&](int from) { return min((from + lane / kUnit) * kFewRows + (wave * kUnit + lane % kUnit) * 16, last_row); };
+            loader.places.ask(z, row_of(base));
+            loader.places.take(z, row_of(base));
+            loader.places.ask(z, row_of(base + 64 / kUnit));
+            auto load = [&](int t, Unit& unit) {
+                if (t >= base + 64 / kUnit) {
+                    base += 64 / kUnit;
+                    loader.places.take(z, row_of(base));
+                    loader.places.ask(z, row_of(base + 64 / kUnit));
+                }
+#pragma unroll
+                for (int u = 0; u < kUnit; ++u) loader.load(off, (t - base) * kUnit + u, unit.x[u]);
+            };
             Unit even, odd;
             load(it.t0, even);
             for (int t = it.t0;;) {
@@ -277,6 +358,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
             }
         }
 
+        const TreeParams& p = parameters().t;
         // the drafted tokens, 16 a wave
         for (int t = stop; t < it.t1; ++t) {
             const int first = (t - cached) * kKeys, key0 = first + 16 * wave;
@@ -296,24 +378,24 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
                 for (int kk = 0; kk < KS; ++kk) s[0] = E::mma32(key_operand<D, true>(staging, kk), qr[nt][kk], s[0]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[0][i] = bits >> i & 1u ? s[0][i] : kNegInf;
-                softmax_step<1, MD, F16>(s, p.scale_log2, m[nt], l[nt], o[nt]);
+                softmax_step<1, MD, F16>(s, scale_log2, x.m[nt], x.l[nt], x.o[nt]);
                 const u32x2 pb = {E::pack(s[0][0], s[0][1]), E::pack(s[0][2], s[0][3])};
 #pragma unroll
                 for (int md = 0; md < MD; ++md)
-                    o[nt][md] = E::mma16(value_operand<D>(staging + R::kBytes, md), pb, o[nt][md]);
+                    x.o[nt][md] = E::mma16(value_operand<D>(staging + R::kBytes, md), pb, x.o[nt][md]);
             }
             wave_fence();
         }
 
         __syncthreads();
-        join_keys<MD, NT, 4>(reinterpret_cast<float*>(sh.rows), kRows, 0, wave, m, l, o);
+        join_keys<MD, NT, 4>(reinterpret_cast<float*>(sh.rows), kRows, 0, wave, x.m, x.l, x.o);
         if (wave == 0) {
             float* part = p.part + (2 * (int64_t)run + (it.t0 == 0)) * kPart;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int row = 16 * nt + col;
-                if (sh.wild) add_unbounded<MD, F16>(p, b, it.h, 0, p.T, row, o[nt]);
-                finish_rows<MD, F16>(p, b, it.h, row, row, kRows, it.t0 == 0 && it.t1 == it.tiles, part, m[nt], l[nt], o[nt]);
+                if (sh.wild) add_unbounded<MD, F16>(p, b, it.h, 0, p.T, row, x.o[nt]);
+                finish_rows<MD, F16>(p, b, it.h, row, row, kRows, it.t0 == 0 && it.t1 == it.tiles, part, x.m[nt], x.l[nt], x.o[nt]);
             }
         }
         pos += it.t1 - it.t0;
@@ -321,16 +403,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
 }
 
 // ---------------------------------------------------------------------------
-// more than 32 query rows a KV head: bound by the matrix cores
+// more than 32 query rows a KV head
 // ---------------------------------------------------------------------------
 
-// Four waves share a tile of 64 rows.  Each turns one group of 16 into operands
-// and leaves them in LDS in the order in which lanes take them (16 bytes a lane side
-// by side: no bank is asked twice), two tiles side by side.
+// Four waves share tiles of 64 rows: RW of them side by side on the query rows, 32
+// each, 4 / RW on a tile's keys.  Each wave turns one group of 16 rows into
+// operands and leaves them in LDS in the order in which lanes take them (16 bytes a
+// lane side by side: no bank is asked twice), two tiles side by side.
 template <int D, bool F16, int RW>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) quant_many_kernel(QuantParams qp) {
-    const TreeParams& p = qp.t;
-    const PoolView& z = qp.z;
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) quant_many_kernel(QuantParams) {
     using R = Rows16<D>;
     using E = Elem<F16>;
     constexpr int NT = 2, KS = D / 32, MD = D / 16;
@@ -339,152 +420,230 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
     constexpr int kTile = 8 * R::kBytes, kApart = 4 * R::kBytes;
     constexpr int kJoin = KW > 1 ? 4 * (KW - 1) * kPart : 0;
     constexpr int kBytes = 2 * kTile > kJoin ? 2 * kTile : kJoin;
-    __shared__ QuantLds<kBytes, 16 * NT> sh;
+    __shared__ QuantLds<kBytes, 4, 16 * NT> sh;
     char* lds = sh.rows;
 
-    const int slot = slot_of_block();
-    const int run = (uint32_t)slot / (uint32_t)p.row_blocks, rb = slot - run * p.row_blocks;
-    const Deal deal(p.deal, total_tiles(p.c, p.deal));
-    if (run >= deal.runs) return;
-    int pos = deal.begin(run);
-    const int end = deal.begin(run + 1);
-
+    int pos, end, slot;
+    {
+        const TreeParams& p = parameters().t;
+        slot = slot_of_block();
+        const int run = (uint32_t)slot / (uint32_t)p.row_blocks;
+        const Deal deal(p.deal, total_tiles(p.c, p.deal));
+        if (run >= deal.runs) return;
+        pos = deal.begin(run);
+        end = deal.begin(run + 1);
+    }
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int rw = wave % RW, kw = wave / RW;
-    const int row0 = rb * kRows + rw * 16 * NT;           // the wave's first query row
     const int key0 = kw * 16 * MT;                        // the wave's first key in a tile
-    GroupLoader<D> loader;
 
     while (pos < end) {
-        const Item it = item_at(p, pos, end);
+        const Item it = item_at(parameters().t, pos, end);
         const int64_t b = it.b;
         const int cached = (it.n + kKeys - 1) / kKeys;
         const int stop = max(it.t0, min(it.t1, cached));
-        loader.item(z, b, it.h);
         __syncthreads();                                   // the item before is done with LDS
         if (threadIdx.x == 0) sh.wild = 0;
+        int row0;                                          // the wave's first query row
+        bool idle;                                         // past the last one: this wave makes operands only
         u32x4 qr[NT][KS];
-        load_queries<KS, NT, true>(p, b, it.h, row0, qr);
-        v4f o[NT][MD];
-        float m[NT], l[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            m[nt] = kNegInf;
-            l[nt] = 0.f;
-#pragma unroll
-            for (int md = 0; md < MD; ++md) o[nt][md] = v4f{0.f, 0.f, 0.f, 0.f};
+        float scale_log2;
+        {
+            const TreeParams& p = parameters().t;
+            row0 = (slot - (uint32_t)slot / (uint32_t)p.row_blocks * p.row_blocks) * kRows + rw * 16 * NT;
+            idle = row0 >= p.M;
+            load_queries<KS, NT, true>(p, b, it.h, row0, qr);
+            scale_log2 = p.scale_log2;
         }
+        Softmax<NT, MT, MD, F16> x;
+        x.clear();
 
-        // the wave's group of tile t: asked for, and left in LDS as operands
-        Group<D> raw;
-        const int last_row = (it.n - 1) & ~15;
-        auto fetch = [&](int t) {
-            const int row = min(t * kKeys + 16 * wave, last_row);
-            loader.load(z, loader.entry(z, row), row, raw);
-        };
-        auto put = [&](int t) {
-            char* tile = lds + (t & 1) * kTile;
-            drop_scales<D>(raw, it.n - (t * kKeys + 16 * wave));
+        // scores, softmax and values of the wave's keys; the operands by key(mt, kk) and value(ss, md), unseen scores by
+        // hide
+        auto attend = [&](auto key, auto value, auto hide) {
+            v4f s[NT][MT];
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk)
-                *reinterpret_cast<u32x4*>(tile + (wave * KS + kk) * 1024 + 16 * lane) = key_values<D, F16>(raw, kk);
-            u32x2 v[MD];
-            value_values<D, F16>(raw, v);
-#pragma unroll
-            for (int md = 0; md < MD; ++md)
-                *reinterpret_cast<u32x2*>(tile + kApart + ((wave >> 1) * MD + md) * 1024 + 16 * lane + 8 * (wave & 1)) = v[md];
-        };
-
-        // the wave's MT groups of 16 keys: scores, softmax, values; the operands by key(mt, kk) and value(ss, md)
-        auto scores = [&](auto key, v4f(&s)[NT][MT]) {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[nt][mt] = v4f{0.f, 0.f, 0.f, 0.f};
-            u32x4 a[KS][MT];                               // two steps' rows asked for ahead of their products
-            auto read = [&](int kk) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) a[kk][mt] = key(mt, kk);
-            };
-            read(0);
-            read(1);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int kk = 0; kk < KS; ++kk) {
+                    const u32x4 a = key(mt, kk);
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                if (kk + 2 < KS) read(kk + 2);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) s[nt][mt] = E::mma32(a[kk][mt], qr[nt][kk], s[nt][mt]);
-                __builtin_amdgcn_sched_barrier(0);
+                    for (int nt = 0; nt < NT; ++nt) s[nt][mt] = E::mma32(a, qr[nt][kk], s[nt][mt]);
+                }
             }
-        };
-        auto softmax = [&](v4f(&s)[NT][MT], u32x4(&pb)[MT / 2][NT]) {
+            hide(s);
+            x.move(s, scale_log2);
+            u32x4 pb[MT / 2][NT];
+            x.weigh(s, pb);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                softmax_step<MT, MD, F16>(s[nt], p.scale_log2, m[nt], l[nt], o[nt]);
+            for (int ss = 0; ss < MT / 2; ++ss)
 #pragma unroll
-                for (int ss = 0; ss < MT / 2; ++ss)
-                    pb[ss][nt] =
-                        u32x4{E::pack(s[nt][2 * ss][0], s[nt][2 * ss][1]), E::pack(s[nt][2 * ss][2], s[nt][2 * ss][3]),
-                              E::pack(s[nt][2 * ss + 1][0], s[nt][2 * ss + 1][1]),
-                              E::pack(s[nt][2 * ss + 1][2], s[nt][2 * ss + 1][3])};
-            }
-        };
-        auto values = [&](auto value, const u32x4(&pb)[MT / 2][NT]) {
-            constexpr int kGroups = MT / 2 * MD / 4;       // four 16-column operands a group, one group ahead
-            u32x4 a[kGroups][4];
-            auto read = [&](int g) {
-                const int ss = g / (MD / 4), m0 = g % (MD / 4) * 4;
+                for (int md = 0; md < MD; ++md) {
+                    const u32x4 a = value(ss, md);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[g][i] = value(ss, m0 + i);
-            };
-            read(0);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                const int ss = g / (MD / 4), m0 = g % (MD / 4) * 4;
-                if (g + 1 < kGroups) read(g + 1);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) o[nt][m0 + i] = E::mma32(a[g][i], pb[ss][nt], o[nt][m0 + i]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                    for (int nt = 0; nt < NT; ++nt) x.o[nt][md] = E::mma32(a, pb[ss][nt], x.o[nt][md]);
+                }
         };
 
         if (it.t0 < stop) {
-            fetch(it.t0);
-            put(it.t0);
-            if (it.t0 + 1 < stop) fetch(it.t0 + 1);
-        }
-        __syncthreads();
-        for (int t = it.t0; t < stop; ++t) {
-            if (t + 1 < stop) put(t + 1);
-            if (t + 2 < stop) fetch(t + 2);
-            const char* tile = lds + (t & 1) * kTile;
-            v4f s[NT][MT];
-            u32x4 pb[MT / 2][NT];
-            scores([&](int mt, int kk) {
-                return *reinterpret_cast<const u32x4*>(tile + ((kw * MT + mt) * KS + kk) * 1024 + 16 * lane);
-            }, s);
-            const int left = it.n - t * kKeys - key0;
-            if (left < 16 * MT) {
+            const PoolView& z = parameters().z;
+            GroupLoader<D> loader(z, b, it.h);
+            const GroupOffsets<D> off;
+            // the wave's groups of 64 tiles from `base` on, one a lane; those past the last group again the last one
+            const int last_row = (it.n - 1) & ~15, last = stop - 1;
+            int base = it.t0;
+            auto row_of = [&](int from) { return min((from + lane) * kKeys + 16 * wave, last_row); };
+            loader.places.ask(z, row_of(base));
+            loader.places.take(z, row_of(base));
+            loader.places.ask(z, row_of(base + 64));
+            auto fetch = [&](int t, Group<D>& raw) {
+                if (t >= base + 64) {
+                    base += 64;
+                    loader.places.take(z, row_of(base));
+                    loader.places.ask(z, row_of(base + 64));
+                }
+                loader.load(off, t - base, raw);
+            };
+            // pieces of the work of turning a group into operands
+            auto put_key = [&](char* tile, const Group<D>& raw, int kk) {
+                *reinterpret_cast<u32x4*>(tile + (wave * KS + kk) * 1024) = key_values<D, F16>(raw, kk);
+            };
+            auto put_values = [&](char* tile, const Group<D>& raw, int pr) {
+                u32x2 v[2];
+                value_values<D, F16>(raw.v, raw.vs, pr, v);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int i = 0; i < 2; ++i)
+                    *reinterpret_cast<u32x2*>(tile + kApart + ((wave >> 1) * MD + 2 * pr + i) * 1024 + 8 * (wave & 1)) = v[i];
+            };
+            auto put = [&](int t, Group<D>& raw) {
+                char* tile = lds + (t & 1) * kTile + 16 * lane;
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                for (int kk = 0; kk < KS; ++kk) put_key(tile, raw, kk);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[nt][mt][i] = 16 * mt + 4 * grp + i < left ? s[nt][mt][i] : kNegInf;
-            }
-            softmax(s, pb);
-            values([&](int ss, int md) {
-                return *reinterpret_cast<const u32x4*>(tile + kApart + ((kw * (MT / 2) + ss) * MD + md) * 1024 + 16 * lane);
-            }, pb);
+                for (int pr = 0; pr < D / 32; ++pr) put_values(tile, raw, pr);
+            };
+            auto drop_behind = [&](int t, Group<D>& raw) {
+                const int left = it.n - (t * kKeys + 16 * wave);
+                if (left < 16) drop_scales<D>(raw.vs, left);
+            };
+            // Tile t, and beside it the operands of tile t + 1 (behind the last tile: nobody reads them).  A matrix product
+            // leaves half of its time to other instructions of its wave, and waves hardly share a SIMD's time otherwise
+            // (32 products and 128 other instructions a wave, one after the other, two waves: 1002 clocks each; mixed
+            // by fours: 837): so each step has two products, a read for a product to come and a piece of other work.
+            auto tile_step = [&](int t, Group<D>& raw) {
+                char* to = lds + ((t + 1) & 1) * kTile + 16 * lane;
+                const char* tile = lds + (t & 1) * kTile + 16 * lane;
+                constexpr int kAhead = 4;
+                u32x4 a[kAhead];
+                // the softmax of one workgroup's wave goes before the scores of the other's, which wait for LDS and the
+                // matrix cores more (26 tokens 261 us without, 254 with; 63 tokens 254 / 238)
+                __builtin_amdgcn_s_setprio(0);
+                v4f s[NT][MT];
+                auto key = [&](int i) {
+                    return *reinterpret_cast<const u32x4*>(tile + ((kw * MT + i / KS) * KS + i % KS) * 1024);
+                };
+                auto value = [&](int i) {
+                    return *reinterpret_cast<const u32x4*>(tile + kApart + ((kw * (MT / 2) + i / MD) * MD + i % MD) * 1024);
+                };
+                constexpr int kScores = MT * KS, kValues = MT / 2 * MD;
+                drop_behind(t + 1, raw);
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) a[i] = key(i);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < kScores; ++i) {
+                    const int mt = i / KS, kk = i % KS;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        s[nt][mt] = E::mma32(a[i % kAhead], qr[nt][kk], kk == 0 ? v4f{0.f, 0.f, 0.f, 0.f} : s[nt][mt]);
+                    if (i + kAhead < kScores) a[i % kAhead] = key(i + kAhead);
+                    constexpr int kEach = kScores / (D / 32);
+                    if (i % kEach == 0) put_values(to, raw, i / kEach);
+                    if (i % 2) __builtin_amdgcn_sched_barrier(0);
+                }
+                __builtin_amdgcn_s_setprio(3);
+                const int left = it.n - t * kKeys - key0;
+                if (left < 16 * MT) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[nt][mt][i] = 16 * mt + 4 * grp + i < left ? s[nt][mt][i] : kNegInf;
+                }
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) a[i] = value(i);
+                x.move(s, scale_log2);
+                u32x4 pb[MT / 2][NT];
+                float sum[NT];
+                // the weights of two groups of 16 keys, 4 NT pairs of them
+                auto weigh = [&](int ss, int piece) {
+                    const int nt = piece % NT, j = piece / NT;
+                    pb[ss][nt][j] = x.weigh(nt, s[nt][2 * ss + j / 2][2 * (j & 1)], s[nt][2 * ss + j / 2][2 * (j & 1) + 1], sum[nt]);
+                };
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) sum[nt] = 0.f;
+#pragma unroll
+                for (int piece = 0; piece < 4 * NT; ++piece) weigh(0, piece);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < kValues; ++i) {
+                    const int ss = i / MD, md = i % MD;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) x.o[nt][md] = E::mma32(a[i % kAhead], pb[ss][nt], x.o[nt][md]);
+                    if (i + kAhead < kValues) a[i % kAhead] = value(i + kAhead);
+                    // the weights of the next groups beside the values of these, K's operands beside the last
+                    if (ss + 1 < MT / 2) {
+                        constexpr int kEach = 4 * NT / MD;
+#pragma unroll
+                        for (int e = 0; e < kEach; ++e) weigh(ss + 1, kEach * md + e);
+                    } else if (md % 2 == 0 && md / 2 < KS) {
+                        put_key(to, raw, md / 2);
+                    }
+                    if (i % 2) __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) x.l[nt] += sum[nt];
+            };
+            // a tile's codes are asked for three tiles before they are worked on and become operands one before
+            Group<D> raw[2];
+            fetch(it.t0, raw[0]);
+            fetch(min(it.t0 + 1, last), raw[1]);
+            drop_behind(it.t0, raw[0]);
+            put(it.t0, raw[0]);
+            fetch(min(it.t0 + 2, last), raw[0]);
             __syncthreads();
+            if (idle) {
+                for (int t = it.t0;;) {
+                    drop_behind(t + 1, raw[1]);
+                    put(t + 1, raw[1]);
+                    fetch(min(t + 3, last), raw[1]);
+                    __syncthreads();
+                    if (++t >= stop) break;
+                    drop_behind(t + 1, raw[0]);
+                    put(t + 1, raw[0]);
+                    fetch(min(t + 3, last), raw[0]);
+                    __syncthreads();
+                    if (++t >= stop) break;
+                }
+            } else {
+                for (int t = it.t0;;) {
+                    tile_step(t, raw[1]);
+                    fetch(min(t + 3, last), raw[1]);
+                    __syncthreads();
+                    if (++t >= stop) break;
+                    tile_step(t, raw[0]);
+                    fetch(min(t + 3, last), raw[0]);
+                    __syncthreads();
+                    if (++t >= stop) break;
+                }
+            }
         }
         // the drafted tokens
+        const TreeParams& p = parameters().t;
         for (int t = stop; p.dk && t < it.t1; ++t) {
             const int first = (t - cached) * kKeys;
             __syncthreads();
@@ -497,37 +656,37 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
             }
             __syncthreads();
             const char* ks = lds + kw * MT * R::kBytes;
-            v4f s[NT][MT];
-            u32x4 pb[MT / 2][NT];
-            scores([&](int mt, int kk) { return key_operand<D, true>(ks + mt * R::kBytes, kk); }, s);
-            const int from = min(row0, p.M - 1) / p.G;
+            if (!idle)
+                attend([&](int mt, int kk) { return key_operand<D, true>(ks + mt * R::kBytes, kk); },
+                       [&](int ss, int md) {
+                           const u32x2 lo = value_operand<D>(ks + kApart + 2 * ss * R::kBytes, md);
+                           const u32x2 hi = value_operand<D>(ks + kApart + (2 * ss + 1) * R::kBytes, md);
+                           return u32x4{lo.x, lo.y, hi.x, hi.y};
+                       },
+                       [&](v4f(&s)[NT][MT]) {
+                           const int from = min(row0, p.M - 1) / p.G;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const uint64_t word = sh.seen[wave][min(row0 + 16 * nt + col, p.M - 1) / p.G - from] >> (key0 + 4 * grp);
+                           for (int nt = 0; nt < NT; ++nt) {
+                               const uint64_t word =
+                                   sh.seen[wave][min(row0 + 16 * nt + col, p.M - 1) / p.G - from] >> (key0 + 4 * grp);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                               for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nt][mt][i] = word >> (16 * mt + i) & 1 ? s[nt][mt][i] : kNegInf;
-            }
-            softmax(s, pb);
-            values([&](int ss, int md) {
-                const u32x2 lo = value_operand<D>(ks + kApart + 2 * ss * R::kBytes, md);
-                const u32x2 hi = value_operand<D>(ks + kApart + (2 * ss + 1) * R::kBytes, md);
-                return u32x4{lo.x, lo.y, hi.x, hi.y};
-            }, pb);
+                                   for (int i = 0; i < 4; ++i) s[nt][mt][i] = word >> (16 * mt + i) & 1 ? s[nt][mt][i] : kNegInf;
+                           }
+                       });
         }
         __syncthreads();
 
-        join_keys<MD, NT, KW>(reinterpret_cast<float*>(lds), kRows, rw * 16 * NT, kw, m, l, o);
+        join_keys<MD, NT, KW>(reinterpret_cast<float*>(lds), kRows, rw * 16 * NT, kw, x.m, x.l, x.o);
         if (kw == 0) {
             float* part = p.part + (2 * (int64_t)slot + (it.t0 == 0)) * kPart;
             const int j0 = max(0, it.t0 - cached) * kKeys, j1 = min(p.T, max(0, it.t1 - cached) * kKeys);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const int in = rw * 16 * NT + 16 * nt + col, row = rb * kRows + in;
-                if (sh.wild) add_unbounded<MD, F16>(p, b, it.h, j0, j1, row, o[nt]);
-                finish_rows<MD, F16>(p, b, it.h, row, in, kRows, it.t0 == 0 && it.t1 == it.tiles, part, m[nt], l[nt],
-                                     o[nt]);
+                const int in = rw * 16 * NT + 16 * nt + col, row = row0 + 16 * nt + col;
+                if (sh.wild) add_unbounded<MD, F16>(p, b, it.h, j0, j1, row, x.o[nt]);
+                finish_rows<MD, F16>(p, b, it.h, row, in, kRows, it.t0 == 0 && it.t1 == it.tiles, part, x.m[nt], x.l[nt], x.o[nt]);
             }
         }
         pos += it.t1 - it.t0;
@@ -609,7 +768,7 @@ extern "C" int slimkv_quantized_attention(const slimkv_quantized_attention_args*
     p.B = (int)B; p.T = (int)T; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk);
     p.M = p.T * p.G;
     p.row_blocks = plan.row_blocks;
-    const int tile = plan.rw == 1 ? kFewRows : kKeys;
+    const int tile = plan.rw == 1 ? 64 * few_groups(plan.nt) : kKeys;
     // without drafted tokens a tile without work, so that a sequence without rows has a run that writes its output
     p.deal = Dealing{p.B, p.Hk, tile, draft ? (p.T + kKeys - 1) / kKeys : 1, plan.runs};
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
