@@ -125,6 +125,7 @@ typedef struct slimkv_quantized_attention_args {
     int32_t dtype;
 } slimkv_quantized_attention_args;
 
+/* By the sizes of the call, `keys` among them. */
 size_t slimkv_quantized_attention_workspace(const slimkv_quantized_attention_args* a);
 int slimkv_quantized_attention(const slimkv_quantized_attention_args* a, void* workspace, size_t workspace_bytes,
                                void* stream);

@@ -27,6 +27,7 @@ namespace {
 struct QuantParams {
     TreeParams t;
     PoolView z;
+    int alone;                        // a run is one item, whole
 };
 
 // The kernel's arguments, read where they are used: kept in scalar registers
@@ -36,6 +37,35 @@ __device__ __forceinline__ const QuantParams& parameters() {
     asm volatile("" : "+s"(args));
     return *(const QuantParams*)args;
 }
+
+// The tiles that a workgroup has to work on: item by item.
+struct Share {
+    int pos, end;
+    bool alone;
+
+    // False: none.
+    __device__ __forceinline__ bool take(const QuantParams& q, int run) {
+        alone = q.alone;
+        pos = run;
+        end = run + 1;
+        if (alone) return run < q.t.B * q.t.Hk;
+        const Deal deal(q.t.deal, total_tiles(q.t.c, q.t.deal));
+        pos = deal.begin(run);
+        end = deal.begin(run + 1);
+        return run < deal.runs;
+    }
+    __device__ __forceinline__ Item item(const TreeParams& p) const {
+        if (!alone) return item_at(p, pos, end);
+        Item it;
+        it.b = (uint32_t)pos / (uint32_t)p.Hk;
+        it.h = pos - (int)it.b * p.Hk;
+        it.n = uniform(cache_length(p.c, it.b));
+        it.tiles = it.t1 = item_tiles(p.deal, it.n);
+        it.t0 = 0;
+        return it;
+    }
+    __device__ __forceinline__ void done(const Item& it) { pos += alone ? 1 : it.t1 - it.t0; }
+};
 
 // 16 rows of K and V as a lane holds them: K of row `col`, elements D / 4 grp on;
 // V of rows 4 grp .. 4 grp + 3, columns col + 16 md; their scales.
@@ -252,20 +282,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
     __shared__ QuantLds<kBytes, 4, kRows> sh;
 
     const int run = slot_of_block();
-    int pos, end;
-    {
-        const TreeParams& p = parameters().t;
-        const Deal deal(p.deal, total_tiles(p.c, p.deal));
-        if (run >= deal.runs) return;
-        pos = deal.begin(run);
-        end = deal.begin(run + 1);
-    }
+    Share share;
+    if (!share.take(parameters(), run)) return;
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     char* staging = sh.rows + wave * kWave;
 
-    while (pos < end) {
-        const Item it = item_at(parameters().t, pos, end);
+    while (share.pos < share.end) {
+        const Item it = share.item(parameters().t);
         const int64_t b = it.b;
         const int cached = (it.n + kFewRows - 1) / kFewRows;
         const int stop = max(it.t0, min(it.t1, cached));                 // tiles [t0, stop) of the cache
@@ -398,7 +422,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
                 finish_rows<MD, F16>(p, b, it.h, row, row, kRows, it.t0 == 0 && it.t1 == it.tiles, part, x.m[nt], x.l[nt], x.o[nt]);
             }
         }
-        pos += it.t1 - it.t0;
+        share.done(it);
     }
 }
 
@@ -423,23 +447,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
     __shared__ QuantLds<kBytes, 4, 16 * NT> sh;
     char* lds = sh.rows;
 
-    int pos, end, slot;
+    const int slot = slot_of_block();
+    Share share;
     {
-        const TreeParams& p = parameters().t;
-        slot = slot_of_block();
-        const int run = (uint32_t)slot / (uint32_t)p.row_blocks;
-        const Deal deal(p.deal, total_tiles(p.c, p.deal));
-        if (run >= deal.runs) return;
-        pos = deal.begin(run);
-        end = deal.begin(run + 1);
+        const QuantParams& q = parameters();
+        if (!share.take(q, (uint32_t)slot / (uint32_t)q.t.row_blocks)) return;
     }
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int rw = wave % RW, kw = wave / RW;
     const int key0 = kw * 16 * MT;                        // the wave's first key in a tile
 
-    while (pos < end) {
-        const Item it = item_at(parameters().t, pos, end);
+    while (share.pos < share.end) {
+        const Item it = share.item(parameters().t);
         const int64_t b = it.b;
         const int cached = (it.n + kKeys - 1) / kKeys;
         const int stop = max(it.t0, min(it.t1, cached));
@@ -689,7 +709,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
                 finish_rows<MD, F16>(p, b, it.h, row, in, kRows, it.t0 == 0 && it.t1 == it.tiles, part, x.m[nt], x.l[nt], x.o[nt]);
             }
         }
-        pos += it.t1 - it.t0;
+        share.done(it);
     }
 }
 
@@ -707,17 +727,40 @@ int check_attention(const slimkv_quantized_attention_args* a) {
     return SLIMKV_OK;
 }
 
-int64_t query_rows(const slimkv_quantized_attention_args* a) { return a->tokens * (a->heads / a->kv_heads); }
+// Short items are worked on whole, by one workgroup each, with nothing to merge and one launch less: caches of up
+// to 1024 rows (512 with more than 32 query rows), and twice that where 64 workgroups or more have an item.  Times in
+// a graph, dealt and merged / whole: one token over 512 rows 11.3 / 9.6 us, 1024 12.8 / 11.9, 1536 12.9 / 14.3; of 16
+// sequences 1024 20.1 / 12.4, 2048 20.6 / 18.4; 26 tokens over 512 rows 20.9 / 20.7, 768 20.8 / 25.5; of 8 sequences
+// 1024 46.6 / 31.4, 2048 51.5 / 52.1.
+struct QuantPlan : TreePlan {
+    int tile;                                      // cache rows of a tile
+    bool alone;
+    size_t bytes(int64_t D) const { return alone ? 0 : TreePlan::bytes(D); }
+};
+
+QuantPlan plan_attention(const slimkv_quantized_attention_args* a) {
+    QuantPlan t{};
+    static_cast<TreePlan&>(t) = plan_tree(a->tokens * (a->heads / a->kv_heads));
+    t.tile = t.rw == 1 ? 64 * few_groups(t.nt) : kKeys;
+    const int64_t items = a->batch * a->kv_heads;
+    const int64_t workgroups = items * t.row_blocks;
+    t.alone = a->keys <= (t.rw == 1 ? 1024 : 512) * (workgroups >= 64 ? 2 : 1) && workgroups <= 65536;
+    if (t.alone) {
+        t.runs = (int)items;
+        t.slots = workgroups;
+    }
+    return t;
+}
 
 template <int D, bool F16>
-void launch_attention(const QuantParams& p, const TreePlan& plan, hipStream_t st) {
+void launch_attention(const QuantParams& p, const QuantPlan& plan, hipStream_t st) {
     const dim3 grid((unsigned)((plan.slots + kXcdCount - 1) / kXcdCount * kXcdCount));
     void (*kernel)(QuantParams) = plan.rw == 4   ? quant_many_kernel<D, F16, 4>
                                   : plan.rw == 2 ? quant_many_kernel<D, F16, 2>
                                   : plan.nt == 2 ? quant_few_kernel<D, F16, 2>
                                                  : quant_few_kernel<D, F16, 1>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p);
-    launch_merge<D, F16>(p.t, plan, st);
+    if (!plan.alone) launch_merge<D, F16>(p.t, plan, st);
 }
 
 }  // namespace
@@ -728,7 +771,7 @@ using namespace slimkv;
 
 extern "C" size_t slimkv_quantized_attention_workspace(const slimkv_quantized_attention_args* a) {
     if (check_attention(a) != SLIMKV_OK) return 0;
-    return std::max<size_t>(plan_tree(query_rows(a)).bytes(a->head_dim), 16);
+    return std::max<size_t>(plan_attention(a).bytes(a->head_dim), 16);
 }
 
 extern "C" int slimkv_quantized_attention(const slimkv_quantized_attention_args* a, void* workspace,
@@ -754,8 +797,9 @@ extern "C" int slimkv_quantized_attention(const slimkv_quantized_attention_args*
     for (int64_t s : {a->dk_sn, a->dv_sn})
         if (draft && T > 1 && (s < D || s >= (1 << 23)))
             return fail(SLIMKV_EUNSUP, "quantized attention: drafted rows must lie [head_dim, 2^23) elements apart");
-    const TreePlan plan = plan_tree(query_rows(a));
-    if (!plan.whole() &&
+    const QuantPlan plan = plan_attention(a);
+    const bool merges = !plan.alone && !plan.whole();
+    if (merges &&
         (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes(D)))
         return fail(SLIMKV_EWORKSPACE, "quantized attention: workspace missing, misaligned or too small");
     p.c.lengths = a->lengths; p.c.keys = (int)a->keys;
@@ -768,12 +812,12 @@ extern "C" int slimkv_quantized_attention(const slimkv_quantized_attention_args*
     p.B = (int)B; p.T = (int)T; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk);
     p.M = p.T * p.G;
     p.row_blocks = plan.row_blocks;
-    const int tile = plan.rw == 1 ? 64 * few_groups(plan.nt) : kKeys;
+    qp.alone = plan.alone;
     // without drafted tokens a tile without work, so that a sequence without rows has a run that writes its output
-    p.deal = Dealing{p.B, p.Hk, tile, draft ? (p.T + kKeys - 1) / kKeys : 1, plan.runs};
+    p.deal = Dealing{p.B, p.Hk, plan.tile, draft ? (p.T + kKeys - 1) / kKeys : 1, plan.runs};
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.part = static_cast<float*>(workspace);
-    if (B * Hk * p.M > 0x7fffffff || (!plan.whole() && !launchable(B * Hk * plan_merge(plan, B * Hk, p.M, D).chunks, 256)) ||
+    if (B * Hk * p.M > 0x7fffffff || (merges && !launchable(B * Hk * plan_merge(plan, B * Hk, p.M, D).chunks, 256)) ||
         B * Hk * ((a->keys + T) / kKeys + 2) > 0x7fffffff)
         return fail(SLIMKV_EINVAL, "quantized attention: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -32,16 +32,38 @@ or a forward-mode tangent lost, and for negative views.
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib
-from .cache_ops import (_DTYPES, _apart, _asked, _call, _common, _dtype, _folded, _lengths, _new, _overlap, _packer, _ptr,
-                        _rows16, _status)
+from .cache_ops import (_DTYPES, _asked, _call, _common, _dtype, _folded, _lengths, _new, _overlap, _packer, _ptr,
+                        _rows16, _span, _status)
 from .kernels import check_status
 
 _pack_rows = _packer(_lib.QuantizeRowsArgs)
 _pack_attention = _packer(_lib.QuantizedAttentionArgs)
 _pack_norm_rope = _packer(_lib.NormRopeArgs)
+
+
+def _device(name, *tensors):
+    """cache_ops._common in the time that it takes where nothing is refused."""
+    index = tensors[0].get_device()
+    grad = torch.is_grad_enabled()
+    if index < 0 or forward_ad._current_level >= 0:
+        return _common(name, *tensors)
+    for t in tensors:
+        if t is not None and (t.get_device() != index or t.is_neg() or grad and t.requires_grad):
+            return _common(name, *tensors)
+    return tensors[0].device
+
+
+def _clear_of(written, *read):
+    """Whether `written` shares no memory with the other tensors: most lie before or behind it as a whole."""
+    w0, w1 = _span(written)
+    for t in read:
+        if t is not None and t.data_ptr() < w1 and _span(t)[1] > w0 and _overlap(written, t):
+            return False
+    return True
 
 
 def page_bytes(block, head_dim):
@@ -57,29 +79,32 @@ def new_pages(pages, kv_heads, block, head_dim, device='cuda'):
 
 
 def _pool(name, pages, table, batch, heads, dim):
-    """A pool as the C struct's values but for the status word: (fields, rows of a sequence, the table they point
-    into)."""
-    if dim not in (64, 128):
+    """A pool as the C struct's values but for the status word: (fields, rows of a sequence, KV heads, the table they
+    point into)."""
+    if dim != 128 and dim != 64:
         raise ValueError(f'{name}: head_dim must be 64 or 128')
-    if pages.dim() != 3 or pages.dtype is not torch.uint8 or pages.stride(2) != 1 and pages.shape[2] != 1:
+    if pages.dim() != 3 or pages.dtype is not torch.uint8:
         raise ValueError(f'{name}: pages must be uint8 [pages, Hkv, bytes] with contiguous bytes')
     count, found, size = pages.shape
-    block = size // (dim + dim // 16)
-    if block == 0 or block % 16 or block * (dim + dim // 16) != size:
+    page_stride, head_stride, step = pages.stride()
+    if step != 1:
+        raise ValueError(f'{name}: pages must be uint8 [pages, Hkv, bytes] with contiguous bytes')
+    block, rest = divmod(size, dim + dim // 16)
+    if rest or block == 0 or block % 16:
         raise ValueError(f'{name}: a page of {size} bytes is no multiple of 16 rows of head_dim {dim}')
-    if heads is not None and found != heads:
+    if found != heads and heads is not None:
         raise ValueError(f'{name}: pages of {found} KV heads, rows of {heads}')
     if table is None:
         if count < batch:
             raise ValueError(f'{name}: without a block table every sequence needs a page ({batch} for {count})')
-        return (pages.data_ptr(), pages.stride(0), pages.stride(1), 0, 0, 0, count, block), block, None
+        return (pages.data_ptr(), page_stride, head_stride, 0, 0, 0, count, block), block, found, None
     if table.dtype is not torch.int64 or table.dim() != 2 or table.shape[0] != batch or table.shape[1] == 0:
         raise ValueError(f'{name}: the block table must be int64 [{batch}, cols]')
     if table.stride(1) != 1:
         table = table.contiguous()
     cols = table.shape[1]
-    return (pages.data_ptr(), pages.stride(0), pages.stride(1), table.data_ptr(), table.stride(0), cols, count,
-            block), cols * block, table
+    return (pages.data_ptr(), page_stride, head_stride, table.data_ptr(), table.stride(0), cols, count, block), \
+        cols * block, found, table
 
 
 def _whole_numbers(name, what, t, batch):
@@ -100,13 +125,13 @@ def quantize_rows(k, v, pages, table=None, *, starts=None, counts=None, status=N
         raise ValueError(f'{name}: k and v must be [B, n, Hkv, D] with contiguous features')
     B, n, H, D = k.shape
     code = _dtype(name, k, v)
-    place, rows, table = _pool(name, pages, table, B, H, D)
+    place, rows, _, table = _pool(name, pages, table, B, H, D)
     starts, counts = _whole_numbers(name, 'starts', starts, B), _whole_numbers(name, 'counts', counts, B)
-    if _folded(pages) or table is not None and _folded(table):
+    if not pages.is_contiguous() and _folded(pages) or table is not None and not table.is_contiguous() and _folded(table):
         raise ValueError(f'{name}: pages and table must not be expanded or overlapping views')
-    if not _apart((pages,), (k, v, table, starts, counts)):
+    if not _clear_of(pages, k, v, table, starts, counts):
         raise ValueError(f'{name}: pages must share no memory with the other tensors')
-    device = _common(name, k, v, pages, table, starts, counts)
+    device = _device(name, k, v, pages, table, starts, counts)
     k, v = _rows16(k), _rows16(v)
     status, owned = _status(name, status, device, table is not None or starts is not None or n > rows)
     a = _pack_rows(*place, _ptr(status), k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], _ptr(starts),
@@ -127,29 +152,35 @@ def dequantize_rows(pages, rows, head_dim, table=None, *, starts=None, counts=No
     rows, D = int(rows), int(head_dim)
     if rows < 0:
         raise ValueError(f'{name}: rows must not be negative')
-    sized = next((t for t in (table, starts, counts, pages) if t is not None))
+    sized = table if table is not None else starts if starts is not None else counts if counts is not None else pages
     B = sized.shape[0] if sized.dim() else 0
-    place, capacity, table = _pool(name, pages, table, B, None, D)
-    H = pages.shape[1]
+    place, capacity, H, table = _pool(name, pages, table, B, None, D)
     starts, counts = _whole_numbers(name, 'starts', starts, B), _whole_numbers(name, 'counts', counts, B)
     code = _DTYPES.get(dtype)
     if code is None:
         raise ValueError(f'{name}: dtype must be bfloat16 or float16')
+    shape = (B, rows, H, D)
     for t in (out_k, out_v):
-        if t is not None and (t.shape != (B, rows, H, D) or t.dtype is not dtype or t.stride(3) != 1 or _folded(t) or
-                              any(s is not None and _overlap(t, s) for s in (pages, table, starts, counts))):
-            raise ValueError(f'{name}: outputs must be {dtype} [{B}, {rows}, {H}, {D}] with contiguous features, no expanded '
-                             'views and apart from the cache and the other inputs')
+        if t is not None and (t.shape != shape or t.dtype is not dtype or t.stride(3) != 1 or _folded(t) or
+                              not _clear_of(t, pages, table, starts, counts)):
+            raise ValueError(f'{name}: outputs must be {dtype} {list(shape)} with contiguous features, no expanded views and '
+                             'apart from the cache and the other inputs')
     if out_k is not None and out_v is not None and _overlap(out_k, out_v):
         raise ValueError(f'{name}: out_k and out_v must lie apart')
-    device = _common(name, pages, table, starts, counts, out_k, out_v)
+    device = _device(name, pages, table, starts, counts, out_k, out_v)
+    row = H * D
+    dense = (rows * row, row, D, 1)
     if out_k is None:
-        out_k = torch.empty_strided((B, rows, H, D), (rows * H * D, H * D, D, 1), dtype=dtype, device=device)
+        out_k, k_strides = torch.empty_strided(shape, dense, dtype=dtype, device=device), dense
+    else:
+        k_strides = out_k.stride()
     if out_v is None:
-        out_v = torch.empty_strided((B, rows, H, D), (rows * H * D, H * D, D, 1), dtype=dtype, device=device)
+        out_v, v_strides = torch.empty_strided(shape, dense, dtype=dtype, device=device), dense
+    else:
+        v_strides = out_v.stride()
     status, owned = _status(name, status, device, table is not None or starts is not None or rows > capacity)
-    a = _pack_rows(*place, _ptr(status), out_k.data_ptr(), *out_k.stride()[:3], out_v.data_ptr(), *out_v.stride()[:3],
-                   _ptr(starts), _ptr(counts), B, rows, H, D, code)
+    a = _pack_rows(*place, _ptr(status), out_k.data_ptr(), *k_strides[:3], out_v.data_ptr(), *v_strides[:3], _ptr(starts),
+                   _ptr(counts), B, rows, H, D, code)
     _call(device, lib().slimkv_dequantize_rows, a)
     if owned:
         check_status(status)
@@ -158,9 +189,9 @@ def dequantize_rows(pages, rows, head_dim, table=None, *, starts=None, counts=No
 
 # Asked for once for each set of sizes (and the device).
 @lru_cache(1024)
-def _attention_bytes(index, B, T, Hq, H, D):
+def _attention_bytes(index, B, T, Hq, H, D, keys):
     return _asked(lib().slimkv_quantized_attention_workspace, _lib.QuantizedAttentionArgs(
-        q=16, batch=B, tokens=T, heads=Hq, kv_heads=H, head_dim=D, scale=1.0), index)
+        q=16, keys=keys, batch=B, tokens=T, heads=Hq, kv_heads=H, head_dim=D, scale=1.0), index)
 
 
 def quantized_attention(q, draft_k, draft_v, scale, pages, table=None, *, lengths=None, keys=None, mask=None, out=None,
@@ -179,8 +210,7 @@ def quantized_attention(q, draft_k, draft_v, scale, pages, table=None, *, length
     if q.dim() != 4 or pages.dim() != 3:
         raise ValueError(f'{name}: q must be [B, T, Hq, D] and pages [pages, Hkv, bytes]')
     B, T, Hq, D = q.shape
-    place, capacity, table = _pool(name, pages, table, B, None, D)
-    H = pages.shape[1]
+    place, capacity, H, table = _pool(name, pages, table, B, None, D)
     code = _dtype(name, q, draft_k, draft_v, out)
     if H == 0 or Hq % H or q.stride(3) != 1:
         raise ValueError(f'{name}: q must be [B, T, Hq, D] with Hq a multiple of {H} and contiguous features')
@@ -202,36 +232,41 @@ def quantized_attention(q, draft_k, draft_v, scale, pages, table=None, *, length
             mask = mask.contiguous()
         m = (mask.data_ptr(), mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
     inputs = (q, draft_k, draft_v, pages, table, lengths, mask)
-    if out is not None and (out.shape != q.shape or out.stride(3) != 1 or _folded(out) or
-                            any(t is not None and _overlap(out, t) for t in inputs)):
+    if out is not None and (out.shape != q.shape or out.stride(3) != 1 or _folded(out) or not _clear_of(out, *inputs)):
         raise ValueError(f'{name}: out must have the shape of q with contiguous features, no expanded view and apart '
                          'from the inputs')
     if lse is not None and (lse.shape != (B, Hq, T) or lse.dtype is not torch.float32 or not lse.is_contiguous() or
-                            any(t is not None and _overlap(lse, t) for t in (*inputs, out))):
+                            not _clear_of(lse, *inputs, out)):
         raise ValueError(f'{name}: lse must be a contiguous float32 [{B}, {Hq}, {T}], apart from the other tensors')
-    device = _common(name, *inputs, out, lse)
+    device = _device(name, *inputs, out, lse)
     q = _rows16(q)
     d = (0, 0, 0, 0, 0, 0, 0, 0)
     if draft_k is not None:
         draft_k, draft_v = _rows16(draft_k), _rows16(draft_v)
         d = (draft_k.data_ptr(), *draft_k.stride()[:3], draft_v.data_ptr(), *draft_v.stride()[:3])
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        row = Hq * D
+        o_strides = (T * row, row, D, 1)
+        out = torch.empty_strided((B, T, Hq, D), o_strides, dtype=q.dtype, device=device)
+    else:
+        o_strides = out.stride()
     if lse is None:
         lse = _new(torch.float32, device, B, Hq, T)
     status, owned = _status(name, status, device, table is not None and keys > 0)
-    nbytes = _attention_bytes(device.index, B, T, Hq, H, D)
+    nbytes = _attention_bytes(device.index, B, T, Hq, H, D, keys)
     a = _pack_attention(*place, _ptr(status), _ptr(lengths), keys, q.data_ptr(), *q.stride()[:3], *d, *m, out.data_ptr(),
-                        *out.stride()[:3], lse.data_ptr(), B, T, Hq, H, D, float(scale), code)
+                        *o_strides[:3], lse.data_ptr(), B, T, Hq, H, D, float(scale), code)
     _call(device, lib().slimkv_quantized_attention, a, nbytes)
     if owned:
         check_status(status)
     return out, lse
 
 
-def _packed16(w):
-    """w, or a copy where it is not contiguous from a 16-byte boundary."""
-    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+def _packed16(t):
+    """t, or a copy where it is not contiguous from a 16-byte boundary."""
+    if t is None or t.data_ptr() % 16 == 0 and t.is_contiguous():
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def norm_rope(q, k, cos, sin, positions, *, q_weight=None, k_weight=None, eps=1e-6, out_q=None, out_k=None,
@@ -246,53 +281,62 @@ def norm_rope(q, k, cos, sin, positions, *, q_weight=None, k_weight=None, eps=1e
     kernels.rope_decode takes the reference's bf16 steps.  A position outside the tables raises IndexError (or is left in
     `status`), its token's rows are not written.  Returns (out_q, out_k); out_q may be q itself, out_k k."""
     name = 'norm_rope'
-    if q.dim() != 4 or q.stride(3) != 1 or k is not None and (k.dim() != 4 or k.stride(3) != 1 or k.shape[:2] != q.shape[:2]
-                                                             or k.shape[3] != q.shape[3]):
-        raise ValueError(f'{name}: q must be [B, L, Hq, D] and k [B, L, Hkv, D] with contiguous features')
+    if q.dim() != 4 or q.stride(3) != 1:
+        raise ValueError(f'{name}: q must be [B, L, Hq, D] with contiguous features')
     B, L, Hq, D = q.shape
-    H = 0 if k is None else k.shape[2]
+    H = 0
+    if k is not None:
+        if k.dim() != 4 or k.stride(3) != 1 or k.shape[0] != B or k.shape[1] != L or k.shape[3] != D:
+            raise ValueError(f'{name}: with q must be k [{B}, {L}, Hkv, {D}] with contiguous features')
+        H = k.shape[2]
     code = _dtype(name, q, k, out_q, out_k)
-    if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape or \
-            cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
+    rows, width = cos.shape if cos.dim() == 2 else (0, 0)
+    if width != D or sin.shape != cos.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise ValueError(f'{name}: cos and sin must be float32 [rows, {D}]')
     if positions.dtype is not torch.int64 or positions.shape not in ((B, L), (1, L)):
         raise ValueError(f'{name}: positions must be int64 [{B}, {L}] or [1, {L}]')
+    kind = q.dtype
     for what, w in (('q_weight', q_weight), ('k_weight', k_weight)):
-        if w is not None and (w.shape != (D,) or w.dtype not in (q.dtype, torch.float32)):
-            raise ValueError(f'{name}: {what} must be [{D}] of {q.dtype} or float32')
-    kinds = {w.dtype for w in (q_weight, k_weight) if w is not None}
-    if len(kinds) > 1:
+        if w is not None:
+            if w.shape != (D,) or w.dtype not in (q.dtype, torch.float32):
+                raise ValueError(f'{name}: {what} must be [{D}] of {q.dtype} or float32')
+            kind = w.dtype
+    if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
         raise ValueError(f'{name}: q_weight and k_weight must be of one type')
     if k is None and (k_weight is not None or out_k is not None):
         raise ValueError(f'{name}: k_weight and out_k belong to keys')
-    given = [t for t in (out_q, out_k) if t is not None]
     for what, x, t in (('out_q', q, out_q), ('out_k', k, out_k)):
         if t is None:
             continue
         if t.shape != x.shape or t.stride(3) != 1 or _folded(t):
             raise ValueError(f'{name}: {what} must have the shape of its input with contiguous features, no expanded view')
         same = t.data_ptr() == x.data_ptr() and t.stride() == x.stride()
-        if any(s is not None and _overlap(t, s) for s in (q, k, cos, sin, positions, q_weight, k_weight)
-               if not (same and s is x)):
+        if not _clear_of(t, *(s for s in (q, k, cos, sin, positions, q_weight, k_weight) if not (same and s is x))):
             raise ValueError(f'{name}: {what} must be its input itself or lie apart from all inputs')
-    if len(given) == 2 and _overlap(*given):
+    if out_q is not None and out_k is not None and _overlap(out_q, out_k):
         raise ValueError(f'{name}: out_q and out_k must lie apart')
-    device = _common(name, q, k, cos, sin, positions, q_weight, k_weight, out_q, out_k)
-    q_weight, k_weight = (None if w is None else _packed16(w) for w in (q_weight, k_weight))
-    cos, sin = _packed16(cos), _packed16(sin)
-    q = _rows16(q)
-    k = None if k is None else _rows16(k)
+    device = _device(name, q, k, cos, sin, positions, q_weight, k_weight, out_q, out_k)
+    q_weight, k_weight, cos, sin = _packed16(q_weight), _packed16(k_weight), _packed16(cos), _packed16(sin)
+    q, k = _rows16(q), None if k is None else _rows16(k)
     if out_q is None:
-        out_q = torch.empty_strided((B, L, Hq, D), (L * Hq * D, Hq * D, D, 1), dtype=q.dtype, device=device)
+        row = Hq * D
+        q_strides = (L * row, row, D, 1)
+        out_q = torch.empty_strided((B, L, Hq, D), q_strides, dtype=q.dtype, device=device)
+    else:
+        q_strides = out_q.stride()
     if out_k is None and k is not None:
-        out_k = torch.empty_strided((B, L, H, D), (L * H * D, H * D, D, 1), dtype=q.dtype, device=device)
+        row = H * D
+        k_strides = (L * row, row, D, 1)
+        out_k = torch.empty_strided((B, L, H, D), k_strides, dtype=q.dtype, device=device)
+    elif k is not None:
+        k_strides = out_k.stride()
     none = (0, 0, 0, 0)
     status, owned = _status(name, status, device, True)
     a = _pack_norm_rope(q.data_ptr(), *q.stride()[:3], *(none if k is None else (k.data_ptr(), *k.stride()[:3])),
-                        _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
+                        _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), rows, positions.data_ptr(),
                         positions.stride(0) if positions.shape[0] > 1 else 0, positions.stride(1), out_q.data_ptr(),
-                        *out_q.stride()[:3], *(none if k is None else (out_k.data_ptr(), *out_k.stride()[:3])),
-                        _ptr(status), B, L, Hq, H, D, float(eps), torch.float32 in kinds, code)
+                        *q_strides[:3], *(none if k is None else (out_k.data_ptr(), *k_strides[:3])), status.data_ptr(), B, L,
+                        Hq, H, D, float(eps), kind is torch.float32, code)
     _call(device, lib().slimkv_norm_rope, a)
     if owned:
         check_status(status)
