@@ -133,11 +133,16 @@ struct GroupLoader {
         const uint8_t* base = head + page * p_sb;
         return Parts{base + (int64_t)slot * (D / 2), base + (int64_t)slot * (D / 32)};
     }
+    // ONCE: codes that no other workgroup reads are loaded non-temporal (16 sequences of 8-32K rows, one token 79.5 us
+    // without, 71.3 with; 26 tokens 202.5 / 199.8).
+    template <bool ONCE>
     __device__ __forceinline__ void load(const GroupOffsets<D>& off, int at, Group<D>& x) const {
         typedef typename Group<D>::vec vec;
         const Parts from = parts(at);
-        x.k = *reinterpret_cast<const vec*>(from.codes + off.k);
-        x.v = *reinterpret_cast<const vec*>(from.codes + v_at + off.v);
+        const vec* k = reinterpret_cast<const vec*>(from.codes + off.k);
+        const vec* v = reinterpret_cast<const vec*>(from.codes + v_at + off.v);
+        x.k = ONCE ? __builtin_nontemporal_load(k) : *k;
+        x.v = ONCE ? __builtin_nontemporal_load(v) : *v;
         x.ks = (from.scales + ks_at)[off.ks];
         x.vs = *reinterpret_cast<const vec*>(from.scales + vs_at + off.vs);
     }
@@ -368,7 +373,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
                     loader.places.ask(z, row_of(base + 64 / kUnit));
                 }
 #pragma unroll
-                for (int u = 0; u < kUnit; ++u) loader.load(off, (t - base) * kUnit + u, unit.x[u]);
+                for (int u = 0; u < kUnit; ++u) loader.template load<true>(off, (t - base) * kUnit + u, unit.x[u]);
             };
             Unit even, odd;
             load(it.t0, even);
@@ -467,12 +472,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
         if (threadIdx.x == 0) sh.wild = 0;
         int row0;                                          // the wave's first query row
         bool idle;                                         // past the last one: this wave makes operands only
+        bool once;                                         // no other block of query rows reads the codes
         u32x4 qr[NT][KS];
         float scale_log2;
         {
             const TreeParams& p = parameters().t;
             row0 = (slot - (uint32_t)slot / (uint32_t)p.row_blocks * p.row_blocks) * kRows + rw * 16 * NT;
             idle = row0 >= p.M;
+            once = p.row_blocks == 1;
             load_queries<KS, NT, true>(p, b, it.h, row0, qr);
             scale_log2 = p.scale_log2;
         }
@@ -525,7 +532,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
                     loader.places.take(z, row_of(base));
                     loader.places.ask(z, row_of(base + 64));
                 }
-                loader.load(off, t - base, raw);
+                if (once) loader.template load<true>(off, t - base, raw);
+                else loader.template load<false>(off, t - base, raw);
             };
             // pieces of the work of turning a group into operands
             auto put_key = [&](char* tile, const Group<D>& raw, int kk) {
