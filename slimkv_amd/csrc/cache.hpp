@@ -134,9 +134,10 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
 // sequence: its cache rows in tiles of `rows`, and `extra` tiles after them.  The
 // tiles of all items lie in a row, sequence by sequence and head by head, and
 // are dealt to at most `runs` workgroups in equal runs, whatever the lengths
-// are.  The host keeps their number below 2^31.
+// are.  The host keeps their number below 2^31.  With `splits` every item is cut
+// into so many runs of its own instead, item by item (the last ones may be empty).
 struct Dealing {
-    int B, Hk, rows, extra, runs;
+    int B, Hk, rows, extra, runs, splits;
 };
 
 __device__ __forceinline__ int item_tiles(const Dealing& d, int n) {

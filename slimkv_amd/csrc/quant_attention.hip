@@ -27,7 +27,6 @@ namespace {
 struct QuantParams {
     TreeParams t;
     PoolView z;
-    int alone;                        // a run is one item, whole
 };
 
 // The kernel's arguments, read where they are used: kept in scalar registers
@@ -38,33 +37,36 @@ __device__ __forceinline__ const QuantParams& parameters() {
     return *(const QuantParams*)args;
 }
 
-// The tiles that a workgroup has to work on: item by item.
+// The tiles that a workgroup has to work on, item by item; of a split item its part
+// of that alone.
 struct Share {
-    int pos, end;
-    bool alone;
+    int pos, end, splits;
 
     // False: none.
-    __device__ __forceinline__ bool take(const QuantParams& q, int run) {
-        alone = q.alone;
+    __device__ __forceinline__ bool take(const TreeParams& p, int run) {
+        splits = p.deal.splits;
         pos = run;
         end = run + 1;
-        if (alone) return run < q.t.B * q.t.Hk;
-        const Deal deal(q.t.deal, total_tiles(q.t.c, q.t.deal));
+        if (splits) return run < p.B * p.Hk * splits;
+        const Deal deal(p.deal, total_tiles(p.c, p.deal));
         pos = deal.begin(run);
         end = deal.begin(run + 1);
         return run < deal.runs;
     }
     __device__ __forceinline__ Item item(const TreeParams& p) const {
-        if (!alone) return item_at(p, pos, end);
+        if (!splits) return item_at(p, pos, end);
+        const int item = (uint32_t)pos / (uint32_t)splits;
         Item it;
-        it.b = (uint32_t)pos / (uint32_t)p.Hk;
-        it.h = pos - (int)it.b * p.Hk;
+        it.b = (uint32_t)item / (uint32_t)p.Hk;
+        it.h = item - (int)it.b * p.Hk;
         it.n = uniform(cache_length(p.c, it.b));
-        it.tiles = it.t1 = item_tiles(p.deal, it.n);
-        it.t0 = 0;
+        it.tiles = item_tiles(p.deal, it.n);
+        const int each = (uint32_t)(it.tiles + splits - 1) / (uint32_t)splits;
+        it.t0 = min(it.tiles, (pos - item * splits) * each);
+        it.t1 = min(it.tiles, it.t0 + each);
         return it;
     }
-    __device__ __forceinline__ void done(const Item& it) { pos += alone ? 1 : it.t1 - it.t0; }
+    __device__ __forceinline__ void done(const Item& it) { pos += splits ? 1 : it.t1 - it.t0; }
 };
 
 // 16 rows of K and V as a lane holds them: K of row `col`, elements D / 4 grp on;
@@ -288,19 +290,27 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
 
     const int run = slot_of_block();
     Share share;
-    if (!share.take(parameters(), run)) return;
+    if (!share.take(parameters().t, run)) return;
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     char* staging = sh.rows + wave * kWave;
 
     while (share.pos < share.end) {
         const Item it = share.item(parameters().t);
+        if (it.t0 == it.t1) return;                                      // a split behind the item's last tile
         const int64_t b = it.b;
         const int cached = (it.n + kFewRows - 1) / kFewRows;
         const int stop = max(it.t0, min(it.t1, cached));                 // tiles [t0, stop) of the cache
         __syncthreads();                                                 // the item before is done with LDS
         if (threadIdx.x == 0) sh.wild = 0;
         __syncthreads();
+        // the wave's groups of 16 tiles from `base` on, one a lane; those past the last group again the last one
+        const PoolView& z = parameters().z;
+        GroupLoader<D> loader(z, b, it.h);
+        const int last_row = (it.n - 1) & ~15;
+        int base = it.t0;
+        auto row_of = [&](int from) { return min((from + lane / kUnit) * kFewRows + (wave * kUnit + lane % kUnit) * 16, last_row); };
+        if (it.t0 < stop) loader.places.ask(z, row_of(base));
         u32x4 qr[NT][KS];
         load_queries<KS, NT, true>(parameters().t, b, it.h, 0, qr);
         const float scale_log2 = parameters().t.scale_log2;
@@ -356,14 +366,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
         };
 
         if (it.t0 < stop) {
-            const PoolView& z = parameters().z;
-            GroupLoader<D> loader(z, b, it.h);
             const GroupOffsets<D> off;
-            // the wave's groups of 16 tiles from `base` on, one a lane; those past the last group again the last one
-            const int last_row = (it.n - 1) & ~15;
-            int base = it.t0;
-            auto row_of = [&](int from) { return min((from + lane / kUnit) * kFewRows + (wave * kUnit + lane % kUnit) * 16, last_row); };
-            loader.places.ask(z, row_of(base));
             loader.places.take(z, row_of(base));
             loader.places.ask(z, row_of(base + 64 / kUnit));
             auto load = [&](int t, Unit& unit) {
@@ -455,8 +458,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
     const int slot = slot_of_block();
     Share share;
     {
-        const QuantParams& q = parameters();
-        if (!share.take(q, (uint32_t)slot / (uint32_t)q.t.row_blocks)) return;
+        const TreeParams& p = parameters().t;
+        if (!share.take(p, (uint32_t)slot / (uint32_t)p.row_blocks)) return;
     }
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
@@ -465,11 +468,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
 
     while (share.pos < share.end) {
         const Item it = share.item(parameters().t);
+        if (it.t0 == it.t1) return;                                      // a split behind the item's last tile
         const int64_t b = it.b;
         const int cached = (it.n + kKeys - 1) / kKeys;
         const int stop = max(it.t0, min(it.t1, cached));
         __syncthreads();                                   // the item before is done with LDS
         if (threadIdx.x == 0) sh.wild = 0;
+        // the wave's groups of 64 tiles from `base` on, one a lane; those past the last group again the last one
+        const PoolView& z = parameters().z;
+        GroupLoader<D> loader(z, b, it.h);
+        const int last_row = (it.n - 1) & ~15;
+        int base = it.t0;
+        auto row_of = [&](int from) { return min((from + lane) * kKeys + 16 * wave, last_row); };
+        if (it.t0 < stop) loader.places.ask(z, row_of(base));
         int row0;                                          // the wave's first query row
         bool idle;                                         // past the last one: this wave makes operands only
         bool once;                                         // no other block of query rows reads the codes
@@ -516,14 +527,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) q
         };
 
         if (it.t0 < stop) {
-            const PoolView& z = parameters().z;
-            GroupLoader<D> loader(z, b, it.h);
             const GroupOffsets<D> off;
-            // the wave's groups of 64 tiles from `base` on, one a lane; those past the last group again the last one
-            const int last_row = (it.n - 1) & ~15, last = stop - 1;
-            int base = it.t0;
-            auto row_of = [&](int from) { return min((from + lane) * kKeys + 16 * wave, last_row); };
-            loader.places.ask(z, row_of(base));
+            const int last = stop - 1;
             loader.places.take(z, row_of(base));
             loader.places.ask(z, row_of(base + 64));
             auto fetch = [&](int t, Group<D>& raw) {
@@ -735,28 +740,35 @@ int check_attention(const slimkv_quantized_attention_args* a) {
     return SLIMKV_OK;
 }
 
-// Short items are worked on whole, by one workgroup each, with nothing to merge and one launch less: caches of up
-// to 1024 rows (512 with more than 32 query rows), and twice that where 64 workgroups or more have an item.  Times in
-// a graph, dealt and merged / whole: one token over 512 rows 11.3 / 9.6 us, 1024 12.8 / 11.9, 1536 12.9 / 14.3; of 16
-// sequences 1024 20.1 / 12.4, 2048 20.6 / 18.4; 26 tokens over 512 rows 20.9 / 20.7, 768 20.8 / 25.5; of 8 sequences
-// 1024 46.6 / 31.4, 2048 51.5 / 52.1.
+// How the tiles come to the workgroups.  Dealt over all items, every workgroup has the same number of them however
+// ragged the batch is, but most work on two items, each with its own start and end.  Where an item's tiles are few
+// it is cut into splits of its own instead: so many that two workgroups a CU have work, of at least two tiles, and
+// where no split has more than 16; up to five tiles stay whole and need no merge.  Dealt / split, in a graph: one
+// token of 16 sequences of 1024 rows 20.1 / 14.2 us (whole 12.4), 4096 28.8 / 22.4, 8192 38.9 / 32.3, of a quarter to
+// all of 8192 30.7 / 28.9; of one sequence of 4096 13.6 / 11.2; 26 tokens of 4 sequences of 2048 37.5 / 31.2, 8192 50.1
+// / 41.0; longer ones are equal.  Splits of one tile and of four: one sequence of 4096 9.9 and 13.2, 26 tokens over
+// 512 rows of 4 sequences 25.4 and 19.0 against 17.7.
+constexpr int kLeastTiles = 2, kMostTiles = 16, kWholeTiles = 5;
+
 struct QuantPlan : TreePlan {
     int tile;                                      // cache rows of a tile
-    bool alone;
-    size_t bytes(int64_t D) const { return alone ? 0 : TreePlan::bytes(D); }
+    int splits;                                    // of every item; 0: dealt
+    bool merges() const { return splits ? splits > 1 : !whole(); }
+    size_t bytes(int64_t D) const { return merges() ? (size_t)slots * 2 * rows() * (D + 2) * sizeof(float) : 0; }
 };
 
 QuantPlan plan_attention(const slimkv_quantized_attention_args* a) {
     QuantPlan t{};
     static_cast<TreePlan&>(t) = plan_tree(a->tokens * (a->heads / a->kv_heads));
     t.tile = t.rw == 1 ? 64 * few_groups(t.nt) : kKeys;
-    const int64_t items = a->batch * a->kv_heads;
-    const int64_t workgroups = items * t.row_blocks;
-    t.alone = a->keys <= (t.rw == 1 ? 1024 : 512) * (workgroups >= 64 ? 2 : 1) && workgroups <= 65536;
-    if (t.alone) {
-        t.runs = (int)items;
-        t.slots = workgroups;
-    }
+    const int64_t workgroups = a->batch * a->kv_heads * t.row_blocks, resident = 2 * device_cu_count();
+    const int64_t tiles = (a->keys + t.tile - 1) / t.tile + (a->tokens + kKeys - 1) / kKeys;
+    if (workgroups == 0 || workgroups > 65536) return t;
+    const int64_t splits = tiles <= kWholeTiles ? 1 : std::max<int64_t>(1, std::min((tiles + kLeastTiles - 1) / kLeastTiles, resident / workgroups));
+    if ((tiles + splits - 1) / splits > kMostTiles) return t;
+    t.splits = (int)splits;
+    t.runs = (int)(a->batch * a->kv_heads * splits);
+    t.slots = workgroups * splits;
     return t;
 }
 
@@ -768,7 +780,7 @@ void launch_attention(const QuantParams& p, const QuantPlan& plan, hipStream_t s
                                   : plan.nt == 2 ? quant_few_kernel<D, F16, 2>
                                                  : quant_few_kernel<D, F16, 1>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p);
-    if (!plan.alone) launch_merge<D, F16>(p.t, plan, st);
+    if (plan.merges()) launch_merge<D, F16>(p.t, plan, st);
 }
 
 }  // namespace
@@ -806,8 +818,7 @@ extern "C" int slimkv_quantized_attention(const slimkv_quantized_attention_args*
         if (draft && T > 1 && (s < D || s >= (1 << 23)))
             return fail(SLIMKV_EUNSUP, "quantized attention: drafted rows must lie [head_dim, 2^23) elements apart");
     const QuantPlan plan = plan_attention(a);
-    const bool merges = !plan.alone && !plan.whole();
-    if (merges &&
+    if (plan.merges() &&
         (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes(D)))
         return fail(SLIMKV_EWORKSPACE, "quantized attention: workspace missing, misaligned or too small");
     p.c.lengths = a->lengths; p.c.keys = (int)a->keys;
@@ -820,12 +831,11 @@ extern "C" int slimkv_quantized_attention(const slimkv_quantized_attention_args*
     p.B = (int)B; p.T = (int)T; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk);
     p.M = p.T * p.G;
     p.row_blocks = plan.row_blocks;
-    qp.alone = plan.alone;
     // without drafted tokens a tile without work, so that a sequence without rows has a run that writes its output
-    p.deal = Dealing{p.B, p.Hk, plan.tile, draft ? (p.T + kKeys - 1) / kKeys : 1, plan.runs};
+    p.deal = Dealing{p.B, p.Hk, plan.tile, draft ? (p.T + kKeys - 1) / kKeys : 1, plan.runs, plan.splits};
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.part = static_cast<float*>(workspace);
-    if (B * Hk * p.M > 0x7fffffff || (merges && !launchable(B * Hk * plan_merge(plan, B * Hk, p.M, D).chunks, 256)) ||
+    if (B * Hk * p.M > 0x7fffffff || (plan.merges() && !launchable(B * Hk * plan_merge(plan, B * Hk, p.M, D).chunks, 256)) ||
         B * Hk * ((a->keys + T) / kKeys + 2) > 0x7fffffff)
         return fail(SLIMKV_EINVAL, "quantized attention: too many rows for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -526,23 +526,32 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p, int rows_
     const int group = threadIdx.x / (D / 4), part = group % SHARE, c = 4 * (threadIdx.x % (D / 4));
     const int row = (blockIdx.x % chunks) * kRowsWg + group / SHARE;
 
-    // first tile of the item: tiles of the sequences before it
-    const int lane = threadIdx.x & 63;
-    int before = 0, all = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int x = b0 + lane < p.B ? item_tiles(p.deal, cache_length(p.c, b0 + lane)) : 0;
-        int lower = b0 + lane < b ? x : 0, any = x;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            lower += __shfl_xor(lower, s, 64);
-            any += __shfl_xor(any, s, 64);
-        }
-        before += lower;
-        all += any;
-    }
     const int tiles = item_tiles(p.deal, cache_length(p.c, b));
-    const Deal deal(p.deal, uniform(all) * p.Hk);
-    const int first = uniform(before) * p.Hk + h * tiles, r0 = deal.run_of(first), r1 = deal.run_of(first + tiles - 1);
+    int r0, r1;                                          // the item's runs
+    if (p.deal.splits) {
+        const int each = (uint32_t)(tiles + p.deal.splits - 1) / (uint32_t)p.deal.splits;
+        r0 = item * p.deal.splits;
+        r1 = r0 + (uint32_t)(tiles - 1) / (uint32_t)each;
+    } else {
+        // first tile of the item: tiles of the sequences before it
+        const int lane = threadIdx.x & 63;
+        int before = 0, all = 0;
+        for (int b0 = 0; b0 < p.B; b0 += 64) {
+            const int x = b0 + lane < p.B ? item_tiles(p.deal, cache_length(p.c, b0 + lane)) : 0;
+            int lower = b0 + lane < b ? x : 0, any = x;
+#pragma unroll
+            for (int s = 1; s < 64; s <<= 1) {
+                lower += __shfl_xor(lower, s, 64);
+                any += __shfl_xor(any, s, 64);
+            }
+            before += lower;
+            all += any;
+        }
+        const Deal deal(p.deal, uniform(all) * p.Hk);
+        const int first = uniform(before) * p.Hk + h * tiles;
+        r0 = deal.run_of(first);
+        r1 = deal.run_of(first + tiles - 1);
+    }
     if (r0 == r1) return;
     const int live = min(row, p.M - 1), rb = live / rows_wg, in = live - rb * rows_wg;
     const int64_t size = (int64_t)rows_wg * (D + 2);
