@@ -402,6 +402,47 @@ def test_offsets_past_32_bits(T):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize('T,N,dtype', [(1, 4300, 'bf16'), (20, 2200, 'fp16'), (40, 1100, 'bf16'), (70, 1200, 'fp16')])
+def test_large_ragged_batches(T, N, dtype):
+    """So many items and tiles that workgroups take parts of several items, one after another."""
+    from slimkv_amd import quant_cache
+    B, H, D, g, dt = 64, 8, 64, gen(58), TYPES[dtype]
+    lengths = [N - (61 * b) % N if b % 9 else 0 for b in range(B)]
+    lengths[5], lengths[6], lengths[63] = 1, N, N - 16
+    k, v = randn(g, B, N, H, D, dtype=dt), randn(g, B, N, H, D, dtype=dt)
+    count, table = scattered(g, B, -(-N // 32))
+    pages = quant_cache.new_pages(count, H, 32, D)
+    quant_cache.quantize_rows(k, v, pages, table)
+    q, dk, dv = randn(g, B, T, H, D, dtype=dt), randn(g, B, T, H, D, dtype=dt), randn(g, B, T, H, D, dtype=dt)
+    kc, vc = quant_cache.dequantize_rows(pages, N, D, table, dtype=dt)
+    for draft in ((dk, dv), (None, None)):
+        out, lse = quant_cache.quantized_attention(q, *draft, 0.125, pages, table, lengths=ints(lengths), keys=N)
+        pick = [0, 5, 6, 31, 63]
+        mask = None if draft[0] is not None else torch.zeros(len(pick), T, T, dtype=torch.bool, device='cuda')
+        check_tree(out[pick], lse[pick], q[pick], kc[pick], vc[pick], [lengths[b] for b in pick], dk[pick], dv[pick], mask, 0.125)
+        again, lse2 = quant_cache.quantized_attention(q, *draft, 0.125, pages, table, lengths=ints(lengths), keys=N)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize('T', [1, 40])
+def test_one_page_past_32_bits(T):
+    """One sequence of 2^26 and more rows in one page, codes past 2^32 bytes: zero keys weigh alike, so the output is the
+    sum of the values over their number; only the last rows have values."""
+    from slimkv_amd import quant_cache
+    D, n = 128, (1 << 26) + 4112
+    pages = torch.zeros(1, 1, n * 136, dtype=torch.uint8, device='cuda')
+    v = torch.full((1, 7, 1, D), 2.0 ** 60, dtype=torch.bfloat16, device='cuda')
+    quant_cache.quantize_rows(torch.zeros_like(v), v, pages, starts=ints([n - 9]))
+    q = randn(gen(59), 1, T, 1, D)
+    out, lse = quant_cache.quantized_attention(q, None, None, 1.0, pages, lengths=ints([n - 2]))
+    # the fp32 sums of at most 2^20 equal weights a lane and of 2^9 runs: 2^-24 each; the output's rounding 2^-8
+    want = 7 * 2.0 ** 60 / (n - 2)
+    assert ((out.double() / want - 1).abs() <= 2.0 ** -8 + 2.0 ** -12).all()
+    assert (lse.double() - float(np.log(n - 2))).abs().max() <= 2.0 ** -12
+    out, _ = quant_cache.quantized_attention(q, None, None, 1.0, pages, lengths=ints([n - 9]))
+    assert not out.any()
+
+
 @pytest.mark.parametrize('T,dtype', [(1, 'bf16'), (40, 'fp16')])
 def test_long_caches_over_pages_of_any_size(T, dtype):
     """The bits of one page a sequence, whatever the pages' size."""
