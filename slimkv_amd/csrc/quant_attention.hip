@@ -16,6 +16,20 @@
 //       rows so that a lane reads its column's codes of its four keys; a byte is two
 //       columns of one key and one block, and pairs of keys are then joined.
 // So the rows pass no LDS where they serve one wave's columns.
+//
+// Up to 32 query rows a KV head the cache's bytes are the bound, 136 a row and head
+// of 128 (quant_few_kernel: 16 sequences of 8-32K rows, a token each, 357 MB in 64
+// us, 5.6 TB/s, the call with its merge 71; a copy moves 5.2).  More rows are bound by
+// the instructions of the softmax and of the conversions beside the products and by
+// the power that they take together (quant_many_kernel: 26 tokens on the same cache 202
+// us a call, 690 TFLOP/s of needed work, 850 with the rows that fill up the last tiles;
+// 63 tokens of 40 heads over 131071 rows 214 us, 790 and 960; the library's 8192^3
+// product reaches 1100-1140).  Figures beside a choice compare its two sides as they
+// were when it was made.
+//
+// Not taken: the product that takes 4-bit operands itself
+// (v_mfma_scale_f32_16x16x128_f8f6f4, the queries cut into exact 8-bit parts).  Its
+// sums are off by up to 1e-4 of sum |q k|, those of 16-bit products by 1e-7.
 
 #include "quant.hpp"
 #include "tree.hpp"
