@@ -251,6 +251,7 @@ def test_pages_of_other_sizes_are_refused():
 def test_the_c_entry_points_refuse_bad_sizes():
     from slimkv_amd import _lib
     lib = _lib.lib()
+    refused = (-1, -2)                                             # arguments, never the launch of a kernel on made-up addresses
     cache = dict(pages=1 << 20, p_sb=2 * 1088, p_sh=1088, num_pages=4, block_size=16)
     rows = dict(k=1 << 12, k_sb=640, k_sn=128, k_sh=64, v=1 << 16, v_sb=640, v_sn=128, v_sh=64, batch=2, rows=5, kv_heads=2,
                 head_dim=64)
@@ -264,13 +265,13 @@ def test_the_c_entry_points_refuse_bad_sizes():
     for entry, mirror in ((lib.slimkv_quantize_rows, _lib.QuantizeRowsArgs),
                           (lib.slimkv_dequantize_rows, _lib.DequantizeRowsArgs)):
         for over in bad_cache:
-            assert rows_call(entry, mirror, over) < 0, over
+            assert rows_call(entry, mirror, over) in refused, over
         for over in (dict(head_dim=96), dict(dtype=2), dict(batch=-1), dict(batch=65536), dict(rows=-1), dict(kv_heads=0),
                      dict(kv_heads=4097), dict(k=0), dict(v=8), dict(k_sn=132), dict(rows=1 << 29),
                      dict(rows=(1 << 30) + 1)):
-            assert rows_call(entry, mirror, **over) < 0, over
+            assert rows_call(entry, mirror, **over) in refused, over
         assert rows_call(entry, mirror, batch=0) == 0 and rows_call(entry, mirror, rows=0) == 0
-        assert entry(None, None) < 0
+        assert entry(None, None) in refused
 
     att = dict(q=1 << 12, q_sb=1536, q_sl=512, q_sh=64, draft_k=1 << 16, dk_sb=384, dk_sn=128, dk_sh=64, draft_v=1 << 18,
                dv_sb=384, dv_sn=128, dv_sh=64, out=1 << 22, o_sb=1536, o_sl=512, o_sh=64, lse=1 << 24, batch=2, tokens=3, heads=8,
@@ -281,13 +282,14 @@ def test_the_c_entry_points_refuse_bad_sizes():
         return lib.slimkv_quantized_attention(ctypes.byref(a), None, 0, None)
 
     for over in bad_cache:
-        assert att_call(over) < 0, over
+        assert att_call(over) in refused, over
     for over in (dict(head_dim=32), dict(dtype=2), dict(batch=65536), dict(tokens=1025), dict(heads=7), dict(heads=4104),
                  dict(heads=1024), dict(kv_heads=0), dict(scale=0.0), dict(scale=float('nan')), dict(scale=1e19),
                  dict(q=0), dict(q=8), dict(out=0), dict(draft_v=0), dict(draft_k=0, draft_v=0, mask=64), dict(keys=17),
                  dict(keys=-1), dict(dk_sn=1 << 23), dict(dv_sn=56), dict(o_sh=68)):
-        assert att_call(**over) < 0, over
-    assert att_call() == -3 or att_call() < 0                      # no workspace given
+        assert att_call(**over) in refused, over
+    long = dict(block_size=4096, p_sb=2 * 4096 * 68, p_sh=4096 * 68)
+    assert att_call(long, keys=4096) == -3                         # cut into parts that are merged: no workspace given
     assert att_call(batch=0) == 0 and att_call(tokens=0) == 0
     a = _lib.QuantizedAttentionArgs(cache=_lib.QuantPages(**cache), **{**att, 'head_dim': 32})
     assert lib.slimkv_quantized_attention_workspace(ctypes.byref(a)) == 0
@@ -299,7 +301,7 @@ def test_the_c_entry_points_refuse_bad_sizes():
                  dict(kv_heads=-1), dict(eps=-1.0), dict(eps=float('nan')), dict(eps=float('inf')), dict(q=0), dict(k=0),
                  dict(out_k=0), dict(cos=0), dict(cos=8), dict(table_rows=0), dict(q_sh=68), dict(q_weight=8),
                  dict(positions=0), dict(length=1 << 30)):
-        assert lib.slimkv_norm_rope(ctypes.byref(_lib.NormRopeArgs(**{**nr, **over})), None) < 0, over
+        assert lib.slimkv_norm_rope(ctypes.byref(_lib.NormRopeArgs(**{**nr, **over})), None) in refused, over
     assert lib.slimkv_norm_rope(ctypes.byref(_lib.NormRopeArgs(**{**nr, 'batch': 0})), None) == 0
 
 
