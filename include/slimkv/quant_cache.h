@@ -134,7 +134,8 @@ int slimkv_quantized_attention(const slimkv_quantized_attention_args* a, void* w
  * Queries and keys of a step or window, each head normalised and rotated:
  *   y = x / sqrt(mean(x^2) + eps) * weight    (weight NULL: y = x)
  *   out = y * cos[pos] + rotate_half(y) * sin[pos],  pos = positions[b, l]
- * rotate_half(y) = (-y[D/2:], y[:D/2]).  fp32 throughout, one rounding.
+ * rotate_half(y) = (-y[D/2:], y[:D/2]).  fp32 throughout, one rounding; a
+ * normalised head's sum of squares has to lie within fp32.
  * q [B, L, Hq, D], k [B, L, Hkv, D] (kv_heads 0: queries alone), q_weight /
  * k_weight [D] in the element type or (weight_f32) fp32, cos / sin [table_rows,
  * D] fp32, positions int64 (strides pos_sb, pos_sl).  A position outside the

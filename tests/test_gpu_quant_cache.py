@@ -552,6 +552,27 @@ def test_norm_rope(case, in_place):
         assert torch.equal(both[:, :, Hq + H:], after)
 
 
+@pytest.mark.parametrize('B,L,Hq,H,D,dtype', [(3, 2001, 33, 7, 64, 'bf16'), (2, 4097, 33, 7, 128, 'fp16'), (1, 5461, 17, 8, 128, 'bf16'),
+                                              (5, 3001, 40, 3, 64, 'fp16')])
+def test_norm_rope_of_many_tokens(B, L, Hq, H, D, dtype):
+    """The bits of calls of a few tokens, where a wave takes several rounds of heads and rows go past the caches: heads
+    that fill neither the last round nor the last wave."""
+    from slimkv_amd import quant_cache
+    g, dt = gen(59), TYPES[dtype]
+    both = randn(g, B, L, Hq + 2 * H, D, dtype=dt)
+    q, k, rest = both[:, :, :Hq], both[:, :, Hq:Hq + H], both[:, :, Hq + H:].clone()
+    cos, sin = torch.rand(700, D, generator=g, device='cuda'), torch.rand(700, D, generator=g, device='cuda')
+    positions = torch.randint(0, 700, (B, L), generator=g, device='cuda')
+    weights = dict(q_weight=randn(g, D, dtype=dt), k_weight=randn(g, D, dtype=dt))
+    pieces = [quant_cache.norm_rope(q[:, i:i + 127], k[:, i:i + 127], cos, sin, positions[:, i:i + 127], **weights)
+              for i in range(0, L, 127)]
+    want = [torch.cat(x, 1) for x in zip(*pieces)]
+    got = quant_cache.norm_rope(q, k, cos, sin, positions, **weights)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    quant_cache.norm_rope(q, k, cos, sin, positions, out_q=q, out_k=k, **weights)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(both[:, :, Hq + H:], rest)
+
+
 def test_norm_rope_shared_positions_views_and_bad_positions():
     from slimkv_amd import quant_cache
     g, B, L, D = gen(54), 3, 6, 128
