@@ -170,17 +170,17 @@ extern "C" int slimkv_norm_rope(const slimkv_norm_rope_args* a, void* stream) {
     p.out_k = static_cast<char*>(a->out_k); p.ok_sb = 2 * a->ok_sb; p.ok_sl = 2 * a->ok_sl; p.ok_sh = 2 * a->ok_sh;
     p.status = a->status;
     const int64_t tokens = B * L, round = 1024 / D, rounds = (Hq + Hk + round - 1) / round;
-    if (tokens * rounds > 0x7fffffff / 64 * 4)
-        return fail(SLIMKV_EINVAL, "norm rope: too many rows for one call");
-    p.tokens = (int)tokens; p.Hq = (int)Hq; p.H = (int)(Hq + Hk);
     // Two rounds a wave where that leaves every SIMD several waves (8192 tokens of 48 heads: one round 47.7 us, two
     // 43.1, three 43.4, four 44.1); past the caches from 64 MB of rows on, twice the L2 (the same call 43.1 / 40.2).
     p.each = tokens * rounds >= 16384 ? 2 : 1;
+    const int64_t chunks = (rounds + p.each - 1) / p.each, workgroups = (tokens * chunks + 3) / 4;
+    // keeps tokens, and waves, below 2^31 as well
+    if (!launchable(workgroups, 256)) return fail(SLIMKV_EINVAL, "norm rope: too many rows for one call");
     const bool far = tokens * (Hq + Hk) * D * 2 >= ((int64_t)64 << 20);
-    const int64_t chunks = (rounds + p.each - 1) / p.each;
+    p.tokens = (int)tokens; p.Hq = (int)Hq; p.H = (int)(Hq + Hk);
     p.by_length = fast_div(L); p.by_chunks = fast_div(chunks);
     p.eps = (float)a->eps; p.weight_f32 = a->weight_f32;
-    const dim3 grid((unsigned)((tokens * chunks + 3) / 4));
+    const dim3 grid((unsigned)workgroups);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool f16 = a->dtype == SLIMKV_DTYPE_F16;
     void (*kernel)(HeadsParams);

@@ -366,3 +366,24 @@ def test_oracle_rotates_by_hand():
     y = x / np.sqrt(12.5) * w
     assert np.allclose(out, [0.6 * y[0] - 0.8 * y[1], 0.6 * y[1] + 0.8 * y[0]])
     assert np.allclose(terms, [0.6 * y[0] + 0.8 * y[1], 0.6 * y[1] + 0.8 * y[0]])
+
+
+@pytest.mark.parametrize('dim,heads,kv_heads', [(128, 8, 0), (128, 5, 3), (128, 12, 4), (128, 17, 0), (64, 16, 0), (64, 20, 12),
+                                                (64, 33, 0), (128, 4096, 4096)])
+def test_norm_rope_refuses_more_threads_than_a_launch_counts(dim, heads, kv_heads):
+    """One, two, three and many rounds of heads a token: a wave takes two, and a launch counts its threads in 32 bits, 4 waves
+    a workgroup of 256."""
+    from slimkv_amd import _lib
+    rounds = -(-(heads + kv_heads) * dim // 1024)
+    chunks = -(-rounds // 2)
+    most = 4 * (0xffffffff // 256) // chunks                        # tokens whose workgroups are launchable
+    for tokens in (most + 1, most + 2, most + most // 3, 2 * most + 7, 4 * most):
+        batch = next(b for b in range(tokens >> 30, 65536) if b and tokens % b == 0 and tokens // b <= 1 << 30)
+        wide, narrow = heads * dim, max(kv_heads, 1) * dim
+        a = _lib.NormRopeArgs(
+            q=1 << 12, q_sb=wide, q_sl=wide, q_sh=dim, k=1 << 16, k_sb=narrow, k_sl=narrow, k_sh=dim, cos=1 << 20, sin=1 << 21,
+            table_rows=9, positions=1 << 22, pos_sb=3, pos_sl=1, out_q=1 << 23, oq_sb=wide, oq_sl=wide, oq_sh=dim, out_k=1 << 24,
+            ok_sb=narrow, ok_sl=narrow, ok_sh=dim, batch=batch, length=tokens // batch, heads=heads, kv_heads=kv_heads,
+            head_dim=dim, eps=1e-6)
+        assert _lib.lib().slimkv_norm_rope(ctypes.byref(a), None) == -1, tokens
+        assert b'too many rows' in _lib.lib().slimkv_last_error(), tokens
