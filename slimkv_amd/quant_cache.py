@@ -306,13 +306,14 @@ def norm_rope(q, k, cos, sin, positions, *, q_weight=None, k_weight=None, eps=1e
         raise ValueError(f'{name}: q_weight and k_weight must be of one type')
     if k is None and (k_weight is not None or out_k is not None):
         raise ValueError(f'{name}: k_weight and out_k belong to keys')
-    for what, x, t in (('out_q', q, out_q), ('out_k', k, out_k)):
+    for what, x, other, t in (('out_q', q, k, out_q), ('out_k', k, q, out_k)):
         if t is None:
             continue
         if t.shape != x.shape or t.stride(3) != 1 or _folded(t):
             raise ValueError(f'{name}: {what} must have the shape of its input with contiguous features, no expanded view')
         same = t.data_ptr() == x.data_ptr() and t.stride() == x.stride()
-        if not _clear_of(t, *(s for s in (q, k, cos, sin, positions, q_weight, k_weight) if not (same and s is x))):
+        # by role: q and k may be one tensor, and what is in place for one is then not apart from the other
+        if not _clear_of(t, other, cos, sin, positions, q_weight, k_weight, None if same else x):
             raise ValueError(f'{name}: {what} must be its input itself or lie apart from all inputs')
     if out_q is not None and out_k is not None and _overlap(out_q, out_k):
         raise ValueError(f'{name}: out_q and out_k must lie apart')

@@ -387,3 +387,20 @@ def test_norm_rope_refuses_more_threads_than_a_launch_counts(dim, heads, kv_head
             head_dim=dim, eps=1e-6)
         assert _lib.lib().slimkv_norm_rope(ctypes.byref(a), None) == -1, tokens
         assert b'too many rows' in _lib.lib().slimkv_last_error(), tokens
+
+
+def test_norm_rope_in_place_over_one_tensor_for_queries_and_keys():
+    """Its key heads would read what its query heads wrote."""
+    x = z(2, 3, 8, 64)
+    for over in (dict(out_q=x), dict(out_k=x), dict(out_q=x, out_k=z(2, 3, 8, 64)), dict(out_q=z(2, 3, 8, 64), out_k=x)):
+        with pytest.raises(ValueError, match='must be its input itself or lie apart'):
+            norm(q=x, k=x, **over)
+    with pytest.raises(ValueError, match='out_q and out_k must lie apart'):
+        norm(q=x, k=x[:], out_q=(y := z(2, 3, 8, 64)), out_k=y)
+    with pytest.raises(ValueError, match='device tensors'):               # read twice, written elsewhere
+        norm(q=x, k=x, out_q=z(2, 3, 8, 64))
+    with pytest.raises(ValueError, match='device tensors'):               # two views of one memory, each in place
+        norm(q=fused[:, :, :8], k=fused[:, :, 8:10], out_q=fused[:, :, :8], out_k=fused[:, :, 8:10])
+    one = z(1, 1, 1, 64)
+    with pytest.raises(ValueError, match='must be its input itself or lie apart'):
+        norm(q=one, k=z(1, 1, 1, 64), positions=z(1, 1, dtype=I64), q_weight=one.view(-1), out_q=one)
