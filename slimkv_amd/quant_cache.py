@@ -125,9 +125,11 @@ def quantize_rows(k, v, pages, table=None, *, starts=None, counts=None, status=N
         raise ValueError(f'{name}: k and v must be [B, n, Hkv, D] with contiguous features')
     B, n, H, D = k.shape
     code = _dtype(name, k, v)
+    given = table
     place, rows, _, table = _pool(name, pages, table, B, H, D)
     starts, counts = _whole_numbers(name, 'starts', starts, B), _whole_numbers(name, 'counts', counts, B)
-    if not pages.is_contiguous() and _folded(pages) or table is not None and not table.is_contiguous() and _folded(table):
+    # the table as it was given: the copy of one that is expanded along its columns is no expanded view
+    if not pages.is_contiguous() and _folded(pages) or given is not None and not given.is_contiguous() and _folded(given):
         raise ValueError(f'{name}: pages and table must not be expanded or overlapping views')
     if not _clear_of(pages, k, v, table, starts, counts):
         raise ValueError(f'{name}: pages must share no memory with the other tensors')

@@ -404,3 +404,22 @@ def test_norm_rope_in_place_over_one_tensor_for_queries_and_keys():
     one = z(1, 1, 1, 64)
     with pytest.raises(ValueError, match='must be its input itself or lie apart'):
         norm(q=one, k=z(1, 1, 1, 64), positions=z(1, 1, dtype=I64), q_weight=one.view(-1), out_q=one)
+
+
+@pytest.mark.parametrize('table', [z(2, 1, dtype=I64).expand(2, 3), z(1, 1, dtype=I64).expand(2, 3),
+                                   z(9, dtype=I64).as_strided((2, 3), (2, 2)), z(9, dtype=I64).as_strided((2, 3), (3, 0)),
+                                   z(9, dtype=I64).as_strided((2, 3), (2, 1))])
+def test_quantize_rows_refuses_tables_that_name_a_page_twice(table):
+    """Expanded or overlapping along either dimension, before the copy that makes a table's rows contiguous."""
+    with pytest.raises(ValueError, match='expanded or overlapping'):
+        quantize(table=table)
+
+
+def test_tables_with_steps_are_written_through():
+    for table in (z(3, 2, dtype=I64).t(), z(2, 6, dtype=I64)[:, ::2], z(2, 9, dtype=I64)[:, 3:6], z(6, 2, dtype=I64)[::2].t()):
+        with pytest.raises(ValueError, match='device tensors'):
+            quantize(table=table)
+        with pytest.raises(ValueError, match='device tensors'):
+            dequantize(table=table)
+    with pytest.raises(ValueError, match='device tensors'):               # reading, sequences may share pages
+        dequantize(table=z(2, 1, dtype=I64).expand(2, 3))
