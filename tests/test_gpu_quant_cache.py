@@ -780,3 +780,49 @@ def test_scores_of_a_thousand_million_and_more():
             out, lse = quant_cache.quantized_attention(q, None, None, scale, pages, lengths=ints([N]))
             assert torch.equal(out[0, :, 0], back[0, 17, 0].expand(T, D))
             assert ((lse / (1.5 * scale) - 1).abs() <= 2.0 ** -21).all()
+
+
+# query rows a KV head -> the kernel: up to 16 and 32 (few), 64 and more (many); of each, in both types and head sizes, items
+# that stay whole, that are cut into splits of their own and (DEALT) that are dealt out with others
+KERNELS = [
+    # T, Hq, Hkv, N of a whole item, N of a split one, N of a dealt one
+    (5, 6, 2, 701, 1500, 4300),
+    (6, 16, 4, 399, 1029, 2200),
+    (5, 14, 2, 201, 700, 1100),
+    (26, 8, 2, 199, 1029, 1100),
+]
+EVERY = [(2, T, Hq, H, D, N, [N, part], block, dtype, mask)
+         for D in (64, 128) for dtype in TYPES for T, Hq, H, whole, split, _ in KERNELS
+         for N, part, block, mask in ((whole, 37, 16, None), (split, 129, 48, 'tree'), (split, split - 70, 32, 'alone'))]
+# B, T, Hq, Hkv, D, N, dtype
+DEALT = [(64, T, 8 * (Hq // H), 8, D, N, dtype) for D in (64, 128) for dtype in TYPES for T, Hq, H, _, _, N in KERNELS]
+
+
+@pytest.mark.parametrize('case', EVERY, ids=[str(i) for i in range(len(EVERY))])
+def test_every_kernel_over_whole_and_split_items(case):
+    test_quantized_attention(case)
+
+
+@pytest.mark.parametrize('case', DEALT, ids=[str(i) for i in range(len(DEALT))])
+def test_every_kernel_over_dealt_items(case):
+    from slimkv_amd import quant_cache
+    B, T, Hq, H, D, N, dtype = case
+    print(case, flush=True)
+    g, dt = gen(62), TYPES[dtype]
+    lengths = [N - (61 * b) % N if b % 9 else 0 for b in range(B)]
+    lengths[5], lengths[6], lengths[63] = 1, N, N - 16
+    count, table = scattered(g, B, -(-N // 32))
+    pages = quant_cache.new_pages(count, H, 32, D)
+    for b in range(0, B, 16):                                       # sixteen sequences' full-width rows at a time
+        rows = [randn(g, 16, N, H, D, dtype=dt) for _ in range(2)]
+        quant_cache.quantize_rows(*rows, pages, table[b:b + 16])
+    q = randn(g, B, T, Hq, D, dtype=dt)
+    dk, dv = randn(g, B, T, H, D, dtype=dt), randn(g, B, T, H, D, dtype=dt)
+    mask = tree_mask(g, B, T, 'tree')
+    pick = [0, 5, 6, 63]
+    kc, vc = quant_cache.dequantize_rows(pages, N, D, table[pick].contiguous(), dtype=dt)
+    call = lambda: quant_cache.quantized_attention(q, dk, dv, D ** -0.5, pages, table, lengths=ints(lengths), keys=N, mask=mask)
+    out, lse = call()
+    check_tree(out[pick], lse[pick], q[pick], kc, vc, [lengths[b] for b in pick], dk[pick], dv[pick], mask[pick], D ** -0.5, str(case))
+    again, lse2 = call()
+    assert torch.equal(out, again) and torch.equal(lse, lse2)

@@ -423,3 +423,22 @@ def test_tables_with_steps_are_written_through():
             dequantize(table=table)
     with pytest.raises(ValueError, match='device tensors'):               # reading, sequences may share pages
         dequantize(table=z(2, 1, dtype=I64).expand(2, 3))
+
+
+def attention_form(B, T, Hq, H, N):
+    """(kernel, how its items are cut) of a call, as the plan has it on 256 CUs."""
+    rows = T * (Hq // H)
+    kernel = 16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128
+    tile = {16: 256, 32: 128}.get(kernel, 64)
+    workgroups = B * H * -(-rows // kernel)
+    tiles = -(-N // tile) + -(-T // 64)
+    splits = 1 if tiles <= 5 else max(1, min(-(-tiles // 2), 512 // workgroups))
+    return kernel, 'dealt' if -(-tiles // splits) > 16 else 'whole' if splits == 1 else 'split'
+
+
+def test_every_attention_kernel_is_compared_with_the_plain_form():
+    from tests import test_gpu_quant_cache as gpu
+    have = {(D, dtype, *attention_form(B, T, Hq, H, N)) for B, T, Hq, H, D, N, _, _, dtype, _ in gpu.EVERY}
+    have |= {(D, dtype, *attention_form(B, T, Hq, H, N)) for B, T, Hq, H, D, N, dtype in gpu.DEALT}
+    assert have == {(D, dtype, kernel, cut) for D in (64, 128) for dtype in gpu.TYPES for kernel in (16, 32, 64, 128)
+                    for cut in ('whole', 'split', 'dealt')}
