@@ -15,10 +15,12 @@ The cache is a uint8 tensor `pages` [pages, Hkv, bytes] (new_pages): `block` row
 of a page, a multiple of 16, take page_bytes(block, head_dim) = block * (D +
 D / 16) bytes a KV head, 17 / 64 of bf16 or fp16 rows.  Blocks of 32 elements share a
 power of two and hold 4-bit floats (0, 0.5, 1, 1.5, 2, 3, 4, 6, and negative)
-times it: an element is off by at most a fifth of its block's largest magnitude.
-A block that held an infinity or NaN reads as NaN.  include/slimkv/quant_cache.h
-gives every byte's place.  With a block table [B, cols] int64 row n of sequence b
-is row n % block of page table[b, n // block]; without one sequence b is page b.
+times it: an element is off by at most a fifth of its block's largest magnitude
+(2^-129 where that is more; a quarter in blocks that reach past 15/16 of the power
+of two at which the type ends, 65536 or 2^128).  A block that held an infinity or
+NaN reads as NaN.  include/slimkv/quant_cache.h gives every byte's place.  With a
+block table [B, cols] int64 row n of sequence b is row n % block of page table[b, n
+// block]; without one sequence b is page b.
 
 Element types bf16 and fp16 (one for all tensors of a call; the cache itself has
 none), head_dim 64 or 128.  Up to 65535 sequences and 4096 heads.  Pages start on

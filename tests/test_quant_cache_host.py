@@ -442,3 +442,27 @@ def test_every_attention_kernel_is_compared_with_the_plain_form():
     have |= {(D, dtype, *attention_form(B, T, Hq, H, N)) for B, T, Hq, H, D, N, dtype in gpu.DEALT}
     assert have == {(D, dtype, kernel, cut) for D in (64, 128) for dtype in gpu.TYPES for kernel in (16, 32, 64, 128)
                     for cut in ('whole', 'split', 'dealt')}
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+def test_the_stated_bound_of_a_written_element(dtype):
+    """Every 16-bit number as its block's largest, beside random smaller ones: off by a fifth of the largest at most, by
+    2^-129 where that is more, by a quarter in blocks past 15/16 of the power of two at which the type ends."""
+    kind, end = (torch.bfloat16, 2.0 ** 128) if dtype == 'bf16' else (torch.float16, 2.0 ** 16)
+    bits = torch.arange(1, 1 << 15, dtype=torch.int32).to(torch.int16)
+    largest = bits.view(kind)
+    largest = largest[torch.isfinite(largest)]
+    g = torch.Generator().manual_seed(5)
+    x = largest[:, None].repeat(1, 32)
+    share = torch.rand(len(largest), 31, generator=g, dtype=torch.float64) * torch.randint(0, 2, (len(largest), 31), generator=g)
+    x[:, 1:] = (share * largest[:, None].double()).to(kind)                          # 0 and anything up to the largest
+    x = x.double().numpy()
+    assert (x <= x[:, :1]).all()
+    error = np.abs(oq.values(*oq.quantize(x, dtype)) - x).max(1)
+    top = x[:, 0]
+    last = top > 15 / 16 * end
+    assert last.any() and (error[last] <= top[last] / 4).all() and (error[last] / top[last]).max() > 0.24
+    usual = np.maximum(top / 5, 2.0 ** -129)
+    assert (error[~last] <= usual[~last]).all() and (error / top)[~last & (top > 2.0 ** -120)].max() > 0.199
+    if dtype == 'bf16':
+        assert error[top < 2.0 ** -129].max() > 0.9 * 2.0 ** -129
