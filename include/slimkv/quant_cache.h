@@ -50,8 +50,8 @@ int slimkv_quant_abi_version(void);
  *   K scales, then V scales   row r at r head_dim / 32, a byte a block
  * table NULL: sequence b is page b (num_pages >= batch), rows 0 .. block_size - 1.
  * table given: row n of sequence b is row n % block_size of page table[b * t_sb
- *   + n / block_size], n < t_cols * block_size.  Entries follow torch's indexing
- *   rules; for one outside the pool that a row needs SLIMKV_STATUS_BAD_PAGE is
+ *   + n / block_size], n < t_cols * block_size and 2^30.  Entries follow torch's
+ *   indexing rules; for one outside the pool that a row needs SLIMKV_STATUS_BAD_PAGE is
  *   stored in *status (optional): that row is not written, reads as zeros, and
  *   makes an attention's results undefined.
  * ---------------------------------------------------------------------- */
@@ -105,7 +105,8 @@ int slimkv_dequantize_rows(const slimkv_dequantize_rows_args* a, void* stream);
  * [B, T, Hq, D], lse [B, Hq, T] fp32 contiguous; query head j reads KV head j /
  * (heads / kv_heads).  A row that sees nothing gives 0 and -inf; what lies behind
  * a sequence's length, or in drafted rows that a query does not see, has no
- * influence.  Softmax weights are rounded to the element type for the product
+ * influence.  Cached rows enter as slimkv_dequantize_rows gives them in this
+ * element type.  Softmax weights are rounded to the element type for the product
  * with V (fp16: held 2^15 times as large); sums and LSE are fp32.
  * Up to 1024 tokens, 256 query heads a KV head, 2^30 keys; scale in [1e-18,
  * 1e18]; drafted rows lie [head_dim, 2^23) elements apart.

@@ -7,8 +7,9 @@
 // MFMA, S^T = K . Q^T, O^T = V^T . P^T with P^T straight from the score registers,
 // and the tiles of all (sequence, KV head) items are dealt to two workgroups a CU in
 // equal runs.  The cached rows come as codes and scales and become MFMA operands
-// in registers, two elements an instruction, exactly (a 4-bit float times a power
-// of two fits the element type):
+// in registers, two elements an instruction, as rows are read back: exactly in bf16,
+// and in fp16 what fp16 wrote (bf16 writes some that fp16 rounds or that pass its
+// end):
 //   K   a lane reads 16 (D = 64: 8) bytes of one row, one block of 32 elements
 //       (half of one), so one scale serves them.  The order of the elements in the
 //       product is free as long as the queries follow it (load_queries GROUPED).

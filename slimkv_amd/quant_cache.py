@@ -208,8 +208,9 @@ def quantized_attention(q, draft_k, draft_v, scale, pages, table=None, *, length
     j]; None is a chain (j <= t).  Every token sees rows 0 .. lengths[b] - 1 of its sequence (lengths [B] int32,
     default and at most `keys`, itself by default all rows the cache has room for).  Returns (out [B, T, Hq, D], lse
     [B, Hq, T] fp32); a row that sees nothing gives 0 and -inf, and what lies in unseen rows has no influence.  The
-    cached rows enter as the values they stand for; rounding is tree_attention's.  (out, lse) of the cache alone merge
-    with another branch by kernels.merge."""
+    cached rows enter as dequantize_rows returns them in the type of q: exact in bf16 and, of what fp16 wrote, in fp16;
+    fp16 rounds numbers below 2^-22 that bf16 wrote and takes those past 65504 as infinities.  All other rounding is
+    tree_attention's.  (out, lse) of the cache alone merge with another branch by kernels.merge."""
     name = 'quantized_attention'
     if q.dim() != 4 or pages.dim() != 3:
         raise ValueError(f'{name}: q must be [B, T, Hq, D] and pages [pages, Hkv, bytes]')

@@ -826,3 +826,52 @@ def test_every_kernel_over_dealt_items(case):
     check_tree(out[pick], lse[pick], q[pick], kc, vc, [lengths[b] for b in pick], dk[pick], dv[pick], mask[pick], D ** -0.5, str(case))
     again, lse2 = call()
     assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize('T', [1, 6, 12, 40])
+@pytest.mark.parametrize('D', [64, 128])
+def test_attention_in_another_type_than_the_writing(T, D):
+    """The cached rows enter as dequantize_rows gives them in the type of q: bf16 exact, fp16 with bf16's smallest numbers
+    rounded and its largest infinite.  check_tree's bounds, for outputs below 2^-14 with half a step of fp16 there, 2^-25."""
+    from oracle import cache as oc
+    from slimkv_amd import quant_cache
+    g, B, N, H = gen(63), 2, 300, 2
+    lengths = [N, 3]
+    for wrote, dt in ((torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16)):
+        k, v = randn(g, B, N, H, D, dtype=wrote), randn(g, B, N, H, D, dtype=wrote)
+        # blocks of 2^-20 to 2^-25, some of whose numbers fp16 rounds
+        v[..., 32:64] = (randn(g, B, N, H, 32).float() * 2.0 ** -(20 + torch.arange(N, device='cuda') % 6)[:, None, None]).to(wrote)
+        pages = quant_cache.new_pages(B, H, 304, D)
+        q, dk, dv = randn(g, B, T, 4, D, dtype=dt, gain=2.0), randn(g, B, T, H, D, dtype=dt), randn(g, B, T, H, D, dtype=dt)
+        dv[..., 32:64] = 0
+        for huge in (False, True):
+            if huge:
+                if wrote is torch.float16:
+                    continue
+                v[1, 2, 1, 5], v[0, 17, 0, 31] = 3e5, -1e30
+            quant_cache.quantize_rows(k, v, pages)
+            rk, rv = quant_cache.dequantize_rows(pages, N, D, dtype=dt)
+            exact = quant_cache.dequantize_rows(pages, N, D, dtype=torch.bfloat16)[1]
+            assert torch.equal(exact.to(dt), rv) and (dt is torch.bfloat16 or not torch.equal(rv.float(), exact.float()))
+            out, lse = quant_cache.quantized_attention(q, dk, dv, D ** -0.5, pages, lengths=ints(lengths))
+            values = to_np(rv)
+            if huge:                                                             # any weight makes an infinity of them
+                assert np.isinf(values[1, 2, 1, 5]) and np.isinf(values[0, 17, 0, 31])
+                got = to_np(out)
+                assert (got[1, :, 2:, 5] == np.inf).all() and (got[0, :, :2, 31] == -np.inf).all()
+                assert np.isfinite(np.delete(got, [5, 31], 3)).all() and np.isfinite(to_np(lse)).all()
+                continue
+            eo, el, terms, top, mass, total = oc.tree_attention(to_np(q), to_np(rk), values, lengths, to_np(dk), to_np(dv), None,
+                                                                D ** -0.5)
+            u = HALF[dt]
+            d = (2.0 ** -24 * (D + 8) * mass + 2.0 ** -22 * (1 + top)).transpose(0, 2, 1)[..., None]
+            tol = (2 * d + u) * terms + u * np.abs(eo) * (1 + u) + 1e-30
+            if dt is torch.float16:
+                tiny = 2.0 ** -25 * (N + T) / total.transpose(0, 2, 1)[..., None]
+                columns = np.abs(values).max((0, 1, 2)).clip(np.abs(to_np(dv)).max((0, 1, 2)))
+                tol = tol + tiny * columns + 2.0 ** -25
+            worst = (np.abs(to_np(out) - eo) / tol).max()
+            print(T, D, dt, 'worst output error over its bound', worst, flush=True)
+            assert worst <= 1.0
+            # the small columns are there, in steps of 2^-24 or finer than their sizes
+            assert (np.abs(eo[..., 32:64]) > 2.0 ** -23).any() and to_np(out)[..., 32:64].any()
