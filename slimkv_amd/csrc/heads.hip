@@ -171,7 +171,12 @@ extern "C" int slimkv_norm_rope(const slimkv_norm_rope_args* a, void* stream) {
     p.status = a->status;
     const int64_t tokens = B * L, round = 1024 / D, rounds = (Hq + Hk + round - 1) / round;
     // Two rounds a wave where that leaves every SIMD several waves (8192 tokens of 48 heads: one round 47.7 us, two
-    // 43.1, three 43.4, four 44.1); past the caches from 64 MB of rows on, twice the L2 (the same call 43.1 / 40.2).
+    // 43.1, three 43.4, four 44.1).  The sides cross near the border: 10240 and 12288 rounds 14.0 / 13.5 and 15.1 / 14.2,
+    // 13108 and 16384 (10 + 2 heads) 15.8 / 16.4 and 17.7 / 18.1, 16385 19.4 / 19.5, 24576 26.4 / 24.0.
+    // Past the caches from 64 MB of rows on, twice the L2 (the same call 43.1 / 40.2).  By itself that is faster below as
+    // well (5 MB 5.0 / 4.6, 48 MB 24.0 / 22.7), but a step writes the rows before and reads them after: with both
+    // (elementwise kernels) 38 MB 51.6 / 54.3, 48 MB 57.1 / 56.8, 64 MB 77.1 / 72.6, 77 MB 89.8 / 84.2, 96 MB 103.7 / 105.7,
+    // 192 MB 217.2 / 217.6, 384 MB 416 / 410.
     p.each = tokens * rounds >= 16384 ? 2 : 1;
     const int64_t chunks = (rounds + p.each - 1) / p.each, workgroups = (tokens * chunks + 3) / 4;
     // keeps tokens, and waves, below 2^31 as well

@@ -20,13 +20,15 @@
 //
 // Up to 32 query rows a KV head the cache's bytes are the bound, 136 a row and head
 // of 128 (quant_few_kernel: 16 sequences of 8-32K rows, a token each, 357 MB in 64
-// us, 5.6 TB/s, the call with its merge 71; a copy moves 5.2).  More rows are bound by
-// the instructions of the softmax and of the conversions beside the products and by
-// the power that they take together (quant_many_kernel: 26 tokens on the same cache 202
-// us a call, 690 TFLOP/s of needed work, 850 with the rows that fill up the last tiles;
-// 63 tokens of 40 heads over 131071 rows 214 us, 790 and 960; the library's 8192^3
-// product reaches 1100-1140).  Figures beside a choice compare its two sides as they
-// were when it was made.
+// us, 5.6 TB/s, the call with its merge 71; a copy moves 5.2, non-temporal reads alone
+// 7.2).  More rows are bound by the instructions of the softmax and of the conversions
+// beside the products and by the power that they take together (quant_many_kernel: 26
+// tokens on the same cache 202 us a call, 690 TFLOP/s of needed work, 850 with the rows
+// that fill up the last tiles; 63 tokens of 40 heads over 131071 rows 214 us, 790 and
+// 960; four windows of 1024 tokens over 32768 rows 2.07 ms, 1080, and over none 140 us,
+// 245, since drafted tiles behind a block's last token are worked on as well; the
+// library's 8192^3 product reaches 1100-1140).  Figures beside a choice compare its two
+// sides as they were when it was made.
 //
 // Not taken: the product that takes 4-bit operands itself
 // (v_mfma_scale_f32_16x16x128_f8f6f4, the queries cut into exact 8-bit parts).  Its
@@ -265,7 +267,9 @@ struct Softmax {
             }
         }
     }
-    // Two weights, rounded to the element type; their sum before that joins `sum`.
+    // Two weights, rounded to the element type, since the matrix instruction takes both operands in it: at most half a step
+    // of sum p |v|, of either sign (16 sequences of 8-32K rows: the outputs' error against 64 bits 0.00167 where the
+    // output's own rounding is 0.00166; six short chains 0.00177 / 0.00165).  Their sum before that joins `sum`.
     __device__ __forceinline__ uint32_t weigh(int nt, float a, float b, float& sum) const {
         const float pa = fast_exp2(__builtin_fmaf(a, factor[nt], -base[nt]));
         const float pb = fast_exp2(__builtin_fmaf(b, factor[nt], -base[nt]));

@@ -282,10 +282,11 @@ def norm_rope(q, k, cos, sin, positions, *, q_weight=None, k_weight=None, eps=1e
 
     q [B, L, Hq, D] and k [B, L, Hkv, D] (None: queries alone), views of a fused projection's output among them;
     weights [D] of their type or float32 (both alike), or None for heads that are not normalised; cos, sin [rows, D]
-    float32 (workloads.rope_tables); positions int64 [B, L] or [1, L].  fp32 throughout and one rounding, where
-    kernels.rope_decode takes the reference's bf16 steps; a normalised head's sum of squares has to lie within fp32.
-    A position outside the tables raises IndexError (or is left in `status`), its token's rows are not written.
-    Returns (out_q, out_k); out_q may be q itself, out_k k."""
+    float32 (workloads.rope_tables), contiguous from a 16-byte boundary (others are copied whole, every call);
+    positions int64 [B, L] or [1, L].  fp32 throughout and one rounding, where kernels.rope_decode takes the reference's
+    bf16 steps; a normalised head's sum of squares has to lie within fp32.  A position outside the tables raises
+    IndexError (or is left in `status`), its token's rows are not written.  Returns (out_q, out_k); out_q may be q itself,
+    out_k k (where q and k are one tensor, neither)."""
     name = 'norm_rope'
     if q.dim() != 4 or q.stride(3) != 1:
         raise ValueError(f'{name}: q must be [B, L, Hq, D] with contiguous features')
